@@ -15,7 +15,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parents[2] / "_lib" / "libgs_raster.so"
-ABI_VERSION = 21
+ABI_VERSION = 22
 
 GS_OK = 0
 GS_ERR_INVALID_ARGUMENT = 1
@@ -25,6 +25,10 @@ GS_ERR_HIP = 4
 GS_ERR_WORKSPACE = 5
 
 MODES = {"gaussian": 0, "ellipsoid": 1}
+
+# gs_type: element types of the sequence operators.
+TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+TYPE_I8, TYPE_E4M3 = 3, 4
 
 
 class GsAdamTensor(ctypes.Structure):
@@ -361,6 +365,34 @@ _SIGNATURES = {
         c_int, [c_void_p, c_int64, c_int32, c_void_p, c_int32, c_int32] + [c_void_p] * 7
     ),
     "gs_ply_pack": (c_int, [c_void_p] * 6 + [c_int64, c_int32, c_void_p, c_void_p]),
+    "gs_add_rms_norm_fwd": (
+        c_int,
+        [c_void_p] * 3 + [c_int64] * 4 + [c_int32] * 3 + [c_float] + [c_void_p] * 4,
+    ),
+    "gs_add_rms_norm_quant": (
+        c_int,
+        [c_void_p] * 3 + [c_int64] * 4 + [c_int32] * 3 + [c_float, c_int32] + [c_void_p] * 4,
+    ),
+    "gs_add_rms_norm_bwd_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "gs_add_rms_norm_bwd": (
+        c_int,
+        [c_void_p] * 5 + [c_int64] * 3 + [c_int32] * 3 + [c_void_p] * 4 + [c_size_t, c_void_p],
+    ),
+    "gs_gated_scan_chunks": (c_int64, [c_int64]),
+    "gs_gated_scan_workspace_bytes": (c_size_t, [c_int64] * 3 + [c_int32]),
+    "gs_gated_scan_fwd": (
+        c_int,
+        [c_void_p] * 3 + [c_int64] * 3 + [c_void_p, c_int32] + [c_void_p] * 4
+        + [c_size_t, c_void_p],
+    ),
+    "gs_gated_scan_bwd": (
+        c_int,
+        [c_void_p] * 5 + [c_int64] * 3 + [c_void_p, c_int32] + [c_void_p] * 4
+        + [c_size_t, c_void_p],
+    ),
+    "gs_gated_scan_step": (
+        c_int, [c_void_p] * 3 + [c_int64] * 2 + [c_int32] + [c_void_p] * 3
+    ),
 }
 
 PLY_MAX_FIELDS = 89

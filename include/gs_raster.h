@@ -42,7 +42,7 @@ extern "C" {
 
 #define GS_API __attribute__((visibility("default")))
 
-#define GS_ABI_VERSION 21
+#define GS_ABI_VERSION 22
 
 typedef enum gs_status {
   GS_OK = 0,
@@ -631,6 +631,84 @@ GS_API int gs_ply_pack(
     const float* mean, const float* normals, const float* rotation,
     const float* scale, const float* opacity, const float* color, int64_t n,
     int32_t sh_coeffs, void* records, void* stream);
+
+/* ---- Sequence operators ---------------------------------------------------
+ * The blocks of a network that predicts splats from a stream of posed views:
+ * norm, recurrence and attention over its tokens.  Tensors are row-major with
+ * the innermost dimension contiguous; strides are in elements. */
+typedef enum gs_type {
+  GS_F32 = 0,
+  GS_F16 = 1,
+  GS_BF16 = 2,
+  GS_I8 = 3,
+  GS_E4M3 = 4 /* 8-bit float, 4 exponent bits, no infinities, largest 448 */
+} gs_type;
+
+/* Root-mean-square norm with the residual's addition, per row of
+ * [rows, width]: s = x + residual, y = s / sqrt(mean(s^2) + eps) * weight.
+ * Writes y in x's type, s rounded to the residual's (sum; with a NULL residual
+ * s is x and sum is not written) and 1 / sqrt(...) of each row (inverse_rms,
+ * may be NULL).  x and residual rows lie x_stride and residual_stride apart (0
+ * repeats a row); outputs are contiguous.  The residual and the weight have
+ * x's type or GS_F32 (GS_ERR_UNSUPPORTED otherwise). */
+GS_API int gs_add_rms_norm_fwd(
+    const void* x, const void* residual, const void* weight, int64_t rows,
+    int64_t width, int64_t x_stride, int64_t residual_stride, int32_t x_type,
+    int32_t residual_type, int32_t weight_type, float eps, void* y, void* sum,
+    float* inverse_rms, void* stream);
+
+/* The same with y as 8-bit codes (code_type GS_I8 or GS_E4M3) and one scale
+ * per row: scale = max|y| / 127 or / 448, code = y / scale rounded to nearest
+ * even.  A row of zeros has scale 0; a NaN in a row makes its scale NaN. */
+GS_API int gs_add_rms_norm_quant(
+    const void* x, const void* residual, const void* weight, int64_t rows,
+    int64_t width, int64_t x_stride, int64_t residual_stride, int32_t x_type,
+    int32_t residual_type, int32_t weight_type, float eps, int32_t code_type,
+    void* codes, float* scales, void* sum, void* stream);
+
+/* Gradients of gs_add_rms_norm_fwd from its sum (x itself where there was no
+ * residual; rows sum_stride apart) and inverse_rms.  grad_y (x's type) and
+ * grad_sum (the residual's) are contiguous, NULL for zeros.  grad_x,
+ * grad_residual and grad_weight are each written unless NULL; grad_weight
+ * needs the workspace and does not depend on the schedule. */
+GS_API size_t gs_add_rms_norm_bwd_workspace_bytes(int64_t rows, int64_t width);
+GS_API int gs_add_rms_norm_bwd(
+    const void* sum, const void* weight, const float* inverse_rms,
+    const void* grad_y, const void* grad_sum, int64_t rows, int64_t width,
+    int64_t sum_stride, int32_t x_type, int32_t residual_type,
+    int32_t weight_type, void* grad_x, void* grad_residual, void* grad_weight,
+    void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gated linear recurrence over the tokens of [batch, tokens, channels]:
+ * a = sigmoid(gate), h_t = a_t h_{t-1} + (1 - a_t) x_t, h_0 = state (float32
+ * [batch, channels], NULL for zeros), h in float32.  Writes y = h in x's type
+ * (contiguous), last = h of the last token (float32 [batch, channels]) and
+ * starts, h before each of the gs_gated_scan_chunks(tokens) chunks (float32
+ * [batch, chunks, channels]), which the backward reads.  strides, host memory:
+ * x's batch and token stride, gate's batch and token stride (the backward:
+ * grad_y's after them).  gs_gated_scan_bwd writes the gradients of x, gate
+ * and, unless NULL, state; grad_y NULL and grad_last NULL stand for zeros.
+ * The results do not depend on the schedule.  With no token nothing is
+ * written. */
+GS_API int64_t gs_gated_scan_chunks(int64_t tokens);
+GS_API size_t gs_gated_scan_workspace_bytes(
+    int64_t batch, int64_t tokens, int64_t channels, int32_t backward);
+GS_API int gs_gated_scan_fwd(
+    const void* x, const void* gate, const float* state, int64_t batch,
+    int64_t tokens, int64_t channels, const int64_t* strides, int32_t type,
+    void* y, float* last, float* starts, void* workspace,
+    size_t workspace_bytes, void* stream);
+GS_API int gs_gated_scan_bwd(
+    const void* x, const void* gate, const float* starts, const void* grad_y,
+    const float* grad_last, int64_t batch, int64_t tokens, int64_t channels,
+    const int64_t* strides, int32_t type, void* grad_x, void* grad_gate,
+    float* grad_state, void* workspace, size_t workspace_bytes, void* stream);
+
+/* One token of the recurrence: all tensors contiguous [batch, channels];
+ * state_out may be state. */
+GS_API int gs_gated_scan_step(
+    const void* x, const void* gate, const float* state, int64_t batch,
+    int64_t channels, int32_t type, void* y, float* state_out, void* stream);
 
 #ifdef __cplusplus
 }
