@@ -1,0 +1,525 @@
+// Attention with a sliding window and visible first tokens, backward.  With
+// P_ij = exp(scale q_i . k_j - lse_i) where query i sees key j and 0 elsewhere,
+//   delta_i = sum_d grad_out_i out_i,   dP = grad_out V^T,   dS = P (dP - delta),
+//   grad_v = P^T grad_out,   grad_q = scale dS K,   grad_k = scale dS^T Q.
+// P is computed again from q, k and lse instead of being kept.
+//
+// Two kernels: one holds a workgroup's keys and walks the queries that see them
+// (grad_k, grad_v), one holds queries and walks the keys that they see
+// (grad_q).  P and dP are computed twice, 7 products for 5, and in return every
+// gradient is added up in registers in a fixed order: no atomics.  Heads that
+// share keys are walked one after the other by their keys' workgroup.
+//
+// The first tokens are seen by every later query.  Their keys' walk, far longer
+// than a window, is cut into segments of about a window's length, each a
+// workgroup of its own that leaves float32 sums, which a last kernel adds in the
+// order of the segments.
+#include "attention_tile.h"
+
+namespace gs {
+namespace {
+
+using namespace att;
+
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * kWave;
+constexpr int kBlockKeys = 32 * kWaves;     // keys of a workgroup of the first kernel
+constexpr int kBlockQueries = 32 * kWaves;  // queries of one of the second
+
+// Rows of the tiles that are walked: halved for float32 to leave registers.
+template <typename T, int kDim>
+constexpr int kTileRows = sizeof(T) == 2 ? 64 : 32;
+
+struct BackwardArgs {
+  Problem p;
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* out;
+  const void* grad;
+  Strides sq, sk, sv, sg;
+  const float* lse;
+  float* delta;  // [batch, heads, queries]
+  void* dq;
+  void* dk;
+  void* dv;
+  // Segments of the workgroups whose keys hold first tokens.
+  float* parts;  // [batch, kv_heads, sink_blocks, segments, 2, kBlockKeys, dim]
+  int sink_blocks, segments, segment;  // segment: queries of one
+};
+
+// delta, a group of 16 lanes for each row.
+template <typename T>
+__global__ __launch_bounds__(256) void attention_delta_kernel(BackwardArgs a) {
+  const Problem& p = a.p;
+  const int64_t rows = int64_t(p.batch) * p.queries * p.heads;
+  const int64_t row = int64_t(blockIdx.x) * 16 + (threadIdx.x >> 4);
+  const int d = (threadIdx.x & 15) * 8;
+  float sum = 0.0f;
+  const int head = int(row % p.heads);
+  const int64_t i = row / p.heads % p.queries, b = row / p.heads / p.queries;
+  if (row < rows && d < p.dim) {
+    const Frag<T> o = load_global<T>(static_cast<const T*>(a.out) + row * p.dim + d, true);
+    const Frag<T> g = load_global<T>(static_cast<const T*>(a.grad) + b * a.sg.batch +
+                                         i * a.sg.token + head * a.sg.head + d, true);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += float(o[e]) * float(g[e]);
+  }
+#pragma unroll
+  for (int s = 8; s > 0; s >>= 1) sum += __shfl_xor(sum, s, 64);
+  if (row < rows && (threadIdx.x & 15) == 0) a.delta[(b * p.heads + head) * p.queries + i] = sum;
+}
+
+// grad_k and grad_v of a workgroup's keys: a wave holds 32, queries walk by.
+template <typename T, int kDim>
+__global__ __launch_bounds__(kThreads) void attention_bwd_keys_kernel(BackwardArgs a) {
+  constexpr int kRows = kTileRows<T, kDim>;
+  constexpr int kPitchT = kPitch<T, kDim>;
+  constexpr int kSteps = kDim / 16, kBlocks = kDim / 32;
+  __shared__ __align__(16) T tiles[2][2][kRows * kPitchT];
+  __shared__ float rows[2][2][kRows];  // lse (in powers of two) and delta
+  const Problem& p = a.p;
+  const int blocks = (p.keys + kBlockKeys - 1) / kBlockKeys;
+  // Workgroups of a key head: the segments of the first tokens' blocks, then
+  // the other blocks.
+  const int split = a.sink_blocks * a.segments;
+  const int per = split + blocks - a.sink_blocks;
+  const int64_t total = int64_t(per) * p.kv_heads * p.batch;
+  const int64_t id = xcd_order(blockIdx.x, total);
+  if (id >= total) return;
+  const int item = int(id % per);
+  const int kv = int(id / per % p.kv_heads), b = int(id / per / p.kv_heads);
+  const bool part = item < split;
+  const int block = part ? item / a.segments : item - split + a.sink_blocks;
+  const int segment = part ? item % a.segments : 0;
+  const int group = p.heads / p.kv_heads;
+  const int length = p.length(b);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int k0 = block * kBlockKeys;  // first key of the workgroup
+  const int w0 = k0 + wave * 32;      // of the wave
+  const int j = w0 + (lane & 31);     // the lane's
+
+  Frag<T> kf[kSteps], vf[kSteps];
+  {
+    const T* kr = static_cast<const T*>(a.k) + b * a.sk.batch + j * a.sk.token + kv * a.sk.head;
+    const T* vr = static_cast<const T*>(a.v) + b * a.sv.batch + j * a.sv.token + kv * a.sv.head;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int d = 16 * s + 8 * (lane >> 5);
+      kf[s] = load_global<T>(kr + d, j < length && d < p.dim);
+      vf[s] = load_global<T>(vr + d, j < length && d < p.dim);
+    }
+  }
+
+  // Queries that see any of the keys, cut to the segment.
+  const int off = p.offset();
+  int from = max(0, k0 - off);
+  int to = k0 < p.sinks ? p.queries
+                        : int(min(int64_t(p.queries), int64_t(k0) + kBlockKeys - 1 + p.window - off));
+  if (part) {
+    from = max(from, segment * a.segment);
+    to = min(p.queries, (segment + 1) * a.segment);
+  }
+  if (k0 >= length) to = from;
+  const int first_tile = from / kRows;
+  const int tiles_per_head = to > from ? (to - 1) / kRows - first_tile + 1 : 0;
+  const int count = tiles_per_head * group;
+
+  Acc dk[kBlocks], dv[kBlocks];
+#pragma unroll
+  for (int n = 0; n < kBlocks; ++n) dk[n] = dv[n] = Acc(0.0f);
+  const float c = p.scale * kLog2e;
+
+  Stage<T, kRows, kDim, kThreads> sq, sg;
+  float row_lse = 0.0f, row_delta = 0.0f;
+  const auto fetch = [&](int it) {
+    const int head = kv * group + it / tiles_per_head;
+    const int i0 = (first_tile + it % tiles_per_head) * kRows;
+    sq.load(static_cast<const T*>(a.q) + b * a.sq.batch + head * a.sq.head, a.sq.token, i0,
+            p.queries, p.dim);
+    sg.load(static_cast<const T*>(a.grad) + b * a.sg.batch + head * a.sg.head, a.sg.token, i0,
+            p.queries, p.dim);
+    if (threadIdx.x < kRows) {
+      const int i = i0 + threadIdx.x;
+      const int64_t at = (int64_t(b) * p.heads + head) * p.queries + i;
+      row_lse = i < p.queries ? a.lse[at] * kLog2e : 0.0f;
+      row_delta = i < p.queries ? a.delta[at] : 0.0f;
+    }
+  };
+  const auto keep = [&](int buffer) {
+    sq.store(tiles[buffer][0]);
+    sg.store(tiles[buffer][1]);
+    if (threadIdx.x < kRows) {
+      rows[buffer][0][threadIdx.x] = row_lse;
+      rows[buffer][1][threadIdx.x] = row_delta;
+    }
+  };
+  if (count > 0) {
+    fetch(0);
+    keep(0);
+  }
+  __syncthreads();
+  for (int it = 0; it < count; ++it) {
+    if (it + 1 < count) fetch(it + 1);
+    const T* qt = tiles[it & 1][0];
+    const T* gt = tiles[it & 1][1];
+    const int i0 = (first_tile + it % tiles_per_head) * kRows;
+#pragma unroll
+    for (int h = 0; h < kRows / 32; ++h) {
+      const int p0 = off + i0 + 32 * h, p1 = p0 + 31;  // positions
+      // Queries outside [from, to) belong to other segments.
+      const bool inside = i0 + 32 * h >= from && i0 + 32 * h + 31 < to;
+      const bool any = w0 <= p1 && w0 < length && i0 + 32 * h < to &&
+                       (w0 + 31 > p0 - p.window || w0 < p.sinks);
+      const bool all = inside && w0 + 31 <= p0 && w0 + 31 < length &&
+                       (w0 > p1 - p.window || w0 + 31 < p.sinks);
+      if (!any) continue;
+      const auto seen = [&](int row) {  // row of the 32: query i0 + 32 h + row, key j
+        const int i = i0 + 32 * h + row;
+        return i >= from && i < to && p.sees(off + i, j, length);
+      };
+      Acc s(0.0f), dp(0.0f);
+#pragma unroll
+      for (int st = 0; st < kSteps; ++st) mma(load_rows<T>(qt, kPitchT, 32 * h, 16 * st), kf[st], s);
+#pragma unroll
+      for (int st = 0; st < kSteps; ++st) mma(load_rows<T>(gt, kPitchT, 32 * h, 16 * st), vf[st], dp);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int row = 32 * h + acc_row(r);
+        const float lse = rows[it & 1][0][row], delta = rows[it & 1][1][row];
+        s[r] = power<T>(s[r] * c - lse);
+        dp[r] = s[r] * (dp[r] - delta);
+      }
+      if (!all) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const bool see = seen(acc_row(r));
+          s[r] = see ? s[r] : 0.0f;
+          dp[r] = see ? dp[r] : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        const Frag<T> pf = acc_frag<T>(s, st), df = acc_frag<T>(dp, st);
+        Frag<T> f[kBlocks];
+#pragma unroll
+        for (int n = 0; n < kBlocks; ++n) f[n] = load_turned<T>(gt, kPitchT, 32 * h + 16 * st, 32 * n);
+        if (all) {
+#pragma unroll
+          for (int n = 0; n < kBlocks; ++n) mma(f[n], pf, dv[n]);
+        } else {
+          mma_seen<T>(f, pf, dv, [&](int e) { return seen(16 * st + e); });
+        }
+#pragma unroll
+        for (int n = 0; n < kBlocks; ++n) f[n] = load_turned<T>(qt, kPitchT, 32 * h + 16 * st, 32 * n);
+        if (all) {
+#pragma unroll
+          for (int n = 0; n < kBlocks; ++n) mma(f[n], df, dk[n]);
+        } else {
+          mma_seen<T>(f, df, dk, [&](int e) { return seen(16 * st + e); });
+        }
+      }
+    }
+    if (it + 1 < count) keep((it + 1) & 1);
+    __syncthreads();
+  }
+  if (part) {
+    float* at = a.parts + ((((int64_t(b) * p.kv_heads + kv) * a.sink_blocks + block) * a.segments +
+                            segment) * 2 * kBlockKeys + wave * 32 + (lane & 31)) * p.dim;
+#pragma unroll
+    for (int n = 0; n < kBlocks; ++n)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = 32 * n + 8 * g + 4 * (lane >> 5);
+        if (d >= p.dim) continue;
+        FloatVec<4> x, y;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          x[r] = dk[n][4 * g + r];
+          y[r] = dv[n][4 * g + r];
+        }
+        *reinterpret_cast<FloatVec<4>*>(at + d) = x;
+        *reinterpret_cast<FloatVec<4>*>(at + kBlockKeys * p.dim + d) = y;
+      }
+    return;
+  }
+  if (j >= p.keys) return;
+  const int64_t row = ((int64_t(b) * p.keys + j) * p.kv_heads + kv) * p.dim;
+#pragma unroll
+  for (int n = 0; n < kBlocks; ++n)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = 32 * n + 8 * g + 4 * (lane >> 5);
+      if (d >= p.dim) continue;
+      FloatVec<4> x, y;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        x[r] = dk[n][4 * g + r] * p.scale;
+        y[r] = dv[n][4 * g + r];
+      }
+      *reinterpret_cast<Vec<T, 4>*>(static_cast<T*>(a.dk) + row + d) = from_float<T, 4>(x);
+      *reinterpret_cast<Vec<T, 4>*>(static_cast<T*>(a.dv) + row + d) = from_float<T, 4>(y);
+    }
+}
+
+// The first tokens' blocks: their segments' sums in order.  One thread for each
+// element of [batch, kv_heads, sink_blocks, kBlockKeys, dim].
+template <typename T>
+__global__ __launch_bounds__(256) void attention_bwd_join_kernel(BackwardArgs a) {
+  const Problem& p = a.p;
+  const int64_t plane = int64_t(kBlockKeys) * p.dim;
+  const int64_t e = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (e >= int64_t(p.batch) * p.kv_heads * a.sink_blocks * plane) return;
+  const int64_t block = e / plane, in = e % plane;
+  const int j = int(block % a.sink_blocks) * kBlockKeys + int(in / p.dim);
+  if (j >= p.keys) return;
+  const int64_t kv = block / a.sink_blocks % p.kv_heads, b = block / a.sink_blocks / p.kv_heads;
+  const float* at = a.parts + block * a.segments * 2 * plane + in;
+  float dk = 0.0f, dv = 0.0f;
+  for (int s = 0; s < a.segments; ++s) {
+    dk += at[2 * s * plane];
+    dv += at[(2 * s + 1) * plane];
+  }
+  const int64_t row = ((b * p.keys + j) * p.kv_heads + kv) * p.dim + in % p.dim;
+  static_cast<T*>(a.dk)[row] = T(dk * p.scale);
+  static_cast<T*>(a.dv)[row] = T(dv);
+}
+
+// grad_q of a workgroup's queries: a wave holds 32, the keys that they see walk by.
+template <typename T, int kDim>
+__global__ __launch_bounds__(kThreads) void attention_bwd_queries_kernel(BackwardArgs a) {
+  constexpr int kRows = kTileRows<T, kDim>;
+  constexpr int kPitchT = kPitch<T, kDim>;
+  constexpr int kSteps = kDim / 16, kBlocks = kDim / 32;
+  __shared__ __align__(16) T tiles[2][2][kRows * kPitchT];
+  const Problem& p = a.p;
+  const int blocks = (p.queries + kBlockQueries - 1) / kBlockQueries;
+  const int64_t total = int64_t(blocks) * p.heads * p.batch;
+  const int64_t id = xcd_order(blockIdx.x, total);
+  if (id >= total) return;
+  const int group = p.heads / p.kv_heads;
+  const int of = int(id % group);
+  const int block = int(id / group % blocks);
+  const int kv = int(id / group / blocks % p.kv_heads);
+  const int b = int(id / group / blocks / p.kv_heads);
+  const int head = kv * group + of;
+  const int length = p.length(b);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int i = block * kBlockQueries + wave * 32 + (lane & 31);
+  const int pos = p.offset() + i;
+  const bool live = i < p.queries;
+  Frag<T> q[kSteps], g[kSteps];
+  {
+    const T* qr = static_cast<const T*>(a.q) + b * a.sq.batch + i * a.sq.token + head * a.sq.head;
+    const T* gr = static_cast<const T*>(a.grad) + b * a.sg.batch + i * a.sg.token + head * a.sg.head;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int d = 16 * s + 8 * (lane >> 5);
+      q[s] = load_global<T>(qr + d, live && d < p.dim);
+      g[s] = load_global<T>(gr + d, live && d < p.dim);
+    }
+  }
+  const int64_t at = (int64_t(b) * p.heads + head) * p.queries + i;
+  const float lse = live ? a.lse[at] * kLog2e : 0.0f, delta = live ? a.delta[at] : 0.0f;
+
+  const int first = p.offset() + block * kBlockQueries;
+  const int last = min(p.offset() + min((block + 1) * kBlockQueries, p.queries), length) - 1;
+  int tail = max(0, first - p.window + 1) / kRows;
+  const int head_tiles = min((min(p.sinks, last + 1) + kRows - 1) / kRows, tail);
+  const int count = last < 0 ? 0 : head_tiles + max(0, last / kRows - tail + 1);
+  tail -= head_tiles;
+  const int wave_first = first + wave * 32, wave_last = wave_first + 31;
+  const float c = p.scale * kLog2e;
+  Acc dq[kBlocks];
+#pragma unroll
+  for (int n = 0; n < kBlocks; ++n) dq[n] = Acc(0.0f);
+
+  const T* kbase = static_cast<const T*>(a.k) + b * a.sk.batch + kv * a.sk.head;
+  const T* vbase = static_cast<const T*>(a.v) + b * a.sv.batch + kv * a.sv.head;
+  Stage<T, kRows, kDim, kThreads> sk, sv;
+  const auto fetch = [&](int it) {
+    const int j0 = (it < head_tiles ? it : tail + it) * kRows;
+    sk.load(kbase, a.sk.token, j0, length, p.dim);
+    sv.load(vbase, a.sv.token, j0, length, p.dim);
+  };
+  if (count > 0) {
+    fetch(0);
+    sk.store(tiles[0][0]);
+    sv.store(tiles[0][1]);
+  }
+  __syncthreads();
+  for (int it = 0; it < count; ++it) {
+    if (it + 1 < count) fetch(it + 1);
+    const T* kt = tiles[it & 1][0];
+    const T* vt = tiles[it & 1][1];
+#pragma unroll
+    for (int h = 0; h < kRows / 32; ++h) {
+      const int j0 = (it < head_tiles ? it : tail + it) * kRows + 32 * h, j1 = j0 + 31;
+      const bool any = j0 <= wave_last && j0 < length && (j1 > wave_first - p.window || j0 < p.sinks);
+      const bool all = j1 <= wave_first && j1 < length && (j0 > wave_last - p.window || j1 < p.sinks);
+      if (!any) continue;
+      Acc s(0.0f), dp(0.0f);
+#pragma unroll
+      for (int st = 0; st < kSteps; ++st) mma(load_rows<T>(kt, kPitchT, 32 * h, 16 * st), q[st], s);
+#pragma unroll
+      for (int st = 0; st < kSteps; ++st) mma(load_rows<T>(vt, kPitchT, 32 * h, 16 * st), g[st], dp);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dp[r] = power<T>(s[r] * c - lse) * (dp[r] - delta);
+      if (!all) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (!p.sees(pos, j0 + acc_row(r), length)) dp[r] = 0.0f;
+      }
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        const Frag<T> df = acc_frag<T>(dp, st);
+        Frag<T> f[kBlocks];
+#pragma unroll
+        for (int n = 0; n < kBlocks; ++n) f[n] = load_turned<T>(kt, kPitchT, 32 * h + 16 * st, 32 * n);
+        if (all) {
+#pragma unroll
+          for (int n = 0; n < kBlocks; ++n) mma(f[n], df, dq[n]);
+        } else {
+          mma_seen<T>(f, df, dq, [&](int e) { return p.sees(pos, j0 + 16 * st + e, length); });
+        }
+      }
+    }
+    if (it + 1 < count) {
+      sk.store(tiles[(it + 1) & 1][0]);
+      sv.store(tiles[(it + 1) & 1][1]);
+    }
+    __syncthreads();
+  }
+  if (!live) return;
+  T* out = static_cast<T*>(a.dq) + ((int64_t(b) * p.queries + i) * p.heads + head) * p.dim;
+#pragma unroll
+  for (int n = 0; n < kBlocks; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = 32 * n + 8 * e + 4 * (lane >> 5);
+      FloatVec<4> x;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = dq[n][4 * e + r] * p.scale;
+      if (d < p.dim) *reinterpret_cast<Vec<T, 4>*>(out + d) = from_float<T, 4>(x);
+    }
+}
+
+// How the first tokens' walk is cut: segments of about as many queries as
+// another workgroup walks.
+void plan_segments(const Problem& p, BackwardArgs& a) {
+  const int blocks = (p.keys + kBlockKeys - 1) / kBlockKeys;
+  a.sink_blocks = std::min(blocks, (p.sinks + kBlockKeys - 1) / kBlockKeys);
+  // Segments start at a tile's first query.
+  a.segment = (p.window + kBlockKeys + 63) / 64 * 64;
+  a.segments = (p.queries + a.segment - 1) / a.segment;
+  if (a.segments <= 1) a.sink_blocks = 0;
+}
+
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+
+size_t delta_bytes(const Problem& p) {
+  return align256(size_t(p.batch) * size_t(p.heads) * size_t(p.queries) * sizeof(float));
+}
+
+}  // namespace
+}  // namespace gs
+
+using namespace gs;
+
+extern "C" GS_API size_t gs_window_attention_bwd_workspace_bytes(const gs_attention* desc) {
+  if (!desc || check_attention(*desc) != GS_OK) return 0;
+  const Problem p = make_problem(*desc, nullptr);
+  BackwardArgs a{};
+  plan_segments(p, a);
+  return delta_bytes(p) + size_t(p.batch) * size_t(p.kv_heads) * size_t(a.sink_blocks) *
+                              size_t(a.segments) * 2 * kBlockKeys * size_t(p.dim) * sizeof(float);
+}
+
+extern "C" GS_API int gs_window_attention_bwd(const gs_attention* desc, const void* q,
+                                              const void* k, const void* v, const void* out,
+                                              const float* lse, const void* grad_out,
+                                              const int64_t* strides, const int32_t* lengths,
+                                              void* grad_q, void* grad_k, void* grad_v,
+                                              void* workspace, size_t workspace_bytes,
+                                              void* stream) {
+  clear_error();
+  GS_REQUIRE(desc, GS_ERR_INVALID_ARGUMENT, "null description");
+  GS_TRY(check_attention(*desc));
+  if (desc->batch == 0 || (desc->queries == 0 && desc->keys == 0)) return GS_OK;
+  GS_REQUIRE(strides, GS_ERR_INVALID_ARGUMENT, "null strides");
+  const int64_t none[3] = {0, 0, 0};
+  if (desc->queries > 0) {
+    GS_TRY(check_rows(q, strides, desc->type, "q"));
+    GS_TRY(check_rows(grad_out, strides + 9, desc->type, "grad_out"));
+    GS_TRY(check_rows(out, none, desc->type, "out"));
+    GS_TRY(check_rows(grad_q, none, desc->type, "grad_q"));
+    GS_REQUIRE(lse, GS_ERR_INVALID_ARGUMENT, "null lse");
+  }
+  if (desc->keys > 0) {
+    GS_TRY(check_rows(k, strides + 3, desc->type, "k"));
+    GS_TRY(check_rows(v, strides + 6, desc->type, "v"));
+    GS_TRY(check_rows(grad_k, none, desc->type, "grad_k"));
+    GS_TRY(check_rows(grad_v, none, desc->type, "grad_v"));
+  }
+  const size_t need = gs_window_attention_bwd_workspace_bytes(desc);
+  GS_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), GS_ERR_WORKSPACE,
+             "workspace too small: %zu bytes, %zu needed", workspace_bytes, need);
+  GS_REQUIRE(seq::aligned_to(workspace, 16), GS_ERR_INVALID_ARGUMENT,
+             "workspace must be 16-byte aligned");
+  BackwardArgs a{};
+  a.p = make_problem(*desc, lengths);
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.out = out;
+  a.grad = grad_out;
+  a.sq = {strides[0], strides[1], strides[2]};
+  a.sk = {strides[3], strides[4], strides[5]};
+  a.sv = {strides[6], strides[7], strides[8]};
+  a.sg = {strides[9], strides[10], strides[11]};
+  a.lse = lse;
+  a.delta = static_cast<float*>(workspace);
+  a.dq = grad_q;
+  a.dk = grad_k;
+  a.dv = grad_v;
+  plan_segments(a.p, a);
+  a.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes(a.p));
+  const Problem& p = a.p;
+  const int64_t rows = int64_t(p.batch) * p.queries * p.heads;
+  const int64_t key_items = (int64_t(p.keys + kBlockKeys - 1) / kBlockKeys - a.sink_blocks +
+                             int64_t(a.sink_blocks) * a.segments) * p.kv_heads * p.batch;
+  const int64_t query_items =
+      int64_t(p.queries + kBlockQueries - 1) / kBlockQueries * p.heads * p.batch;
+  const int64_t joined = int64_t(p.batch) * p.kv_heads * a.sink_blocks * kBlockKeys * p.dim;
+  GS_REQUIRE(rows / 16 < (int64_t(1) << 30) && key_items < (int64_t(1) << 30) &&
+                 query_items < (int64_t(1) << 30) && joined / 256 < (int64_t(1) << 30),
+             GS_ERR_OVERFLOW, "attention problem too large");
+  const hipStream_t s = as_stream(stream);
+  return seq::with_type(desc->type, [&](auto t) {
+    using T = decltype(t);
+    if (rows) {
+      attention_delta_kernel<T><<<unsigned((rows + 15) / 16), 256, 0, s>>>(a);
+      GS_TRY(check_launch("window_attention backward"));
+    }
+    if (key_items) {
+      const unsigned grid = unsigned(xcd_grid(key_items));
+      if (p.dim <= 64)
+        attention_bwd_keys_kernel<T, 64><<<grid, kThreads, 0, s>>>(a);
+      else
+        attention_bwd_keys_kernel<T, 128><<<grid, kThreads, 0, s>>>(a);
+      GS_TRY(check_launch("window_attention backward, keys"));
+    }
+    if (joined) {
+      attention_bwd_join_kernel<T><<<unsigned((joined + 255) / 256), 256, 0, s>>>(a);
+      GS_TRY(check_launch("window_attention backward, first tokens"));
+    }
+    if (query_items) {
+      const unsigned grid = unsigned(xcd_grid(query_items));
+      if (p.dim <= 64)
+        attention_bwd_queries_kernel<T, 64><<<grid, kThreads, 0, s>>>(a);
+      else
+        attention_bwd_queries_kernel<T, 128><<<grid, kThreads, 0, s>>>(a);
+    }
+    return check_launch("window_attention backward, queries");
+  });
+}

@@ -46,6 +46,21 @@ class GsAdamTensor(ctypes.Structure):
 ADAM_MAX_TENSORS = 8
 
 
+class GsAttention(ctypes.Structure):
+    _fields_ = [
+        ("batch", c_int64),
+        ("queries", c_int64),
+        ("keys", c_int64),
+        ("window", c_int64),
+        ("sinks", c_int64),
+        ("heads", c_int32),
+        ("kv_heads", c_int32),
+        ("head_dim", c_int32),
+        ("type", c_int32),
+        ("scale", c_float),
+    ]
+
+
 class GsView(ctypes.Structure):
     _fields_ = [
         ("fx", c_float),
@@ -393,6 +408,11 @@ _SIGNATURES = {
     "gs_gated_scan_step": (
         c_int, [c_void_p] * 3 + [c_int64] * 2 + [c_int32] + [c_void_p] * 3
     ),
+    "gs_window_attention_fwd": (c_int, [c_void_p] * 9),
+    "gs_window_attention_bwd_workspace_bytes": (c_size_t, [c_void_p]),
+    "gs_window_attention_bwd": (c_int, [c_void_p] * 13 + [c_size_t, c_void_p]),
+    "gs_window_attention_step_workspace_bytes": (c_size_t, [c_void_p]),
+    "gs_window_attention_step": (c_int, [c_void_p] * 10 + [c_size_t, c_void_p]),
 }
 
 PLY_MAX_FIELDS = 89

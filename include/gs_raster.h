@@ -710,6 +710,64 @@ GS_API int gs_gated_scan_step(
     const void* x, const void* gate, const float* state, int64_t batch,
     int64_t channels, int32_t type, void* y, float* state_out, void* stream);
 
+/* Attention with a sliding window and visible first tokens.  q [batch,
+ * queries, heads, head_dim], k and v [batch, keys, kv_heads, head_dim], heads a
+ * multiple of kv_heads (head h reads key head h * kv_heads / heads).  Query i
+ * stands at position p = keys - queries + i and sees key j when j <= p and
+ * (j > p - window or j < sinks) and j < lengths[b] (int32, device memory; NULL:
+ * all keys).  A query that sees no key gets zeros; values at places that a query
+ * does not see, infinities and NaN among them, do not reach it.  head_dim is a
+ * multiple of 8 up to 128; window > 0 (at or above keys: none), sinks >= 0,
+ * scale > 0.  type is that of all tensors. */
+typedef struct gs_attention {
+  int64_t batch;
+  int64_t queries;
+  int64_t keys;
+  int64_t window;
+  int64_t sinks;
+  int32_t heads;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t type;
+  float scale;
+} gs_attention;
+
+/* strides, host memory: batch, token and head stride of q, of k and of v;
+ * rows start on 16-byte boundaries.  Writes out [batch, queries, heads,
+ * head_dim] and lse, the logarithm of each softmax's sum (float32 [batch,
+ * heads, queries]; -inf where a query sees no key). */
+GS_API int gs_window_attention_fwd(
+    const gs_attention* attention, const void* q, const void* k, const void* v,
+    const int64_t* strides, const int32_t* lengths, void* out, float* lse,
+    void* stream);
+
+/* Gradients of q, k and v (contiguous, shaped like them; those of shared key
+ * heads summed over their queries' heads) from the forward's out and lse and
+ * from grad_out; strides: those of q, k, v and grad_out.  The results do not
+ * depend on the schedule. */
+GS_API size_t gs_window_attention_bwd_workspace_bytes(const gs_attention* attention);
+GS_API int gs_window_attention_bwd(
+    const gs_attention* attention, const void* q, const void* k, const void* v,
+    const void* out, const float* lse, const void* grad_out,
+    const int64_t* strides, const int32_t* lengths, void* grad_q, void* grad_k,
+    void* grad_v, void* workspace, size_t workspace_bytes, void* stream);
+
+/* One token of each of `batch` streams (queries = 1; keys is not read).  The
+ * caches k_cache and v_cache [batch, sinks + window, kv_heads, head_dim] hold
+ * the first `sinks` tokens and a ring of the last `window` ones: the token at
+ * position p has slot p, from `sinks` on sinks + (p - sinks) mod window.  Writes
+ * k and v [batch, kv_heads, head_dim] to the slot of positions[b] (int32, device
+ * memory) and attends from q [batch, heads, head_dim] to the slots that are
+ * filled, its own among them; a stream at a negative position is left alone and
+ * gets zeros.  strides: batch, token and head stride of k_cache and of v_cache;
+ * q, k, v and out are contiguous. */
+GS_API size_t gs_window_attention_step_workspace_bytes(const gs_attention* attention);
+GS_API int gs_window_attention_step(
+    const gs_attention* attention, const void* q, const void* k, const void* v,
+    void* k_cache, void* v_cache, const int64_t* strides,
+    const int32_t* positions, void* out, void* workspace,
+    size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
