@@ -34,7 +34,7 @@ constexpr int kQueries = 32 * kWaves;  // of a workgroup
 constexpr int kKeys = 64;              // of a tile
 
 template <typename T, int kDim>
-__global__ __launch_bounds__(kThreads) void attention_fwd_kernel(ForwardArgs a) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fwd_kernel(ForwardArgs a) {
   constexpr int kPitchT = kPitch<T, kDim>;
   constexpr int kSteps = kDim / 16, kBlocks = kDim / 32;
   __shared__ __align__(16) T tiles[2][2][kKeys * kPitchT];

@@ -72,7 +72,7 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(BackwardArgs a) {
 
 // grad_k and grad_v of a workgroup's keys: a wave holds 32, queries walk by.
 template <typename T, int kDim>
-__global__ __launch_bounds__(kThreads) void attention_bwd_keys_kernel(BackwardArgs a) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) void attention_bwd_keys_kernel(BackwardArgs a) {
   constexpr int kRows = kTileRows<T, kDim>;
   constexpr int kPitchT = kPitch<T, kDim>;
   constexpr int kSteps = kDim / 16, kBlocks = kDim / 32;
@@ -287,7 +287,7 @@ __global__ __launch_bounds__(256) void attention_bwd_join_kernel(BackwardArgs a)
 
 // grad_q of a workgroup's queries: a wave holds 32, the keys that they see walk by.
 template <typename T, int kDim>
-__global__ __launch_bounds__(kThreads) void attention_bwd_queries_kernel(BackwardArgs a) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) void attention_bwd_queries_kernel(BackwardArgs a) {
   constexpr int kRows = kTileRows<T, kDim>;
   constexpr int kPitchT = kPitch<T, kDim>;
   constexpr int kSteps = kDim / 16, kBlocks = kDim / 32;
