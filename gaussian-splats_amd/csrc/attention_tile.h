@@ -10,6 +10,8 @@
 // one product into the next without leaving their registers.
 #pragma once
 
+#include <type_traits>
+
 #include "sequence.h"
 
 namespace gs {
@@ -22,8 +24,9 @@ using Acc = FloatVec<16>;
 template <typename T>
 using Frag = Vec<T, 8>;
 
+__device__ __forceinline__ constexpr int acc_row_of_half(int r) { return (r & 3) + 8 * (r >> 2); }
 __device__ __forceinline__ int acc_row(int r) {
-  return (r & 3) + 8 * (r >> 2) + 4 * (int(threadIdx.x & 63) >> 5);
+  return acc_row_of_half(r) + 4 * (int(threadIdx.x & 63) >> 5);
 }
 
 __device__ __forceinline__ void mma(const Frag<bf16>& a, const Frag<bf16>& b, Acc& c) {
@@ -108,6 +111,28 @@ __device__ __forceinline__ Frag<T> acc_frag(const Acc& c, int s) {
   return from_float<T, 8>(v);
 }
 
+// sum + the fragment's elements: two at a time where the type has a product of
+// pairs, which takes half the instructions of plain additions.
+__device__ __forceinline__ float add_all(const Frag<bf16>& f, float sum) {
+  const Vec<bf16, 2> one(bf16(1.0f));
+#pragma unroll
+  for (int i = 0; i < 8; i += 2)
+    sum = __builtin_amdgcn_fdot2_f32_bf16(Vec<bf16, 2>{f[i], f[i + 1]}, one, sum, false);
+  return sum;
+}
+__device__ __forceinline__ float add_all(const Frag<f16>& f, float sum) {
+  const Vec<f16, 2> one(f16(1.0f));
+#pragma unroll
+  for (int i = 0; i < 8; i += 2)
+    sum = __builtin_amdgcn_fdot2(Vec<f16, 2>{f[i], f[i + 1]}, one, sum, false);
+  return sum;
+}
+__device__ __forceinline__ float add_all(const Frag<float>& f, float sum) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum += f[i];
+  return sum;
+}
+
 // A [kRows, kDim] tile on its way from global memory through a workgroup's
 // registers into LDS.  Rows outside [0, end) and columns from dim on are zeros.
 template <typename T, int kRows, int kDim, int kThreads>
@@ -140,45 +165,66 @@ struct Stage {
 
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.4028235e38f; }
 
-// acc[n] += a[n] b over 16 of the contraction, where `seen(k)` says whether the
-// lane's column takes element k of it at all.  b is zero where it does not, but
-// zero times an infinity or a NaN of a, which the column must not see, is a NaN:
-// where a holds one, the product is formed without it, and what it gives is
-// added, one element of the contraction at a time, to the columns that see it.
-// The others keep the bits that they would have had.
-template <typename T, int kCount, typename F>
-__device__ __forceinline__ void mma_seen(Frag<T> (&a)[kCount], const Frag<T>& b,
-                                         Acc (&acc)[kCount], F&& seen) {
-  const int half = int(threadIdx.x & 63) >> 5;
-#pragma unroll
-  for (int n = 0; n < kCount; ++n) {
+// Infinities and NaN at places that some columns of a tile do not see.  In a
+// product those columns hold a zero there, but zero times such a value is a NaN.
+// So guard() takes them out of the first operand, and marks by two bits for each
+// element of the result what they add to the columns that do see them; apply()
+// adds that at the end.  The other columns keep the bits that they would have.
+template <typename T, int kCount>
+struct Poison {
+  uint32_t marks[kCount] = {};  // +inf: bit r, -inf: bit 16 + r, NaN: both
+
+  // a[n]: the turned fragments of rows row0 .. row0 + 15 and columns 32 n .. of
+  // the tile, which are multiplied with b; seen(k): whether the lane's column
+  // takes row row0 + k.  Marks are made element by element: the code is small
+  // and needs few registers beside the caller's.
+  template <typename F>
+  __device__ __forceinline__ void guard(const T* tile, int pitch, int row0, Frag<T> (&a)[kCount],
+                                        const Frag<T>& b, F&& seen) {
     bool bad = false;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) bad |= !finite(float(a[n][i]));
-    if (__any(bad)) {
+    for (int n = 0; n < kCount; ++n)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) bad |= !finite(float(a[n][i]));
+    if (__builtin_expect(!__any(bad), 1)) return;
+    const int lane = threadIdx.x & 63;
 #pragma unroll 1
-      for (int k = 0; k < 16; ++k) {
-        const int at = ((k >> 2) & 1) == half ? (k & 3) + 4 * (k >> 3) : -1;
-        Frag<T> a1(T(0.0f)), b1(T(0.0f));
+    for (int k = 0; k < 16; ++k) {
+      float w = float(b[0]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (i != at) continue;
-          b1[i] = b[i];
-          if (!finite(float(a[n][i]))) a1[i] = a[n][i];
+      for (int i = 1; i < 8; ++i) w = (k & 3) + 4 * (k >> 3) == i ? float(b[i]) : w;
+      w = __shfl(w, (lane & 31) + 32 * ((k >> 2) & 1), 64);
+      const bool see = seen(k);
+#pragma unroll 1
+      for (int r = 0; r < 16; ++r) {
+        const T* at = tile + (row0 + k) * pitch + acc_row(r);
+#pragma unroll
+        for (int n = 0; n < kCount; ++n) {
+          const float v = float(at[32 * n]), t = w * v;
+          const uint32_t up = !(t <= 3.4028235e38f), down = !(t >= -3.4028235e38f);
+          if (see && !finite(v)) marks[n] |= (up << r) | (down << (16 + r));
         }
-        Acc one(0.0f);
-        mma(a1, b1, one);
-        const bool see = seen(k);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[n][r] += see ? one[r] : 0.0f;
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (!finite(float(a[n][i]))) a[n][i] = T(0.0f);
     }
-    mma(a[n], b, acc[n]);
+#pragma unroll
+    for (int n = 0; n < kCount; ++n)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a[n][i] = finite(float(a[n][i])) ? a[n][i] : T(0.0f);
   }
-}
+  __device__ __forceinline__ void apply(Acc (&acc)[kCount]) const {
+    uint32_t any = 0;
+#pragma unroll
+    for (int n = 0; n < kCount; ++n) any |= marks[n];
+    if (!__any(any != 0)) return;
+#pragma unroll
+    for (int n = 0; n < kCount; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        if (marks[n] >> r & 1) acc[n][r] += INFINITY;
+        if (marks[n] >> (16 + r) & 1) acc[n][r] -= INFINITY;
+      }
+  }
+};
 
 // Problem of one call; strides in elements, rows contiguous.
 struct Strides {
@@ -196,9 +242,30 @@ struct Problem {
   __device__ __forceinline__ int length(int b) const {
     return lengths ? min(max(lengths[b], 0), keys) : keys;
   }
-  // Key j (below the length) is seen from position p.
-  __device__ __forceinline__ bool sees(int p, int j, int length) const {
-    return j <= p && (j > p - window || j < sinks) && j < length;
+};
+
+// Which of the keys base + k a query at position p sees: comparisons of k,
+// known at compile time, with a few registers.
+struct KeySight {
+  int top, low, sinks;
+  __device__ __forceinline__ KeySight(const Problem& p, int pos, int base, int length)
+      : top(min(pos, length - 1) - base), low(pos - p.window - base), sinks(p.sinks - base) {}
+  __device__ __forceinline__ bool sees(int k) const {
+    return bool(int(k <= top) & (int(k > low) | int(k < sinks)));
+  }
+};
+
+// Which of the queries base + k, of those in [from, to), see key j.
+struct QuerySight {
+  int low, end;
+  __device__ __forceinline__ QuerySight(const Problem& p, int j, int base, int from, int to,
+                                        int length) {
+    const int at = p.offset() + base;  // position of k = 0
+    low = max(j - at, from - base);
+    end = j >= length ? low : j < p.sinks ? to - base : min(to - base, j - at + p.window);
+  }
+  __device__ __forceinline__ bool sees(int k) const {
+    return bool(int(k >= low) & int(k < end));
   }
 };
 

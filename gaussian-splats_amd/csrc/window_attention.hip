@@ -10,7 +10,7 @@
 // 32 scores of one query: maximum, sum and rescaling are the lane's own up to
 // one exchange with the other half, and the exponentials are the next product's
 // operand in place.  Probabilities are rounded to the inputs' type for that
-// product (the sum adds them unrounded).
+// product and for the sum alike, so that a row's weights add up to one.
 #include "attention_tile.h"
 
 namespace gs {
@@ -50,7 +50,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
   const int b = int(id / group / blocks / p.kv_heads);
   const int head = kv * group + of;
   const int length = p.length(b);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
   const int i = block * kQueries + wave * 32 + (lane & 31);  // the lane's query
   const int pos = p.offset() + i;
@@ -81,6 +81,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
 #pragma unroll
   for (int n = 0; n < kBlocks; ++n) o[n] = Acc(0.0f);
 
+  Poison<T, kBlocks> poison;
   Stage<T, kKeys, kDim, kThreads> sk, sv;
   const auto fetch = [&](int it) {
     const int j0 = (it < head_tiles ? it : tail + it) * kKeys;
@@ -110,21 +111,23 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
           mma(load_rows<T>(kt, kPitchT, 32 * h, 16 * st), q[st], s[h]);
       }
       if (!all) {
+        const KeySight sight(p, pos, j0 + 4 * (lane >> 5), length);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if (!p.sees(pos, j0 + 32 * h + acc_row(r), length)) s[h][r] = -INFINITY;
+            if (!sight.sees(32 * h + acc_row_of_half(r))) s[h][r] = -INFINITY;
       }
-      float m = -INFINITY;
+      float m = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) m = fmaxf(m, s[h][r]);
+      for (int r = 1; r < 16; ++r) m = fmaxf(fmaxf(m, s[0][r]), s[1][r]);
       m = fmaxf(m, __shfl_xor(m, 32, 64)) * c;
-      if (__any(m > top)) {
-        const float up = fmaxf(top, m);
-        const float shrink = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - up);
+      // The maximum that exponents are taken against follows the true one at a
+      // distance of up to 2^8, so that most tiles rescale nothing.
+      if (__any(m > top + 8.0f)) {
+        const float up = m > top + 8.0f ? m : top;
+        float shrink = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - up);
+        asm volatile("" : "+v"(shrink));  // or the compiler rescales without the branch
         sum *= shrink;
 #pragma unroll
         for (int n = 0; n < kBlocks; ++n) o[n] *= shrink;
@@ -134,27 +137,21 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[h][r] = power<T>(s[h][r] * c - base);
-          sum += s[h][r];
-        }
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
         for (int st = 0; st < 2; ++st) {
+#pragma unroll
+          for (int r = 8 * st; r < 8 * st + 8; ++r) s[h][r] = power<T>(s[h][r] * c - base);
           const Frag<T> pf = acc_frag<T>(s[h], st);
+          sum = add_all(pf, sum);
           Frag<T> vf[kBlocks];
 #pragma unroll
           for (int n = 0; n < kBlocks; ++n)
             vf[n] = load_turned<T>(vt, kPitchT, 32 * h + 16 * st, 32 * n);
-          if (all) {
-#pragma unroll
-            for (int n = 0; n < kBlocks; ++n) mma(vf[n], pf, o[n]);
-          } else {
-            mma_seen<T>(vf, pf, o, [&](int e) {
-              return p.sees(pos, j0 + 32 * h + 16 * st + e, length);
-            });
+          if (!all) {
+            const KeySight sight(p, pos, j0 + 32 * h + 16 * st, length);
+            poison.guard(vt, kPitchT, 32 * h + 16 * st, vf, pf, [&](int e) { return sight.sees(e); });
           }
+#pragma unroll
+          for (int n = 0; n < kBlocks; ++n) mma(vf[n], pf, o[n]);
         }
     }
     if (it + 1 < count) {
@@ -163,6 +160,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
     }
     __syncthreads();
   }
+  poison.apply(o);
   if (i >= p.queries) return;
   sum += __shfl_xor(sum, 32, 64);
   const float inverse = top == -INFINITY && sum == 0.0f ? 0.0f : 1.0f / sum;

@@ -94,7 +94,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
   const int segment = part ? item % a.segments : 0;
   const int group = p.heads / p.kv_heads;
   const int length = p.length(b);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int k0 = block * kBlockKeys;  // first key of the workgroup
   const int w0 = k0 + wave * 32;      // of the wave
   const int j = w0 + (lane & 31);     // the lane's
@@ -130,6 +130,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
   for (int n = 0; n < kBlocks; ++n) dk[n] = dv[n] = Acc(0.0f);
   const float c = p.scale * kLog2e;
 
+  Poison<T, kBlocks> pk, pv;
   Stage<T, kRows, kDim, kThreads> sq, sg;
   float row_lse = 0.0f, row_delta = 0.0f;
   const auto fetch = [&](int it) {
@@ -164,7 +165,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
     const T* qt = tiles[it & 1][0];
     const T* gt = tiles[it & 1][1];
     const int i0 = (first_tile + it % tiles_per_head) * kRows;
-#pragma unroll
+#pragma unroll 1
     for (int h = 0; h < kRows / 32; ++h) {
       const int p0 = off + i0 + 32 * h, p1 = p0 + 31;  // positions
       // Queries outside [from, to) belong to other segments.
@@ -173,56 +174,57 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
                        (w0 + 31 > p0 - p.window || w0 < p.sinks);
       const bool all = inside && w0 + 31 <= p0 && w0 + 31 < length &&
                        (w0 > p1 - p.window || w0 + 31 < p.sinks);
-      if (!any) continue;
-      const auto seen = [&](int row) {  // row of the 32: query i0 + 32 h + row, key j
-        const int i = i0 + 32 * h + row;
-        return i >= from && i < to && p.sees(off + i, j, length);
-      };
-      Acc s(0.0f), dp(0.0f);
+      if (any) {
+        Acc s(0.0f), dp(0.0f);
 #pragma unroll
-      for (int st = 0; st < kSteps; ++st) mma(load_rows<T>(qt, kPitchT, 32 * h, 16 * st), kf[st], s);
+        for (int st = 0; st < kSteps; ++st)
+          mma(load_rows<T>(qt, kPitchT, 32 * h, 16 * st), kf[st], s);
 #pragma unroll
-      for (int st = 0; st < kSteps; ++st) mma(load_rows<T>(gt, kPitchT, 32 * h, 16 * st), vf[st], dp);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int row = 32 * h + acc_row(r);
-        const float lse = rows[it & 1][0][row], delta = rows[it & 1][1][row];
-        s[r] = power<T>(s[r] * c - lse);
-        dp[r] = s[r] * (dp[r] - delta);
-      }
-      if (!all) {
+        for (int st = 0; st < kSteps; ++st)
+          mma(load_rows<T>(gt, kPitchT, 32 * h, 16 * st), vf[st], dp);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const bool see = seen(acc_row(r));
-          s[r] = see ? s[r] : 0.0f;
-          dp[r] = see ? dp[r] : 0.0f;
+          const int row = 32 * h + acc_row(r);
+          const float lse = rows[it & 1][0][row], delta = rows[it & 1][1][row];
+          s[r] = power<T>(s[r] * c - lse);
+          dp[r] = s[r] * (dp[r] - delta);
         }
-      }
+        if (!all) {
+          const QuerySight sight(p, j, i0 + 32 * h + 4 * (lane >> 5), from, to, length);
 #pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        const Frag<T> pf = acc_frag<T>(s, st), df = acc_frag<T>(dp, st);
-        Frag<T> f[kBlocks];
+          for (int r = 0; r < 16; ++r) {
+            const bool see = sight.sees(acc_row_of_half(r));
+            s[r] = see ? s[r] : 0.0f;
+            dp[r] = see ? dp[r] : 0.0f;
+          }
+        }
 #pragma unroll
-        for (int n = 0; n < kBlocks; ++n) f[n] = load_turned<T>(gt, kPitchT, 32 * h + 16 * st, 32 * n);
-        if (all) {
+        for (int st = 0; st < 2; ++st) {
+          const Frag<T> pf = acc_frag<T>(s, st), df = acc_frag<T>(dp, st);
+          Frag<T> f[kBlocks];
+#pragma unroll
+          for (int n = 0; n < kBlocks; ++n)
+            f[n] = load_turned<T>(gt, kPitchT, 32 * h + 16 * st, 32 * n);
+          const QuerySight sight(p, j, i0 + 32 * h + 16 * st, from, to, length);
+          if (!all)
+            pv.guard(gt, kPitchT, 32 * h + 16 * st, f, pf, [&](int e) { return sight.sees(e); });
 #pragma unroll
           for (int n = 0; n < kBlocks; ++n) mma(f[n], pf, dv[n]);
-        } else {
-          mma_seen<T>(f, pf, dv, [&](int e) { return seen(16 * st + e); });
-        }
 #pragma unroll
-        for (int n = 0; n < kBlocks; ++n) f[n] = load_turned<T>(qt, kPitchT, 32 * h + 16 * st, 32 * n);
-        if (all) {
+          for (int n = 0; n < kBlocks; ++n)
+            f[n] = load_turned<T>(qt, kPitchT, 32 * h + 16 * st, 32 * n);
+          if (!all)
+            pk.guard(qt, kPitchT, 32 * h + 16 * st, f, df, [&](int e) { return sight.sees(e); });
 #pragma unroll
           for (int n = 0; n < kBlocks; ++n) mma(f[n], df, dk[n]);
-        } else {
-          mma_seen<T>(f, df, dk, [&](int e) { return seen(16 * st + e); });
         }
       }
     }
     if (it + 1 < count) keep((it + 1) & 1);
     __syncthreads();
   }
+  pk.apply(dk);
+  pv.apply(dv);
   if (part) {
     float* at = a.parts + ((((int64_t(b) * p.kv_heads + kv) * a.sink_blocks + block) * a.segments +
                             segment) * 2 * kBlockKeys + wave * 32 + (lane & 31)) * p.dim;
@@ -304,7 +306,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
   const int b = int(id / group / blocks / p.kv_heads);
   const int head = kv * group + of;
   const int length = p.length(b);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i = block * kBlockQueries + wave * 32 + (lane & 31);
   const int pos = p.offset() + i;
   const bool live = i < p.queries;
@@ -336,6 +338,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
 
   const T* kbase = static_cast<const T*>(a.k) + b * a.sk.batch + kv * a.sk.head;
   const T* vbase = static_cast<const T*>(a.v) + b * a.sv.batch + kv * a.sv.head;
+  Poison<T, kBlocks> poison;
   Stage<T, kRows, kDim, kThreads> sk, sv;
   const auto fetch = [&](int it) {
     const int j0 = (it < head_tiles ? it : tail + it) * kRows;
@@ -352,35 +355,39 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
     if (it + 1 < count) fetch(it + 1);
     const T* kt = tiles[it & 1][0];
     const T* vt = tiles[it & 1][1];
-#pragma unroll
+#pragma unroll 1
     for (int h = 0; h < kRows / 32; ++h) {
       const int j0 = (it < head_tiles ? it : tail + it) * kRows + 32 * h, j1 = j0 + 31;
       const bool any = j0 <= wave_last && j0 < length && (j1 > wave_first - p.window || j0 < p.sinks);
       const bool all = j1 <= wave_first && j1 < length && (j0 > wave_last - p.window || j1 < p.sinks);
-      if (!any) continue;
-      Acc s(0.0f), dp(0.0f);
+      if (any) {
+        Acc s(0.0f), dp(0.0f);
 #pragma unroll
-      for (int st = 0; st < kSteps; ++st) mma(load_rows<T>(kt, kPitchT, 32 * h, 16 * st), q[st], s);
+        for (int st = 0; st < kSteps; ++st)
+          mma(load_rows<T>(kt, kPitchT, 32 * h, 16 * st), q[st], s);
 #pragma unroll
-      for (int st = 0; st < kSteps; ++st) mma(load_rows<T>(vt, kPitchT, 32 * h, 16 * st), g[st], dp);
+        for (int st = 0; st < kSteps; ++st)
+          mma(load_rows<T>(vt, kPitchT, 32 * h, 16 * st), g[st], dp);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) dp[r] = power<T>(s[r] * c - lse) * (dp[r] - delta);
-      if (!all) {
+        for (int r = 0; r < 16; ++r) dp[r] = power<T>(s[r] * c - lse) * (dp[r] - delta);
+        if (!all) {
+          const KeySight sight(p, pos, j0 + 4 * (lane >> 5), length);
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (!p.sees(pos, j0 + acc_row(r), length)) dp[r] = 0.0f;
-      }
+          for (int r = 0; r < 16; ++r) dp[r] = sight.sees(acc_row_of_half(r)) ? dp[r] : 0.0f;
+        }
 #pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        const Frag<T> df = acc_frag<T>(dp, st);
-        Frag<T> f[kBlocks];
+        for (int st = 0; st < 2; ++st) {
+          const Frag<T> df = acc_frag<T>(dp, st);
+          Frag<T> f[kBlocks];
 #pragma unroll
-        for (int n = 0; n < kBlocks; ++n) f[n] = load_turned<T>(kt, kPitchT, 32 * h + 16 * st, 32 * n);
-        if (all) {
+          for (int n = 0; n < kBlocks; ++n)
+            f[n] = load_turned<T>(kt, kPitchT, 32 * h + 16 * st, 32 * n);
+          if (!all) {
+            const KeySight sight(p, pos, j0 + 16 * st, length);
+            poison.guard(kt, kPitchT, 32 * h + 16 * st, f, df, [&](int e) { return sight.sees(e); });
+          }
 #pragma unroll
           for (int n = 0; n < kBlocks; ++n) mma(f[n], df, dq[n]);
-        } else {
-          mma_seen<T>(f, df, dq, [&](int e) { return p.sees(pos, j0 + 16 * st + e, length); });
         }
       }
     }
@@ -390,6 +397,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
     }
     __syncthreads();
   }
+  poison.apply(dq);
   if (!live) return;
   T* out = static_cast<T*>(a.dq) + ((int64_t(b) * p.queries + i) * p.heads + head) * p.dim;
 #pragma unroll

@@ -43,7 +43,7 @@ __global__ __launch_bounds__(kThreads) void attention_step_kernel(StepArgs a) {
   __shared__ __align__(16) T tiles[kWaves][kKeys * kPitchT];
   __shared__ float joined[32][kDim + 1];
   __shared__ float tops[kWaves][32], sums[kWaves][32];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
   const int group = a.heads / a.kv_heads, group_tiles = (group + 31) / 32;
   const int kv = blockIdx.y / group_tiles, group_tile = blockIdx.y % group_tiles;
   const int b = blockIdx.z, split = blockIdx.x;
