@@ -268,19 +268,56 @@ __global__ __launch_bounds__(1024) void scan_bwd_kernel(ScanArgs a) {
 }
 
 // The walk over a channel's chunks: forward, h before each chunk; backward,
-// the carried gradient after each chunk, last chunk first.
+// the carried gradient after each chunk, last chunk first.  A lane has a
+// channel, the sixteen waves a run of chunks each: they compose their run's map,
+// get the state before it from the runs in front, and walk the run from it.
 template <bool kBackward>
-__global__ __launch_bounds__(64) void scan_walk_kernel(ScanArgs a) {
-  const int64_t c = int64_t(blockIdx.x) * 64 + threadIdx.x, b = blockIdx.y;
-  if (c >= a.channels) return;
+__global__ __launch_bounds__(1024) void scan_walk_kernel(ScanArgs a) {
+  constexpr int kWaves = 16, kAhead = 8;
+  __shared__ float mapA[kWaves][kWave], mapB[kWaves][kWave];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t c = int64_t(blockIdx.x) * kWave + lane, b = blockIdx.y;
+  const bool live = c < a.channels;
+  const int64_t run = (a.chunks + kWaves - 1) / kWaves;
+  const int64_t lo = std::min<int64_t>(a.chunks, wave * run), hi = std::min<int64_t>(a.chunks, lo + run);
+  const auto chunk = [&](int64_t i) { return b * a.chunks + (kBackward ? a.chunks - 1 - i : i); };
+  // Calls f(i, A, B) for the run's chunks; kAhead maps are loaded together.
+  const auto each = [&](auto&& f) {
+    for (int64_t i = lo; i < hi; i += kAhead) {
+      float A[kAhead], B[kAhead];
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n)
+        if (i + n < hi) {
+          const float* m = a.maps + 2 * chunk(i + n) * a.channels + c;
+          A[n] = m[0];
+          B[n] = m[a.channels];
+        }
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n)
+        if (i + n < hi) f(i + n, A[n], B[n]);
+    }
+  };
+  float A = 1.0f, B = 0.0f;
+  if (live && a.maps && wave + 1 < kWaves)
+    each([&](int64_t, float x, float y) {
+      B = x * B + y;
+      A *= x;
+    });
+  mapA[wave][lane] = A;
+  mapB[wave][lane] = B;
+  __syncthreads();
+  if (!live) return;
   const float* init = kBackward ? a.grad_last : a.state;
   float h = init ? init[b * a.channels + c] : 0.0f;
+  for (int i = 0; i < wave; ++i) h = mapA[i][lane] * h + mapB[i][lane];
   float* out = kBackward ? a.carries : a.starts;
-  for (int64_t i = 0; i < a.chunks; ++i) {
-    const int64_t k = b * a.chunks + (kBackward ? a.chunks - 1 - i : i);
-    out[k * a.channels + c] = h;
-    if (a.maps) h = a.maps[2 * k * a.channels + c] * h + a.maps[(2 * k + 1) * a.channels + c];
-  }
+  if (a.maps)
+    each([&](int64_t i, float x, float y) {
+      out[chunk(i) * a.channels + c] = h;
+      h = x * h + y;
+    });
+  else if (wave == 0)
+    out[chunk(0) * a.channels + c] = h;
 }
 
 template <typename T, int kChannels>
@@ -355,7 +392,7 @@ int run_scan(const ScanArgs& a, int32_t type, hipStream_t s) {
       GS_TRY(check_launch("gated_scan maps"));
     }
     scan_walk_kernel<kBackward>
-        <<<dim3(unsigned((a.channels + 63) / 64), unsigned(a.batch)), 64, 0, s>>>(a);
+        <<<dim3(unsigned((a.channels + 63) / 64), unsigned(a.batch)), 1024, 0, s>>>(a);
     GS_TRY(check_launch("gated_scan walk"));
     if constexpr (kBackward)
       scan_bwd_kernel<T, kN, false><<<grid, 1024, 0, s>>>(a);
