@@ -24,17 +24,21 @@ namespace {
 
 using namespace seq;
 
-constexpr int kChunk = 128;  // tokens of a workgroup
+// A workgroup has 15 waves that hold a run of tokens each, and one that only
+// looks back: it starts at once, while the others wait for their loads, and its
+// registers and theirs are the same ones.  The backward holds more for a token,
+// so its runs and chunks are half as long; the forward keeps a state at each
+// start of the backward's chunks.
+constexpr int kWaves = 15;
+constexpr int kThreads = (kWaves + 1) * kWave;
 
-// Waves of a workgroup and each one's run of tokens.  The backward holds more
-// for a token, so it gets by with shorter runs: both stay within the registers
-// that let 16 waves share a CU.
 template <bool kBackward>
 struct Shape {
-  static constexpr int kWaves = kBackward ? 16 : 8;
-  static constexpr int kRun = kChunk / kWaves;
-  static constexpr int kThreads = kWaves * kWave;
+  static constexpr int kRun = kBackward ? 8 : 16;
+  static constexpr int kChunk = kWaves * kRun;
 };
+constexpr int kStartTokens = Shape<true>::kChunk;  // tokens from one kept state to the next
+constexpr int kStarts = Shape<false>::kChunk / kStartTokens;  // kept states of a forward chunk
 
 struct Gate {
   float a;     // sigmoid(g)
@@ -43,16 +47,17 @@ struct Gate {
 
 template <typename T>
 __device__ __forceinline__ Gate gate_of(float g) {
-  // exp(-|g|) does not overflow, and neither a nor 1 - a loses bits near 0 or 1.
-  // float32 inputs get the library's exp; for 16-bit ones the instruction's
-  // error is far below their rounding.
+  // With e = exp(-g), a = 1 / (1 + e) and 1 - a = e a lose no bits near 0 or 1.
+  // Where e overflows a is 0 and e a a NaN, of which the minimum makes 1; a NaN
+  // of g stays in a.  float32 inputs get the library's exp; for 16-bit ones the
+  // instruction's error is far below their rounding.
   float e;
   if constexpr (sizeof(T) == 4)
-    e = expf(-fabsf(g));
+    e = expf(-g);
   else
-    e = __builtin_amdgcn_exp2f(-fabsf(g) * 1.44269504f);
-  const float r = __builtin_amdgcn_rcpf(1.0f + e);
-  return g >= 0.0f ? Gate{r, e * r} : Gate{e * r, r};
+    e = __builtin_amdgcn_exp2f(g * -1.44269504f);
+  const float a = __builtin_amdgcn_rcpf(1.0f + e);
+  return {a, fminf(e * a, 1.0f)};
 }
 
 // N channels of one lane.
@@ -76,12 +81,12 @@ struct ScanArgs {
   const void* gate;
   const void* grad_y;      // backward; null: zeros
   int64_t x_batch, x_token, gate_batch, gate_token, grad_batch, grad_token;  // strides
-  int64_t batch, tokens, channels, chunks;
+  int64_t batch, tokens, channels, chunks, starts_count;
+  uint32_t items;          // chunks of all channels' tiles and sequences
   // Published words; all bits set: not yet.  maps [batch, chunks, channels]: A
-  // and B of a chunk in one word.  ends [batch, chunks, channels]: forward, h
-  // before each chunk (the starts that the backward reads); backward, the
-  // carried gradient after each chunk.  The entry of the chunk that comes next
-  // is a chunk's end state.
+  // and B of a chunk in one word.  ends: the state that a chunk starts from,
+  // forward h [batch, starts_count, channels], of which a chunk has kStarts,
+  // backward the carried gradient [batch, chunks, channels].
   uint64_t* maps;
   float* ends;
   uint32_t* ticket;        // null: a single chunk
@@ -98,7 +103,8 @@ struct ScanArgs {
 
 constexpr uint32_t kUnset = 0xffffffffu;
 constexpr int kSpinLimit = 1 << 20;
-constexpr int kAhead = 8;  // published words that are requested together
+constexpr int kComputeUnits = 256;
+constexpr int kAhead = 16;  // published words that are requested together
 
 // A float as a word that is not kUnset (a NaN of that pattern becomes another).
 __device__ __forceinline__ uint32_t word_of(float v) {
@@ -142,59 +148,83 @@ struct Words {
   }
 };
 
-// State before the chunk whose place in the walk is `place` (forward: the chunk,
-// backward: counted from the last), for the channels of one wave's lanes: the
-// nearest published end state and the maps after it.  A place's words are
-// published by a workgroup with an earlier ticket, so every wait ends; the spin
-// limit turns a broken invariant into an error flag.  `init` is the state before
-// place 0.
+// One item of the work: a chunk of a tile of channels of a sequence.  Items are
+// numbered in the order of the chunks' places in the walk (forward the chunk,
+// backward counted from the last one).
+template <bool kBackward, int kChannels>
+struct Item {
+  static constexpr int kRun = Shape<kBackward>::kRun;
+  int64_t b, place, chunk, c, t0;
+  int count;  // tokens of the wave's run that exist
+  bool live;  // the lane has channels; others repeat the last ones
+  __device__ __forceinline__ Item(const ScanArgs& a, uint32_t item, int wave, int lane) {
+    const uint32_t tiles = uint32_t((a.channels + kWave * kChannels - 1) / (kWave * kChannels));
+    c = (int64_t(item % tiles) * kWave + lane) * kChannels;
+    live = c < a.channels;
+    c = live ? c : a.channels - kChannels;
+    b = item / tiles % uint32_t(a.batch);
+    place = item / tiles / uint32_t(a.batch);
+    chunk = kBackward ? a.chunks - 1 - place : place;
+    t0 = chunk * Shape<kBackward>::kChunk + wave * kRun;
+    const int64_t left = a.tokens - t0;
+    count = int(left < 0 ? 0 : (left < kRun ? left : kRun));
+  }
+  __device__ __forceinline__ bool last(const ScanArgs& a) const { return place + 1 >= a.chunks; }
+};
+
+template <bool kBackward>
+__device__ __forceinline__ int64_t map_row(const ScanArgs& a, int64_t b, int64_t place) {
+  return (b * a.chunks + (kBackward ? a.chunks - 1 - place : place)) * a.channels;
+}
+template <bool kBackward>
+__device__ __forceinline__ int64_t end_row(const ScanArgs& a, int64_t b, int64_t place) {
+  return kBackward ? map_row<true>(a, b, place)
+                   : (b * a.starts_count + place * kStarts) * a.channels;
+}
+
+// State before an item's chunk for the channels of one wave's lanes: the nearest
+// published one and the maps after it.  These are published by workgroups that
+// hold earlier tickets, so every wait ends; the spin limit turns a broken
+// invariant into an error flag.  `init` is the state before place 0.
 template <bool kBackward, int kChannels>
 __device__ FloatVec<kChannels> look_back(const ScanArgs& a, int64_t b, int64_t place, int64_t c,
-                                         bool live, FloatVec<kChannels> init) {
-  if (place == 0) return init;
-  const auto row = [&](int64_t i) {
-    return (b * a.chunks + (kBackward ? a.chunks - 1 - i : i)) * a.channels + c;
-  };
-  int spins = 0;
-  // The nearest place whose start is known; that of place 0 always is.
+                                         FloatVec<kChannels> init) {
   FloatVec<kChannels> h = init;
-  int64_t from = place;
+  int64_t from = place;  // down to the nearest place whose start is known
   for (bool found = false; !found && from > 0;) {
     Words<kChannels> w[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i)
-      if (live && from - i > 0) w[i].load(a.ends + row(from - i));
+      if (from - i > 0) w[i].load(a.ends + end_row<kBackward>(a, b, from - i) + c);
     int step = kAhead;
 #pragma unroll
-    for (int i = kAhead - 1; i >= 0; --i) {
-      const bool known = from - i > 0 && __all(!live || w[i].set());
-      if (known) {
+    for (int i = kAhead - 1; i >= 0; --i)
+      if (from - i > 0 && __all(w[i].set())) {
         step = i;
+        found = true;
 #pragma unroll
         for (int n = 0; n < kChannels; ++n) h[n] = __uint_as_float(w[i].w[n]);
-        found = true;
       }
-    }
     from -= step;
+    if (!found) h = init;
   }
-  if (from <= 0) {
-    from = 0;
-    h = init;
-  }
-  // The maps of places from .. place - 1, in order.
-  while (from < place) {
+  from = from > 0 ? from : 0;
+  int spins = 0;
+  while (from < place) {  // the maps of places from .. place - 1, in order
     uint64_t m[kAhead][kChannels];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i)
 #pragma unroll
       for (int n = 0; n < kChannels; ++n)
-        m[i][n] = live && from + i < place ? load_word(a.maps + row(from + i) + n) : 0;
+        m[i][n] = from + i < place
+                      ? load_word(a.maps + map_row<kBackward>(a, b, from + i) + c + n)
+                      : ~uint64_t(0);
     int taken = 0;
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      bool ready = from + i < place && taken == i;
+      bool ready = taken == i;
 #pragma unroll
-      for (int n = 0; n < kChannels; ++n) ready &= bool(__all(m[i][n] != ~uint64_t(0)));
+      for (int n = 0; n < kChannels; ++n) ready = ready && __all(m[i][n] != ~uint64_t(0));
       if (ready) {
 #pragma unroll
         for (int n = 0; n < kChannels; ++n)
@@ -215,39 +245,10 @@ __device__ FloatVec<kChannels> look_back(const ScanArgs& a, int64_t b, int64_t p
   return h;
 }
 
-// A workgroup's place: tickets in the order of the places, so that what a
-// workgroup waits for is held by others that already run.
-template <bool kBackward, int kChannels>
-struct Place {
-  static constexpr int kRun = Shape<kBackward>::kRun;
-  int64_t b, place, chunk, c, t0;
-  int count, lane, wave;
-  bool live;
-  __device__ Place(const ScanArgs& a, uint32_t* shared) {
-    uint32_t item = blockIdx.x;
-    if (a.ticket) {
-      if (threadIdx.x == 0) *shared = atomicAdd(a.ticket, 1u);
-      __syncthreads();
-      item = *shared;
-    }
-    lane = threadIdx.x & 63;
-    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t tiles = uint32_t((a.channels + kWave * kChannels - 1) / (kWave * kChannels));
-    c = (int64_t(item % tiles) * kWave + lane) * kChannels;
-    b = item / tiles % uint32_t(a.batch);
-    place = item / tiles / uint32_t(a.batch);
-    chunk = kBackward ? a.chunks - 1 - place : place;
-    live = c < a.channels;
-    t0 = chunk * kChunk + wave * kRun;
-    const int64_t left = a.tokens - t0;
-    count = int(left < 0 ? 0 : (left < kRun ? left : kRun));
-  }
-};
-
 template <int kChannels>
-__device__ __forceinline__ FloatVec<kChannels> load_state(const float* p, int64_t at, bool live) {
+__device__ __forceinline__ FloatVec<kChannels> load_state(const float* p, int64_t at) {
   FloatVec<kChannels> v(0.0f);
-  if (p && live) {
+  if (p) {
 #pragma unroll
     for (int n = 0; n < kChannels; ++n) v[n] = p[at + n];
   }
@@ -262,199 +263,301 @@ __device__ __forceinline__ FloatVec<kChannels> fma(FloatVec<kChannels> a, FloatV
   return y;
 }
 
-template <typename T, int kChannels>
-__global__ __launch_bounds__(Shape<false>::kThreads, 4) void scan_fwd_kernel(ScanArgs a) {
-  constexpr int kRun = Shape<false>::kRun, kWaves = Shape<false>::kWaves;
+// What a workgroup's waves share.  A workgroup takes items until none is left;
+// of what one item's waves still read, the next item uses the other half.
+// Counters only grow: the n-th item's signals have been given when `runs` is
+// (n + 1) kWaves and `whole` n + 1.  Waves that wait for a counter wait for waves
+// of their own workgroup, which wait for nothing.
+template <int kChannels>
+struct Shared {
+  FloatVec<kChannels> mapA[2][kWaves][kWave], mapB[2][kWaves][kWave];
+  FloatVec<kChannels> wholeA[2][kWave], wholeB[2][kWave], before[2][kWave];
+  uint32_t ticket[4], runs, whole;
+};
+
+__device__ __forceinline__ void signal(uint32_t* counter) {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  if ((threadIdx.x & 63) == 0)
+    __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+}
+__device__ __forceinline__ void await(uint32_t* counter, uint32_t count) {
+  while (__hip_atomic_load(counter, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) < count)
+    __builtin_amdgcn_s_sleep(1);
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// Tickets in the order of the items, two ahead of the work: an item is only
+// waited for by later ones, and whoever holds the earliest unfinished one works
+// on it.
+__device__ __forceinline__ uint32_t next_ticket(const ScanArgs& a, uint32_t turn) {
+  return a.ticket ? atomicAdd(a.ticket, 1u) : turn ? a.items : blockIdx.x;
+}
+
+// The looking wave: finds the state before each item's chunk, publishes the one
+// after it once the chunk's map is there, and leaves the former to the others.
+template <bool kBackward, int kChannels>
+__device__ __forceinline__ void look_wave(const ScanArgs& a, Shared<kChannels>& sh,
+                                          const float* first) {
   using Channels = FloatVec<kChannels>;
-  __shared__ Channels mapA[kWaves][kWave], mapB[kWaves][kWave], before[kWave];
-  __shared__ uint32_t ticket;
-  const Place<false, kChannels> w(a, &ticket);
-  Channels ga[kRun], gb[kRun];  // a and (1 - a) x
-  {
-    Vec<T, kChannels> x[kRun], g[kRun];
-    const T* px = static_cast<const T*>(a.x) + w.b * a.x_batch + w.t0 * a.x_token + w.c;
-    const T* pg = static_cast<const T*>(a.gate) + w.b * a.gate_batch + w.t0 * a.gate_token + w.c;
-#pragma unroll
-    for (int i = 0; i < kRun; ++i)
-      if (w.live && i < w.count) {
-        x[i] = load_channels<T, kChannels>(px + i * a.x_token);
-        g[i] = load_channels<T, kChannels>(pg + i * a.gate_token);
-      }
-#pragma unroll
-    for (int i = 0; i < kRun; ++i) {
-      ga[i] = Channels(1.0f);
-      gb[i] = Channels(0.0f);
-      if (w.live && i < w.count) {
-#pragma unroll
-        for (int n = 0; n < kChannels; ++n) {
-          const Gate gt = gate_of<T>(float(g[i][n]));
-          ga[i][n] = gt.a;
-          gb[i][n] = gt.keep * float(x[i][n]);
-        }
-      }
-    }
-  }
-  Channels A(1.0f), B(0.0f);
-#pragma unroll
-  for (int i = 0; i < kRun; ++i) {
-    B = fma<kChannels>(ga[i], B, gb[i]);
-    A *= ga[i];
-  }
-  mapA[w.wave][w.lane] = A;
-  mapB[w.wave][w.lane] = B;
-  __syncthreads();
-  if (w.wave == 0) {
-    const int64_t at = (w.b * a.chunks + w.chunk) * a.channels + w.c;
-    for (int i = 1; i < kWaves; ++i) {
-      B = fma<kChannels>(mapA[i][w.lane], B, mapB[i][w.lane]);
-      A *= mapA[i][w.lane];
-    }
-    const bool more = w.chunk + 1 < a.chunks;
-    if (w.live && more) {
-#pragma unroll
-      for (int n = 0; n < kChannels; ++n)
-        store_word(a.maps + at + n, word_of(A[n]) | uint64_t(word_of(B[n])) << 32);
-    }
-    const Channels init = load_state<kChannels>(a.state, w.b * a.channels + w.c, w.live);
-    const Channels h = look_back<false, kChannels>(a, w.b, w.place, w.c, w.live, init);
-    const Channels end = fma<kChannels>(A, h, B);
-    if (w.live) {
+  const int lane = threadIdx.x & 63;
+  for (uint32_t n = 0;; ++n) {
+    const uint32_t item = sh.ticket[n & 3];
+    if (item >= a.items) return;
+    if (lane == 0) sh.ticket[(n + 2) & 3] = next_ticket(a, 1);
+    const Item<kBackward, kChannels> w(a, item, 0, lane);
+    const Channels init = load_state<kChannels>(first, w.b * a.channels + w.c);
+    const Channels h = look_back<kBackward, kChannels>(a, w.b, w.place, w.c, init);
+    sh.before[n & 1][lane] = h;
+    if (!w.last(a)) {
+      await(&sh.whole, n + 1);
+      const Channels end = fma<kChannels>(sh.wholeA[n & 1][lane], h, sh.wholeB[n & 1][lane]);
       Words<kChannels> v;
-      if (more) {
 #pragma unroll
-        for (int n = 0; n < kChannels; ++n) v.w[n] = word_of(end[n]);
-        v.store(a.ends + at + a.channels);
-      }
-      if (w.chunk == 0) {
-#pragma unroll
-        for (int n = 0; n < kChannels; ++n) a.ends[at + n] = h[n];
-      }
+      for (int k = 0; k < kChannels; ++k) v.w[k] = word_of(end[k]);
+      if (w.live) v.store(a.ends + end_row<kBackward>(a, w.b, w.place + 1) + w.c);
     }
-    before[w.lane] = h;
-  }
-  __syncthreads();
-  if (!w.live) return;
-  Channels h = before[w.lane];
-  for (int i = 0; i < w.wave; ++i) h = fma<kChannels>(mapA[i][w.lane], h, mapB[i][w.lane]);
-  T* py = static_cast<T*>(a.y) + (w.b * a.tokens + w.t0) * a.channels + w.c;
-#pragma unroll
-  for (int i = 0; i < kRun; ++i)
-    if (i < w.count) {
-      h = fma<kChannels>(ga[i], h, gb[i]);
-      store_channels<T, kChannels>(py + i * a.channels, h);
-    }
-  if (w.count > 0 && w.t0 + w.count == a.tokens) {
-#pragma unroll
-    for (int n = 0; n < kChannels; ++n) a.last[w.b * a.channels + w.c + n] = h[n];
+    __syncthreads();
   }
 }
 
-// Backward, the tokens last to first.
-template <typename T, int kChannels>
-__global__ __launch_bounds__(Shape<true>::kThreads, 4) void scan_bwd_kernel(ScanArgs a) {
-  constexpr int kRun = Shape<true>::kRun, kWaves = Shape<true>::kWaves;
+// The first wave in the walk's order: composes and publishes the chunk's map.
+template <bool kBackward, int kChannels>
+__device__ __forceinline__ void publish_map(const ScanArgs& a, const Item<kBackward, kChannels>& w,
+                                            Shared<kChannels>& sh, uint32_t n) {
   using Channels = FloatVec<kChannels>;
-  // A: the run's gates' product, in both directions; B: forward map of h; R:
-  // backward map of the carried gradient.
-  __shared__ Channels mapA[kWaves][kWave], mapB[kWaves][kWave], mapR[kWaves][kWave], after[kWave];
-  __shared__ uint32_t ticket;
-  const Place<true, kChannels> w(a, &ticket);
-  const int64_t at = (w.b * a.chunks + w.chunk) * a.channels + w.c;
-  Channels ga[kRun], keep[kRun], gap[kRun];  // gap: x, later h_{t-1} - x
-  Vec<T, kChannels> dy[kRun];
-  {
-    Vec<T, kChannels> x[kRun], g[kRun];
-    const T* px = static_cast<const T*>(a.x) + w.b * a.x_batch + w.t0 * a.x_token + w.c;
-    const T* pg = static_cast<const T*>(a.gate) + w.b * a.gate_batch + w.t0 * a.gate_token + w.c;
-    const T* pd = static_cast<const T*>(a.grad_y) + w.b * a.grad_batch + w.t0 * a.grad_token + w.c;
+  const int lane = threadIdx.x & 63;
+  await(&sh.runs, (n + 1) * kWaves);
+  Channels A(1.0f), B(0.0f);
 #pragma unroll
-    for (int i = 0; i < kRun; ++i) {
-      dy[i] = Vec<T, kChannels>(T(0.0f));
-      if (w.live && i < w.count) {
-        x[i] = load_channels<T, kChannels>(px + i * a.x_token);
-        g[i] = load_channels<T, kChannels>(pg + i * a.gate_token);
-        if (a.grad_y) dy[i] = load_channels<T, kChannels>(pd + i * a.grad_token);
+  for (int i = 0; i < kWaves; ++i) {
+    const int k = kBackward ? kWaves - 1 - i : i;
+    B = fma<kChannels>(sh.mapA[n & 1][k][lane], B, sh.mapB[n & 1][k][lane]);
+    A *= sh.mapA[n & 1][k][lane];
+  }
+  if (w.live && !w.last(a)) {
+#pragma unroll
+    for (int k = 0; k < kChannels; ++k)
+      store_word(a.maps + map_row<kBackward>(a, w.b, w.place) + w.c + k,
+                 word_of(A[k]) | uint64_t(word_of(B[k])) << 32);
+  }
+  sh.wholeA[n & 1][lane] = A;
+  sh.wholeB[n & 1][lane] = B;
+  signal(&sh.whole);
+}
+
+// A run's rows of one tensor.  Tokens beyond the sequence repeat its last one;
+// what is made of them is neutral or not stored.
+template <typename T, int kChannels, int kRun>
+struct Rows {
+  Vec<T, kChannels> v[kRun];
+  __device__ __forceinline__ void load(const void* base, int64_t batch, int64_t token, int64_t b,
+                                       int64_t t0, int64_t c, int count, int64_t tokens) {
+    const T* p = static_cast<const T*>(base) + b * batch + c;
+    if (count == kRun) {
+      p += t0 * token;
+#pragma unroll
+      for (int i = 0; i < kRun; ++i) v[i] = load_channels<T, kChannels>(p + i * token);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kRun; ++i) {
+        const int64_t t = t0 + i < tokens ? t0 + i : tokens - 1;
+        v[i] = load_channels<T, kChannels>(p + t * token);
       }
     }
+  }
+};
+
+template <typename T, int kChannels>
+__global__ __launch_bounds__(kThreads, 4) void scan_fwd_kernel(ScanArgs a) {
+  using Channels = FloatVec<kChannels>;
+  constexpr int kRun = Shape<false>::kRun;
+  __shared__ Shared<kChannels> sh;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (threadIdx.x == 0) {
+    sh.ticket[0] = next_ticket(a, 0);
+    sh.ticket[1] = sh.ticket[0] < a.items ? next_ticket(a, 1) : a.items;
+    sh.runs = sh.whole = 0;
+  }
+  __syncthreads();
+  if (wave == kWaves) {
+    look_wave<false, kChannels>(a, sh, a.state);
+    return;
+  }
+  Rows<T, kChannels, kRun> x, g;
+  const auto fetch = [&](uint32_t item) {
+    if (item >= a.items) return;
+    const Item<false, kChannels> w(a, item, wave, lane);
+    x.load(a.x, a.x_batch, a.x_token, w.b, w.t0, w.c, w.count, a.tokens);
+    g.load(a.gate, a.gate_batch, a.gate_token, w.b, w.t0, w.c, w.count, a.tokens);
+  };
+  fetch(sh.ticket[0]);
+  for (uint32_t n = 0;; ++n) {
+    const uint32_t item = sh.ticket[n & 3];
+    if (item >= a.items) return;
+    const Item<false, kChannels> w(a, item, wave, lane);
+    Channels ga[kRun], gb[kRun];  // a and (1 - a) x
 #pragma unroll
-    for (int i = 0; i < kRun; ++i) {
-      ga[i] = Channels(1.0f);
-      keep[i] = gap[i] = Channels(0.0f);
-      if (w.live && i < w.count) {
+    for (int i = 0; i < kRun; ++i)
 #pragma unroll
-        for (int n = 0; n < kChannels; ++n) {
-          const Gate gt = gate_of<T>(float(g[i][n]));
-          ga[i][n] = gt.a;
-          keep[i][n] = gt.keep;
-          gap[i][n] = float(x[i][n]);
+      for (int k = 0; k < kChannels; ++k) {
+        const Gate gt = gate_of<T>(float(g.v[i][k]));
+        ga[i][k] = gt.a;
+        gb[i][k] = gt.keep * float(x.v[i][k]);
+      }
+    fetch(sh.ticket[(n + 1) & 3]);
+    if (w.count < kRun) {
+#pragma unroll
+      for (int i = 0; i < kRun; ++i)
+        if (i >= w.count) {
+          ga[i] = Channels(1.0f);
+          gb[i] = Channels(0.0f);
         }
+    }
+    Channels A(1.0f), B(0.0f);
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+      B = fma<kChannels>(ga[i], B, gb[i]);
+      A *= ga[i];
+    }
+    sh.mapA[n & 1][wave][lane] = A;
+    sh.mapB[n & 1][wave][lane] = B;
+    signal(&sh.runs);
+    if (wave == 0) publish_map<false, kChannels>(a, w, sh, n);
+    __syncthreads();
+    Channels h = sh.before[n & 1][lane];
+    for (int i = 0; i < wave; ++i)
+      h = fma<kChannels>(sh.mapA[n & 1][i][lane], h, sh.mapB[n & 1][i][lane]);
+    T* py = static_cast<T*>(a.y) + (w.b * a.tokens + w.t0) * a.channels + w.c;
+    float* kept = a.ends + end_row<false>(a, w.b, w.place) + w.c;
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+      // States at the starts of the backward's chunks; the one at this chunk's
+      // own start, after place 0, is published by the looking wave.
+      const int t = wave * kRun + i;
+      static_assert(kStarts == 2);
+      if ((t == kStartTokens || (t == 0 && w.place == 0)) && i < w.count && w.live) {
+#pragma unroll
+        for (int k = 0; k < kChannels; ++k) kept[t / kStartTokens * a.channels + k] = h[k];
+      }
+      h = fma<kChannels>(ga[i], h, gb[i]);
+      if (i < w.count && w.live) store_channels<T, kChannels>(py + i * a.channels, h);
+    }
+    if (w.count > 0 && w.t0 + w.count == a.tokens && w.live) {
+#pragma unroll
+      for (int k = 0; k < kChannels; ++k) a.last[w.b * a.channels + w.c + k] = h[k];
+    }
+  }
+}
+
+// Backward, the tokens last to first.  sh.mapA: the runs' gates' products, in both
+// directions; sh.mapB: backward maps of the carried gradient; mapH: forward maps of h.
+template <typename T, int kChannels>
+__global__ __launch_bounds__(kThreads, 4) void scan_bwd_kernel(ScanArgs a) {
+  using Channels = FloatVec<kChannels>;
+  constexpr int kRun = Shape<true>::kRun;
+  __shared__ Shared<kChannels> sh;
+  __shared__ Channels mapH[2][kWaves][kWave];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (threadIdx.x == 0) {
+    sh.ticket[0] = next_ticket(a, 0);
+    sh.ticket[1] = sh.ticket[0] < a.items ? next_ticket(a, 1) : a.items;
+    sh.runs = sh.whole = 0;
+  }
+  __syncthreads();
+  if (wave == kWaves) {
+    look_wave<true, kChannels>(a, sh, a.grad_last);
+    return;
+  }
+  Rows<T, kChannels, kRun> x, g, d;
+  const auto fetch = [&](uint32_t item) {
+    if (item >= a.items) return;
+    const Item<true, kChannels> w(a, item, wave, lane);
+    x.load(a.x, a.x_batch, a.x_token, w.b, w.t0, w.c, w.count, a.tokens);
+    g.load(a.gate, a.gate_batch, a.gate_token, w.b, w.t0, w.c, w.count, a.tokens);
+    if (a.grad_y)
+      d.load(a.grad_y, a.grad_batch, a.grad_token, w.b, w.t0, w.c, w.count, a.tokens);
+  };
+  if (!a.grad_y) {
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) d.v[i] = Vec<T, kChannels>(T(0.0f));
+  }
+  fetch(sh.ticket[0]);
+  for (uint32_t n = 0;; ++n) {
+    const uint32_t item = sh.ticket[n & 3];
+    if (item >= a.items) return;
+    const Item<true, kChannels> w(a, item, wave, lane);
+    Channels h = load_state<kChannels>(a.starts, map_row<true>(a, w.b, w.place) + w.c);
+    Channels ga[kRun], keep[kRun], gap[kRun];  // gap: x, later h_{t-1} - x
+    Vec<T, kChannels> dy[kRun];
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+      dy[i] = d.v[i];
+#pragma unroll
+      for (int k = 0; k < kChannels; ++k) {
+        const Gate gt = gate_of<T>(float(g.v[i][k]));
+        ga[i][k] = gt.a;
+        keep[i][k] = gt.keep;
+        gap[i][k] = float(x.v[i][k]);
       }
     }
-  }
-  Channels A(1.0f), B(0.0f), R(0.0f);
+    fetch(sh.ticket[(n + 1) & 3]);
+    if (w.count < kRun) {
 #pragma unroll
-  for (int i = 0; i < kRun; ++i) {
-    A *= ga[i];
-#pragma unroll
-    for (int n = 0; n < kChannels; ++n) {
-      // Token i's gradient reaches the run's start through a_0 .. a_i.
-      R[n] = __builtin_fmaf(A[n], float(dy[i][n]), R[n]);
-      B[n] = __builtin_fmaf(ga[i][n], B[n], keep[i][n] * gap[i][n]);
+      for (int i = 0; i < kRun; ++i)
+        if (i >= w.count) {
+          ga[i] = Channels(1.0f);
+          keep[i] = gap[i] = Channels(0.0f);
+          dy[i] = Vec<T, kChannels>(T(0.0f));
+        }
     }
-  }
-  mapA[w.wave][w.lane] = A;
-  mapB[w.wave][w.lane] = B;
-  mapR[w.wave][w.lane] = R;
-  __syncthreads();
-  if (w.wave == kWaves - 1) {
-    for (int i = kWaves - 2; i >= 0; --i) {
-      R = fma<kChannels>(mapA[i][w.lane], R, mapR[i][w.lane]);
-      A *= mapA[i][w.lane];
+    Channels A(1.0f), B(0.0f), R(0.0f);
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+      A *= ga[i];
+#pragma unroll
+      for (int k = 0; k < kChannels; ++k) {
+        // Token i's gradient reaches the run's start through a_0 .. a_i.
+        R[k] = __builtin_fmaf(A[k], float(dy[i][k]), R[k]);
+        B[k] = __builtin_fmaf(ga[i][k], B[k], keep[i][k] * gap[i][k]);
+      }
     }
-    const bool more = w.place + 1 < a.chunks;
-    if (w.live && more) {
+    sh.mapA[n & 1][wave][lane] = A;
+    sh.mapB[n & 1][wave][lane] = R;
+    mapH[n & 1][wave][lane] = B;
+    signal(&sh.runs);
+    if (wave == kWaves - 1) publish_map<true, kChannels>(a, w, sh, n);
+    // While the looking wave is at work, the states: gap becomes h_{t-1} - x.
+    await(&sh.runs, (n + 1) * kWaves);
+    for (int i = 0; i < wave; ++i)
+      h = fma<kChannels>(sh.mapA[n & 1][i][lane], h, mapH[n & 1][i][lane]);
 #pragma unroll
-      for (int n = 0; n < kChannels; ++n)
-        store_word(a.maps + at + n, word_of(A[n]) | uint64_t(word_of(R[n])) << 32);
+    for (int i = 0; i < kRun; ++i) {
+      const Channels next = fma<kChannels>(ga[i], h, keep[i] * gap[i]);
+      gap[i] = h - gap[i];
+      h = next;
     }
-    const Channels init = load_state<kChannels>(a.grad_last, w.b * a.channels + w.c, w.live);
-    const Channels r = look_back<true, kChannels>(a, w.b, w.place, w.c, w.live, init);
-    const Channels end = fma<kChannels>(A, r, R);
-    if (w.live && more) {
-      Words<kChannels> v;
+    __syncthreads();
+    Channels r = sh.before[n & 1][lane];
+    for (int i = kWaves - 1; i > wave; --i)
+      r = fma<kChannels>(sh.mapA[n & 1][i][lane], r, sh.mapB[n & 1][i][lane]);
+    const int64_t row = (w.b * a.tokens + w.t0) * a.channels + w.c;
+    T* pdx = static_cast<T*>(a.grad_x) + row;
+    T* pdg = static_cast<T*>(a.grad_gate) + row;
 #pragma unroll
-      for (int n = 0; n < kChannels; ++n) v.w[n] = word_of(end[n]);
-      v.store(a.ends + at - a.channels);
-    }
-    after[w.lane] = r;
-  }
-  // Meanwhile the states: gap becomes h_{t-1} - x.
-  Channels h = load_state<kChannels>(a.starts, at, w.live);
-  for (int i = 0; i < w.wave; ++i) h = fma<kChannels>(mapA[i][w.lane], h, mapB[i][w.lane]);
-#pragma unroll
-  for (int i = 0; i < kRun; ++i) {
-    const Channels next = fma<kChannels>(ga[i], h, keep[i] * gap[i]);
-    gap[i] = h - gap[i];
-    h = next;
-  }
-  __syncthreads();
-  if (!w.live) return;
-  Channels r = after[w.lane];
-  for (int i = kWaves - 1; i > w.wave; --i) r = fma<kChannels>(mapA[i][w.lane], r, mapR[i][w.lane]);
-  const int64_t row = (w.b * a.tokens + w.t0) * a.channels + w.c;
-  T* pdx = static_cast<T*>(a.grad_x) + row;
-  T* pdg = static_cast<T*>(a.grad_gate) + row;
-#pragma unroll
-  for (int i = kRun - 1; i >= 0; --i)
-    if (i < w.count) {
+    for (int i = kRun - 1; i >= 0; --i) {
       const Channels G = to_float<T, kChannels>(dy[i]) + r;
-      store_channels<T, kChannels>(pdx + i * a.channels, keep[i] * G);
-      store_channels<T, kChannels>(pdg + i * a.channels, G * gap[i] * (ga[i] * keep[i]));
+      if (i < w.count && w.live) {
+        store_channels<T, kChannels>(pdx + i * a.channels, keep[i] * G);
+        store_channels<T, kChannels>(pdg + i * a.channels, G * gap[i] * (ga[i] * keep[i]));
+      }
       r = ga[i] * G;
     }
-  if (a.grad_state && w.t0 == 0) {
+    if (a.grad_state && w.t0 == 0 && w.live) {
 #pragma unroll
-    for (int n = 0; n < kChannels; ++n) a.grad_state[w.b * a.channels + w.c + n] = r[n];
+      for (int k = 0; k < kChannels; ++k) a.grad_state[w.b * a.channels + w.c + k] = r[k];
+    }
   }
 }
 
@@ -498,7 +601,11 @@ int check_scan(int64_t batch, int64_t tokens, int64_t channels, int32_t type) {
   return GS_OK;
 }
 
-int64_t chunks_of(int64_t tokens) { return (tokens + kChunk - 1) / kChunk; }
+template <bool kBackward>
+int64_t chunks_of(int64_t tokens) {
+  return (tokens + Shape<kBackward>::kChunk - 1) / Shape<kBackward>::kChunk;
+}
+int64_t starts_of(int64_t tokens) { return (tokens + kStartTokens - 1) / kStartTokens; }
 
 // Two channels a lane where every row of every tensor allows 4-byte accesses.
 bool pairs(const ScanArgs& a, int32_t type) {
@@ -543,18 +650,24 @@ template <bool kBackward>
 int run_scan(ScanArgs& a, int32_t type, char* workspace, hipStream_t s) {
   const bool two = pairs(a, type);
   const int64_t lanes = two ? 2 * kWave : kWave;
-  const int64_t blocks = (a.channels + lanes - 1) / lanes * a.chunks * a.batch;
-  GS_REQUIRE(blocks < (int64_t(1) << 31), GS_ERR_OVERFLOW, "scan too large");
+  a.chunks = chunks_of<kBackward>(a.tokens);
+  a.starts_count = starts_of(a.tokens);
+  const int64_t items = (a.channels + lanes - 1) / lanes * a.chunks * a.batch;
+  GS_REQUIRE(items < (int64_t(1) << 31), GS_ERR_OVERFLOW, "scan too large");
+  a.items = uint32_t(items);
+  int64_t blocks = items;
   if (a.chunks > 1) {
+    // One workgroup's waves fill a CU.
+    blocks = std::min<int64_t>(items, kComputeUnits);
     const ScanSpace space = scan_space(a.batch, a.chunks, a.channels, kBackward);
     a.ticket = reinterpret_cast<uint32_t*>(workspace + space.ticket);
     a.maps = reinterpret_cast<uint64_t*>(workspace + space.maps);
     if (kBackward) a.ends = reinterpret_cast<float*>(workspace + space.carries);
     GS_TRY(device_flags(s, &a.flags));
-    const int64_t states = a.batch * a.chunks * a.channels;
-    const int64_t words = (states * 3 + 255) / 256;
-    scan_clear_kernel<<<unsigned(std::min<int64_t>(words, 2048)), 256, 0, s>>>(
-        reinterpret_cast<uint32_t*>(a.maps), states * 2, reinterpret_cast<uint32_t*>(a.ends), states,
+    const int64_t maps = a.batch * a.chunks * a.channels * 2;
+    const int64_t ends = a.batch * (kBackward ? a.chunks : a.starts_count) * a.channels;
+    scan_clear_kernel<<<unsigned(std::min<int64_t>((maps + ends + 255) / 256, 2048)), 256, 0, s>>>(
+        reinterpret_cast<uint32_t*>(a.maps), maps, reinterpret_cast<uint32_t*>(a.ends), ends,
         a.ticket);
     GS_TRY(check_launch("gated_scan"));
   }
@@ -562,9 +675,9 @@ int run_scan(ScanArgs& a, int32_t type, char* workspace, hipStream_t s) {
     using T = decltype(v);
     constexpr int kN = decltype(n)::value;
     if constexpr (kBackward)
-      scan_bwd_kernel<T, kN><<<unsigned(blocks), Shape<true>::kThreads, 0, s>>>(a);
+      scan_bwd_kernel<T, kN><<<unsigned(blocks), kThreads, 0, s>>>(a);
     else
-      scan_fwd_kernel<T, kN><<<unsigned(blocks), Shape<false>::kThreads, 0, s>>>(a);
+      scan_fwd_kernel<T, kN><<<unsigned(blocks), kThreads, 0, s>>>(a);
     return check_launch("gated_scan");
   });
 }
@@ -575,13 +688,15 @@ int run_scan(ScanArgs& a, int32_t type, char* workspace, hipStream_t s) {
 using namespace gs;
 
 extern "C" GS_API int64_t gs_gated_scan_chunks(int64_t tokens) {
-  return tokens < 0 ? 0 : chunks_of(tokens);
+  return tokens < 0 ? 0 : starts_of(tokens);
 }
 
 extern "C" GS_API size_t gs_gated_scan_workspace_bytes(int64_t batch, int64_t tokens,
                                                        int64_t channels, int32_t backward) {
   if (batch <= 0 || tokens <= 0 || channels <= 0) return 0;
-  return scan_space(batch, chunks_of(tokens), channels, backward != 0).bytes;
+  return scan_space(batch, backward ? chunks_of<true>(tokens) : chunks_of<false>(tokens), channels,
+                    backward != 0)
+      .bytes;
 }
 
 extern "C" GS_API int gs_gated_scan_fwd(const void* x, const void* gate, const float* state,
@@ -607,7 +722,6 @@ extern "C" GS_API int gs_gated_scan_fwd(const void* x, const void* gate, const f
   a.batch = batch;
   a.tokens = tokens;
   a.channels = channels;
-  a.chunks = chunks_of(tokens);
   a.ends = starts;
   a.state = state;
   a.y = y;
@@ -643,7 +757,6 @@ extern "C" GS_API int gs_gated_scan_bwd(const void* x, const void* gate, const f
   a.batch = batch;
   a.tokens = tokens;
   a.channels = channels;
-  a.chunks = chunks_of(tokens);
   a.starts = starts;
   a.grad_last = grad_last;
   a.grad_x = grad_x;
