@@ -104,7 +104,8 @@ struct ScanArgs {
 constexpr uint32_t kUnset = 0xffffffffu;
 constexpr int kSpinLimit = 1 << 20;
 constexpr int kComputeUnits = 256;
-constexpr int kAhead = 16;  // published words that are requested together
+// Published words that are requested together: starts, and maps.
+constexpr int kSeek = 4, kAhead = 8;
 
 // A float as a word that is not kUnset (a NaN of that pattern becomes another).
 __device__ __forceinline__ uint32_t word_of(float v) {
@@ -192,13 +193,13 @@ __device__ FloatVec<kChannels> look_back(const ScanArgs& a, int64_t b, int64_t p
   FloatVec<kChannels> h = init;
   int64_t from = place;  // down to the nearest place whose start is known
   for (bool found = false; !found && from > 0;) {
-    Words<kChannels> w[kAhead];
+    Words<kChannels> w[kSeek];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i)
+    for (int i = 0; i < kSeek; ++i)
       if (from - i > 0) w[i].load(a.ends + end_row<kBackward>(a, b, from - i) + c);
-    int step = kAhead;
+    int step = kSeek;
 #pragma unroll
-    for (int i = kAhead - 1; i >= 0; --i)
+    for (int i = kSeek - 1; i >= 0; --i)
       if (from - i > 0 && __all(w[i].set())) {
         step = i;
         found = true;
