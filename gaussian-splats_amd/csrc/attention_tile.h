@@ -135,58 +135,91 @@ __device__ __forceinline__ float add_all(const Frag<float>& f, float sum) {
 
 // A [kRows, kDim] tile on its way from global memory through a workgroup's
 // registers into LDS.  Rows outside [0, end) and columns from dim on are zeros.
+// A thread's places are the same in every tile, so a tile inside the tensor
+// takes no address arithmetic but the wave's.
 template <typename T, int kRows, int kDim, int kThreads>
 struct Stage {
   static constexpr int kV = 16 / int(sizeof(T));
   static constexpr int kPerRow = kDim / kV;
-  static constexpr int kCount = kRows * kPerRow / kThreads;
-  static_assert(kRows * kPerRow % kThreads == 0, "whole chunks per thread");
+  static constexpr int kStep = kThreads / kPerRow;  // rows between a thread's chunks
+  static constexpr int kCount = kRows / kStep;
+  static_assert(kThreads % kPerRow == 0 && kRows % kStep == 0, "whole rows per step");
   Vec<T, kV> r[kCount];
+  int row, col;
+  bool in;          // the thread's columns exist
+  uint32_t offset;  // of the thread's first chunk, in bytes
+  int64_t stride;   // of a row, in bytes
 
-  __device__ __forceinline__ void load(const T* base, int64_t stride, int row0, int end, int dim) {
+  __device__ __forceinline__ Stage(int64_t row_stride, int dim)
+      : row(threadIdx.x / kPerRow), col(threadIdx.x % kPerRow * kV), in(col < dim),
+        stride(row_stride * int64_t(sizeof(T))) {
+    offset = uint32_t(row * stride) + uint32_t(col * sizeof(T));
 #pragma unroll
-    for (int i = 0; i < kCount; ++i) {
-      const int chunk = i * kThreads + int(threadIdx.x);
-      const int row = row0 + chunk / kPerRow, col = chunk % kPerRow * kV;
-      r[i] = Vec<T, kV>(T(0.0f));
-      if (row >= 0 && row < end && col < dim)
-        r[i] = *reinterpret_cast<const Vec<T, kV>*>(base + row * stride + col);
+    for (int i = 0; i < kCount; ++i) r[i] = Vec<T, kV>(T(0.0f));
+  }
+  __device__ __forceinline__ void load(const T* base, int row0, int end) {
+    const char* first = reinterpret_cast<const char*>(base) + row0 * stride;
+    if (row0 + kRows <= end) {
+      if (in) {
+#pragma unroll
+        for (int i = 0; i < kCount; ++i)
+          r[i] = *reinterpret_cast<const Vec<T, kV>*>(first + i * kStep * stride + offset);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kCount; ++i) {
+        r[i] = Vec<T, kV>(T(0.0f));
+        if (in && row0 + row + i * kStep < end)
+          r[i] = *reinterpret_cast<const Vec<T, kV>*>(first + i * kStep * stride + offset);
+      }
     }
   }
   __device__ __forceinline__ void store(T* tile) const {
 #pragma unroll
-    for (int i = 0; i < kCount; ++i) {
-      const int chunk = i * kThreads + int(threadIdx.x);
-      *reinterpret_cast<Vec<T, kV>*>(tile + chunk / kPerRow * kPitch<T, kDim> +
-                                     chunk % kPerRow * kV) = r[i];
-    }
+    for (int i = 0; i < kCount; ++i)
+      *reinterpret_cast<Vec<T, kV>*>(tile + (row + i * kStep) * kPitch<T, kDim> + col) = r[i];
   }
 };
 
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.4028235e38f; }
 
+// Whether any lane's fragments hold an infinity or a NaN.
+template <typename T, int kCount>
+__device__ __forceinline__ bool any_not_finite(const Frag<T> (&a)[kCount]) {
+  int none = 0;
+  asm volatile("" : "+v"(none));  // or the compiler looks before the caller's branch
+  bool bad = none != 0;
+#pragma unroll
+  for (int n = 0; n < kCount; ++n)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) bad |= !finite(float(a[n][i]));
+  return __any(bad);
+}
+template <typename T, int kCount>
+__device__ __forceinline__ void drop_not_finite(Frag<T> (&a)[kCount]) {
+#pragma unroll
+  for (int n = 0; n < kCount; ++n)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[n][i] = finite(float(a[n][i])) ? a[n][i] : T(0.0f);
+}
+
 // Infinities and NaN at places that some columns of a tile do not see.  In a
 // product those columns hold a zero there, but zero times such a value is a NaN.
-// So guard() takes them out of the first operand, and marks by two bits for each
-// element of the result what they add to the columns that do see them; apply()
-// adds that at the end.  The other columns keep the bits that they would have.
+// So they are dropped from the first operand, and mark() notes by two bits for
+// each element of the result what they add to the columns that do see them;
+// apply() adds that at the end.  The other columns keep the bits that they would
+// have.
 template <typename T, int kCount>
 struct Poison {
   uint32_t marks[kCount] = {};  // +inf: bit r, -inf: bit 16 + r, NaN: both
 
-  // a[n]: the turned fragments of rows row0 .. row0 + 15 and columns 32 n .. of
-  // the tile, which are multiplied with b; seen(k): whether the lane's column
-  // takes row row0 + k.  Marks are made element by element: the code is small
-  // and needs few registers beside the caller's.
+  // For rows row0 .. row0 + 15 and columns 32 n .. of the tile, which are
+  // multiplied with b; seen(k): whether the lane's column takes row row0 + k.
+  // Marks are made element by element: the code is small and needs few
+  // registers beside the caller's.
   template <typename F>
-  __device__ __forceinline__ void guard(const T* tile, int pitch, int row0, Frag<T> (&a)[kCount],
-                                        const Frag<T>& b, F&& seen) {
-    bool bad = false;
-#pragma unroll
-    for (int n = 0; n < kCount; ++n)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) bad |= !finite(float(a[n][i]));
-    if (__builtin_expect(!__any(bad), 1)) return;
+  __device__ __forceinline__ void mark(const T* tile, int pitch, int row0, const Frag<T>& b,
+                                       F&& seen) {
     const int lane = threadIdx.x & 63;
 #pragma unroll 1
     for (int k = 0; k < 16; ++k) {
@@ -206,10 +239,14 @@ struct Poison {
         }
       }
     }
-#pragma unroll
-    for (int n = 0; n < kCount; ++n)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) a[n][i] = finite(float(a[n][i])) ? a[n][i] : T(0.0f);
+  }
+  // mark() and the dropping for a single second operand.
+  template <typename F>
+  __device__ __forceinline__ void guard(const T* tile, int pitch, int row0, Frag<T> (&a)[kCount],
+                                        const Frag<T>& b, F&& seen) {
+    if (__builtin_expect(!any_not_finite<T>(a), 1)) return;
+    mark(tile, pitch, row0, b, seen);
+    drop_not_finite<T>(a);
   }
   __device__ __forceinline__ void apply(Acc (&acc)[kCount]) const {
     uint32_t any = 0;

@@ -30,13 +30,18 @@ struct ForwardArgs {
 
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
-constexpr int kQueries = 32 * kWaves;  // of a workgroup
-constexpr int kKeys = 64;              // of a tile
+constexpr int kKeys = 64;  // of a tile
 
-template <typename T, int kDim>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fwd_kernel(ForwardArgs a) {
+// kTiles: tiles of 32 queries that a wave holds.
+template <typename T, int kDim, int kTiles>
+constexpr int kWavesPerSimd = sizeof(T) == 2 && kDim * kTiles <= 128 ? 2 : 1;
+
+template <typename T, int kDim, int kTiles>
+__global__ __launch_bounds__(kThreads, (kWavesPerSimd<T, kDim, kTiles>)) void attention_fwd_kernel(
+    ForwardArgs a) {
   constexpr int kPitchT = kPitch<T, kDim>;
   constexpr int kSteps = kDim / 16, kBlocks = kDim / 32;
+  constexpr int kQueries = 32 * kTiles * kWaves;  // of a workgroup
   __shared__ __align__(16) T tiles[2][2][kKeys * kPitchT];
   const Problem& p = a.p;
   const int blocks = (p.queries + kQueries - 1) / kQueries;
@@ -52,15 +57,17 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
   const int length = p.length(b);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
-  const int i = block * kQueries + wave * 32 + (lane & 31);  // the lane's query
-  const int pos = p.offset() + i;
-  Frag<T> q[kSteps];
-  {
+  const int i0 = block * kQueries + wave * 32 * kTiles + (lane & 31);  // the lane's first query
+  const int pos = p.offset() + i0;
+  Frag<T> q[kTiles][kSteps];
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t) {
+    const int i = i0 + 32 * t;
     const T* row = static_cast<const T*>(a.q) + b * a.sq.batch + i * a.sq.token + head * a.sq.head;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       const int d = 16 * s + 8 * (lane >> 5);
-      q[s] = load_global<T>(row + d, i < p.queries && d < p.dim);
+      q[t][s] = load_global<T>(row + d, i < p.queries && d < p.dim);
     }
   }
   const T* kbase = static_cast<const T*>(a.k) + b * a.sk.batch + kv * a.sk.head;
@@ -75,18 +82,23 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
   tail -= head_tiles;
 
   const float c = p.scale * kLog2e;
-  const int wave_first = first + wave * 32, wave_last = wave_first + 31;
-  float top = -INFINITY, sum = 0.0f;
-  Acc o[kBlocks];
+  const int wave_first = first + wave * 32 * kTiles, wave_last = wave_first + 32 * kTiles - 1;
+  float top[kTiles], sum[kTiles];
+  Acc o[kTiles][kBlocks];
+  Poison<T, kBlocks> poison[kTiles];
 #pragma unroll
-  for (int n = 0; n < kBlocks; ++n) o[n] = Acc(0.0f);
+  for (int t = 0; t < kTiles; ++t) {
+    top[t] = -INFINITY;
+    sum[t] = 0.0f;
+#pragma unroll
+    for (int n = 0; n < kBlocks; ++n) o[t][n] = Acc(0.0f);
+  }
 
-  Poison<T, kBlocks> poison;
-  Stage<T, kKeys, kDim, kThreads> sk, sv;
+  Stage<T, kKeys, kDim, kThreads> sk(a.sk.token, p.dim), sv(a.sv.token, p.dim);
   const auto fetch = [&](int it) {
     const int j0 = (it < head_tiles ? it : tail + it) * kKeys;
-    sk.load(kbase, a.sk.token, j0, length, p.dim);
-    sv.load(vbase, a.sv.token, j0, length, p.dim);
+    sk.load(kbase, j0, length);
+    sv.load(vbase, j0, length);
   };
   if (count > 0) {
     fetch(0);
@@ -95,64 +107,90 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
   }
   __syncthreads();
   for (int it = 0; it < count; ++it) {
-    const int j0 = (it < head_tiles ? it : tail + it) * kKeys, j1 = j0 + kKeys - 1;
     if (it + 1 < count) fetch(it + 1);
     const T* kt = tiles[it & 1][0];
     const T* vt = tiles[it & 1][1];
-    const bool any = j0 <= wave_last && j0 < length && (j1 > wave_first - p.window || j0 < p.sinks);
-    const bool all = j1 <= wave_first && j1 < length && (j0 > wave_last - p.window || j1 < p.sinks);
-    if (any) {
-      Acc s[2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        s[h] = Acc(0.0f);
+    for (int h = 0; h < kKeys / 32; ++h) {
+      const int j0 = (it < head_tiles ? it : tail + it) * kKeys + 32 * h, j1 = j0 + 31;
+      const bool any = j0 <= wave_last && j0 < length && (j1 > wave_first - p.window || j0 < p.sinks);
+      const bool all = j1 <= wave_first && j1 < length && (j0 > wave_last - p.window || j1 < p.sinks);
+      if (any) {
+        Acc s[kTiles];
 #pragma unroll
-        for (int st = 0; st < kSteps; ++st)
-          mma(load_rows<T>(kt, kPitchT, 32 * h, 16 * st), q[st], s[h]);
-      }
-      if (!all) {
-        const KeySight sight(p, pos, j0 + 4 * (lane >> 5), length);
+        for (int t = 0; t < kTiles; ++t) s[t] = Acc(0.0f);
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int st = 0; st < kSteps; ++st) {
+          const Frag<T> kf = load_rows<T>(kt, kPitchT, 32 * h, 16 * st);
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (!sight.sees(32 * h + acc_row_of_half(r))) s[h][r] = -INFINITY;
-      }
-      float m = fmaxf(s[0][0], s[1][0]);
+          for (int t = 0; t < kTiles; ++t) mma(kf, q[t][st], s[t]);
+        }
+        if (!all) {
 #pragma unroll
-      for (int r = 1; r < 16; ++r) m = fmaxf(fmaxf(m, s[0][r]), s[1][r]);
-      m = fmaxf(m, __shfl_xor(m, 32, 64)) * c;
-      // The maximum that exponents are taken against follows the true one at a
-      // distance of up to 2^8, so that most tiles rescale nothing.
-      if (__any(m > top + 8.0f)) {
-        const float up = m > top + 8.0f ? m : top;
-        float shrink = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - up);
-        asm volatile("" : "+v"(shrink));  // or the compiler rescales without the branch
-        sum *= shrink;
+          for (int t = 0; t < kTiles; ++t) {
+            const KeySight sight(p, pos + 32 * t, j0 + 4 * (lane >> 5), length);
 #pragma unroll
-        for (int n = 0; n < kBlocks; ++n) o[n] *= shrink;
-        top = up;
-      }
-      const float base = top == -INFINITY ? 0.0f : top;
+            for (int r = 0; r < 16; ++r)
+              if (!sight.sees(acc_row_of_half(r))) s[t][r] = -INFINITY;
+          }
+        }
+        float m[kTiles];
+        bool grows = false;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+        for (int t = 0; t < kTiles; ++t) {
+          m[t] = s[t][0];
+#pragma unroll
+          for (int r = 1; r < 16; ++r) m[t] = fmaxf(m[t], s[t][r]);
+          m[t] *= c;
+          grows |= m[t] > top[t] + 8.0f;
+        }
+        // The maximum that exponents are taken against follows the true one at a
+        // distance of up to 2^8, so that most tiles rescale nothing, and need
+        // nothing of the half of the scores that the lane's other half holds.
+        if (__any(grows)) {
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t) {
+            const float whole = fmaxf(m[t], __shfl_xor(m[t], 32, 64));
+            const float up = whole > top[t] + 8.0f ? whole : top[t];
+            float shrink = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[t] - up);
+            asm volatile("" : "+v"(shrink));  // or the compiler rescales without the branch
+            sum[t] *= shrink;
+#pragma unroll
+            for (int n = 0; n < kBlocks; ++n) o[t][n] *= shrink;
+            top[t] = up;
+          }
+        }
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
-#pragma unroll
-          for (int r = 8 * st; r < 8 * st + 8; ++r) s[h][r] = power<T>(s[h][r] * c - base);
-          const Frag<T> pf = acc_frag<T>(s[h], st);
-          sum = add_all(pf, sum);
-          Frag<T> vf[kBlocks];
+          Frag<T> pf[kTiles], vf[kBlocks];
 #pragma unroll
           for (int n = 0; n < kBlocks; ++n)
             vf[n] = load_turned<T>(vt, kPitchT, 32 * h + 16 * st, 32 * n);
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t) {
+            const float base = top[t] == -INFINITY ? 0.0f : top[t];
+#pragma unroll
+            for (int r = 8 * st; r < 8 * st + 8; ++r) s[t][r] = power<T>(s[t][r] * c - base);
+            pf[t] = acc_frag<T>(s[t], st);
+            sum[t] = add_all(pf[t], sum[t]);
+          }
           if (!all) {
-            const KeySight sight(p, pos, j0 + 32 * h + 16 * st, length);
-            poison.guard(vt, kPitchT, 32 * h + 16 * st, vf, pf, [&](int e) { return sight.sees(e); });
+            if (__builtin_expect(any_not_finite<T>(vf), 0)) {
+#pragma unroll
+              for (int t = 0; t < kTiles; ++t) {
+                const KeySight sight(p, pos + 32 * t, j0 + 16 * st, length);
+                poison[t].mark(vt, kPitchT, 32 * h + 16 * st, pf[t],
+                               [&](int e) { return sight.sees(e); });
+              }
+              drop_not_finite<T>(vf);
+            }
           }
 #pragma unroll
-          for (int n = 0; n < kBlocks; ++n) mma(vf[n], pf, o[n]);
+          for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int n = 0; n < kBlocks; ++n) mma(vf[n], pf[t], o[t][n]);
         }
+      }
     }
     if (it + 1 < count) {
       sk.store(tiles[(it + 1) & 1][0]);
@@ -160,24 +198,38 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
     }
     __syncthreads();
   }
-  poison.apply(o);
-  if (i >= p.queries) return;
-  sum += __shfl_xor(sum, 32, 64);
-  const float inverse = top == -INFINITY && sum == 0.0f ? 0.0f : 1.0f / sum;
-  T* out = static_cast<T*>(a.out) + ((int64_t(b) * p.queries + i) * p.heads + head) * p.dim;
 #pragma unroll
-  for (int n = 0; n < kBlocks; ++n)
+  for (int t = 0; t < kTiles; ++t) {
+    const int i = i0 + 32 * t;
+    poison[t].apply(o[t]);
+    const float l = sum[t] + __shfl_xor(sum[t], 32, 64);
+    if (i >= p.queries) continue;
+    const float inverse = top[t] == -INFINITY && l == 0.0f ? 0.0f : 1.0f / l;
+    T* out = static_cast<T*>(a.out) + ((int64_t(b) * p.queries + i) * p.heads + head) * p.dim;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = 32 * n + 8 * g + 4 * (lane >> 5);
-      FloatVec<4> f;
+    for (int n = 0; n < kBlocks; ++n)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) f[r] = o[n][4 * g + r] * inverse;
-      if (d < p.dim) *reinterpret_cast<Vec<T, 4>*>(out + d) = from_float<T, 4>(f);
-    }
-  if (lane < 32)
-    a.lse[(int64_t(b) * p.heads + head) * p.queries + i] =
-        top == -INFINITY ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) / kLog2e;
+      for (int g = 0; g < 4; ++g) {
+        const int d = 32 * n + 8 * g + 4 * (lane >> 5);
+        FloatVec<4> f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) f[r] = o[t][n][4 * g + r] * inverse;
+        if (d < p.dim) *reinterpret_cast<Vec<T, 4>*>(out + d) = from_float<T, 4>(f);
+      }
+    if (lane < 32)
+      a.lse[(int64_t(b) * p.heads + head) * p.queries + i] =
+          top[t] == -INFINITY ? -INFINITY : (top[t] + __builtin_amdgcn_logf(l)) / kLog2e;
+  }
+}
+
+template <typename T, int kDim, int kTiles>
+int launch_forward(const ForwardArgs& a, hipStream_t s) {
+  constexpr int kQueries = 32 * kTiles * kWaves;
+  const int64_t items =
+      (int64_t(a.p.queries) + kQueries - 1) / kQueries * a.p.heads * a.p.batch;
+  GS_REQUIRE(items < (int64_t(1) << 30), GS_ERR_OVERFLOW, "attention problem too large");
+  attention_fwd_kernel<T, kDim, kTiles><<<unsigned(xcd_grid(items)), kThreads, 0, s>>>(a);
+  return check_launch("window_attention");
 }
 
 }  // namespace
@@ -251,15 +303,9 @@ extern "C" GS_API int gs_window_attention_fwd(const gs_attention* desc, const vo
                 {strides[3], strides[4], strides[5]},
                 {strides[6], strides[7], strides[8]},
                 out, lse};
-  const int64_t blocks = (desc->queries + kQueries - 1) / kQueries * desc->heads * desc->batch;
-  GS_REQUIRE(blocks < (int64_t(1) << 30), GS_ERR_OVERFLOW, "attention problem too large");
-  const unsigned grid = unsigned(att::xcd_grid(blocks));
   return seq::with_type(desc->type, [&](auto t) {
     using T = decltype(t);
-    if (desc->head_dim <= 64)
-      attention_fwd_kernel<T, 64><<<grid, kThreads, 0, as_stream(stream)>>>(a);
-    else
-      attention_fwd_kernel<T, 128><<<grid, kThreads, 0, as_stream(stream)>>>(a);
-    return check_launch("window_attention");
+    if (desc->head_dim <= 64) return launch_forward<T, 64, 1>(a, as_stream(stream));
+    return launch_forward<T, 128, 1>(a, as_stream(stream));
   });
 }

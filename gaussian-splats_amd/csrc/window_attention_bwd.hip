@@ -131,15 +131,13 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
   const float c = p.scale * kLog2e;
 
   Poison<T, kBlocks> pk, pv;
-  Stage<T, kRows, kDim, kThreads> sq, sg;
+  Stage<T, kRows, kDim, kThreads> sq(a.sq.token, p.dim), sg(a.sg.token, p.dim);
   float row_lse = 0.0f, row_delta = 0.0f;
   const auto fetch = [&](int it) {
     const int head = kv * group + it / tiles_per_head;
     const int i0 = (first_tile + it % tiles_per_head) * kRows;
-    sq.load(static_cast<const T*>(a.q) + b * a.sq.batch + head * a.sq.head, a.sq.token, i0,
-            p.queries, p.dim);
-    sg.load(static_cast<const T*>(a.grad) + b * a.sg.batch + head * a.sg.head, a.sg.token, i0,
-            p.queries, p.dim);
+    sq.load(static_cast<const T*>(a.q) + b * a.sq.batch + head * a.sq.head, i0, p.queries);
+    sg.load(static_cast<const T*>(a.grad) + b * a.sg.batch + head * a.sg.head, i0, p.queries);
     if (threadIdx.x < kRows) {
       const int i = i0 + threadIdx.x;
       const int64_t at = (int64_t(b) * p.heads + head) * p.queries + i;
@@ -339,11 +337,11 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
   const T* kbase = static_cast<const T*>(a.k) + b * a.sk.batch + kv * a.sk.head;
   const T* vbase = static_cast<const T*>(a.v) + b * a.sv.batch + kv * a.sv.head;
   Poison<T, kBlocks> poison;
-  Stage<T, kRows, kDim, kThreads> sk, sv;
+  Stage<T, kRows, kDim, kThreads> sk(a.sk.token, p.dim), sv(a.sv.token, p.dim);
   const auto fetch = [&](int it) {
     const int j0 = (it < head_tiles ? it : tail + it) * kRows;
-    sk.load(kbase, a.sk.token, j0, length, p.dim);
-    sv.load(vbase, a.sv.token, j0, length, p.dim);
+    sk.load(kbase, j0, length);
+    sv.load(vbase, j0, length);
   };
   if (count > 0) {
     fetch(0);
