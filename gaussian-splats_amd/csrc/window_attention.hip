@@ -34,7 +34,7 @@ constexpr int kKeys = 64;  // of a tile
 
 // kTiles: tiles of 32 queries that a wave holds.
 template <typename T, int kDim, int kTiles>
-constexpr int kWavesPerSimd = sizeof(T) == 2 && kDim * kTiles <= 128 ? 2 : 1;
+constexpr int kWavesPerSimd = sizeof(T) == 2 && sizeof(T) == 2 && kDim * kTiles <= 64 ? 4 : sizeof(T) == 2 && kDim * kTiles <= 128 ? 2 : 1;
 
 template <typename T, int kDim, int kTiles>
 __global__ __launch_bounds__(kThreads, (kWavesPerSimd<T, kDim, kTiles>)) void attention_fwd_kernel(
@@ -115,7 +115,7 @@ __global__ __launch_bounds__(kThreads, (kWavesPerSimd<T, kDim, kTiles>)) void at
       const int j0 = (it < head_tiles ? it : tail + it) * kKeys + 32 * h, j1 = j0 + 31;
       const bool any = j0 <= wave_last && j0 < length && (j1 > wave_first - p.window || j0 < p.sinks);
       const bool all = j1 <= wave_first && j1 < length && (j0 > wave_last - p.window || j1 < p.sinks);
-      if (any) {
+      if (__builtin_expect(any, 1)) {
         Acc s[kTiles];
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) s[t] = Acc(0.0f);
@@ -125,7 +125,7 @@ __global__ __launch_bounds__(kThreads, (kWavesPerSimd<T, kDim, kTiles>)) void at
 #pragma unroll
           for (int t = 0; t < kTiles; ++t) mma(kf, q[t][st], s[t]);
         }
-        if (!all) {
+        if (__builtin_expect(!all, 0)) {
 #pragma unroll
           for (int t = 0; t < kTiles; ++t) {
             const KeySight sight(p, pos + 32 * t, j0 + 4 * (lane >> 5), length);
@@ -147,7 +147,7 @@ __global__ __launch_bounds__(kThreads, (kWavesPerSimd<T, kDim, kTiles>)) void at
         // The maximum that exponents are taken against follows the true one at a
         // distance of up to 2^8, so that most tiles rescale nothing, and need
         // nothing of the half of the scores that the lane's other half holds.
-        if (__any(grows)) {
+        if (__builtin_expect(__any(grows), 0)) {
 #pragma unroll
           for (int t = 0; t < kTiles; ++t) {
             const float whole = fmaxf(m[t], __shfl_xor(m[t], 32, 64));
@@ -174,7 +174,7 @@ __global__ __launch_bounds__(kThreads, (kWavesPerSimd<T, kDim, kTiles>)) void at
             pf[t] = acc_frag<T>(s[t], st);
             sum[t] = add_all(pf[t], sum[t]);
           }
-          if (!all) {
+          if (__builtin_expect(!all, 0)) {
             if (__builtin_expect(any_not_finite<T>(vf), 0)) {
 #pragma unroll
               for (int t = 0; t < kTiles; ++t) {

@@ -11,9 +11,14 @@
 // share keys are walked one after the other by their keys' workgroup.
 //
 // The first tokens are seen by every later query.  Their keys' walk, far longer
-// than a window, is cut into segments of about a window's length, each a
+// than a window, is cut into segments of about the others' length, each a
 // workgroup of its own that leaves float32 sums, which a last kernel adds in the
-// order of the segments.
+// order of the segments.  Where there are few keys the other walks are cut too.
+// dS is an operand of products in the inputs' type.  float16 would lose small
+// values of it below its normal range and large ones above it, as gradients come
+// in any size (and P is about one over the window): there dS carries a power of
+// two that brings the largest |grad_out| to between 4 and 8, taken out of the
+// sums in float32.
 #include "attention_tile.h"
 
 namespace gs {
@@ -40,13 +45,44 @@ struct BackwardArgs {
   Strides sq, sk, sv, sg;
   const float* lse;
   float* delta;  // [batch, heads, queries]
+  uint32_t* largest;  // float16: the bits of the largest finite |grad_out|
   void* dq;
   void* dk;
   void* dv;
-  // Segments of the workgroups whose keys hold first tokens.
-  float* parts;  // [batch, kv_heads, sink_blocks, segments, 2, kBlockKeys, dim]
-  int sink_blocks, segments, segment;  // segment: queries of one
+  // The walks of the blocks of keys that hold first tokens are cut into
+  // sink_segments, those of the others into segments; more than one leave parts,
+  // each [2, kBlockKeys, dim].
+  float* parts;
+  int sink_blocks, sink_segments, segments;
 };
+
+__host__ __device__ inline int key_blocks(const Problem& p) {
+  return (p.keys + kBlockKeys - 1) / kBlockKeys;
+}
+// Parts of one key head, and the place of one among all.
+__host__ __device__ inline int64_t parts_per_head(const BackwardArgs& a) {
+  return (a.sink_segments > 1 ? int64_t(a.sink_blocks) * a.sink_segments : 0) +
+         (a.segments > 1 ? int64_t(key_blocks(a.p) - a.sink_blocks) * a.segments : 0);
+}
+__device__ __forceinline__ int64_t part_index(const BackwardArgs& a, int b, int kv, int block,
+                                              int segment) {
+  const int64_t head = (int64_t(b) * a.p.kv_heads + kv) * parts_per_head(a);
+  if (block < a.sink_blocks) return head + int64_t(block) * a.sink_segments + segment;
+  const int64_t before = a.sink_segments > 1 ? int64_t(a.sink_blocks) * a.sink_segments : 0;
+  return head + before + int64_t(block - a.sink_blocks) * a.segments + segment;
+}
+
+// The power of two that dS carries.
+template <typename T>
+__device__ __forceinline__ int gradient_shift(const BackwardArgs& a) {
+  if constexpr (std::is_same_v<T, f16>) {
+    const uint32_t bits = *a.largest;
+    if (bits != 0) return 129 - int(bits >> 23);  // 2^(bits >> 23 - 127) to 2^2
+  }
+  return 0;
+}
+
+__global__ void attention_clear_kernel(uint32_t* largest) { *largest = 0; }
 
 // delta, a group of 16 lanes for each row.
 template <typename T>
@@ -55,7 +91,7 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(BackwardArgs a) {
   const int64_t rows = int64_t(p.batch) * p.queries * p.heads;
   const int64_t row = int64_t(blockIdx.x) * 16 + (threadIdx.x >> 4);
   const int d = (threadIdx.x & 15) * 8;
-  float sum = 0.0f;
+  float sum = 0.0f, top = 0.0f;
   const int head = int(row % p.heads);
   const int64_t i = row / p.heads % p.queries, b = row / p.heads / p.queries;
   if (row < rows && d < p.dim) {
@@ -63,7 +99,18 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(BackwardArgs a) {
     const Frag<T> g = load_global<T>(static_cast<const T*>(a.grad) + b * a.sg.batch +
                                          i * a.sg.token + head * a.sg.head + d, true);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum += float(o[e]) * float(g[e]);
+    for (int e = 0; e < 8; ++e) {
+      sum += float(o[e]) * float(g[e]);
+      const float size = fabsf(float(g[e]));
+      top = finite(size) ? fmaxf(top, size) : top;
+    }
+  }
+  if constexpr (std::is_same_v<T, f16>) {
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
+    // A maximum does not depend on the order; most waves find a larger one there.
+    if ((threadIdx.x & 63) == 0 && __float_as_uint(top) > *a.largest)
+      atomicMax(a.largest, __float_as_uint(top));
   }
 #pragma unroll
   for (int s = 8; s > 0; s >>= 1) sum += __shfl_xor(sum, s, 64);
@@ -72,26 +119,28 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(BackwardArgs a) {
 
 // grad_k and grad_v of a workgroup's keys: a wave holds 32, queries walk by.
 template <typename T, int kDim>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) void attention_bwd_keys_kernel(BackwardArgs a) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) void attention_bwd_keys_kernel(
+    BackwardArgs a) {
   constexpr int kRows = kTileRows<T, kDim>;
   constexpr int kPitchT = kPitch<T, kDim>;
   constexpr int kSteps = kDim / 16, kBlocks = kDim / 32;
   __shared__ __align__(16) T tiles[2][2][kRows * kPitchT];
   __shared__ float rows[2][2][kRows];  // lse (in powers of two) and delta
   const Problem& p = a.p;
-  const int blocks = (p.keys + kBlockKeys - 1) / kBlockKeys;
-  // Workgroups of a key head: the segments of the first tokens' blocks, then
+  const int blocks = key_blocks(p);
+  // Items of a key head: the segments of the first tokens' blocks, then those of
   // the other blocks.
-  const int split = a.sink_blocks * a.segments;
-  const int per = split + blocks - a.sink_blocks;
+  const int split = a.sink_blocks * a.sink_segments;
+  const int per = split + (blocks - a.sink_blocks) * a.segments;
   const int64_t total = int64_t(per) * p.kv_heads * p.batch;
   const int64_t id = xcd_order(blockIdx.x, total);
   if (id >= total) return;
   const int item = int(id % per);
   const int kv = int(id / per % p.kv_heads), b = int(id / per / p.kv_heads);
-  const bool part = item < split;
-  const int block = part ? item / a.segments : item - split + a.sink_blocks;
-  const int segment = part ? item % a.segments : 0;
+  const int pieces = item < split ? a.sink_segments : a.segments;
+  const int block = (item < split ? 0 : a.sink_blocks) + (item < split ? item : item - split) / pieces;
+  const int segment = (item < split ? item : item - split) % pieces;
+  const bool part = pieces > 1;
   const int group = p.heads / p.kv_heads;
   const int length = p.length(b);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -111,26 +160,27 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
     }
   }
 
-  // Queries that see any of the keys, cut to the segment.
+  // Queries that see any of the keys, and the walk over their tiles, head after
+  // head, of which the workgroup takes its segment.
   const int off = p.offset();
-  int from = max(0, k0 - off);
-  int to = k0 < p.sinks ? p.queries
-                        : int(min(int64_t(p.queries), int64_t(k0) + kBlockKeys - 1 + p.window - off));
-  if (part) {
-    from = max(from, segment * a.segment);
-    to = min(p.queries, (segment + 1) * a.segment);
-  }
-  if (k0 >= length) to = from;
+  const int from = max(0, k0 - off);
+  const int to = k0 >= length ? from
+                 : k0 < p.sinks
+                     ? p.queries
+                     : int(min(int64_t(p.queries), int64_t(k0) + kBlockKeys - 1 + p.window - off));
   const int first_tile = from / kRows;
   const int tiles_per_head = to > from ? (to - 1) / kRows - first_tile + 1 : 0;
-  const int count = tiles_per_head * group;
+  const int64_t walk = int64_t(tiles_per_head) * group;
+  const int begin = int(walk * segment / pieces), count = int(walk * (segment + 1) / pieces);
 
+  const int shift = gradient_shift<T>(a);
+  const float up = ldexpf(1.0f, shift), down = ldexpf(1.0f, -shift);
   Acc dk[kBlocks], dv[kBlocks];
+  Poison<T, kBlocks> pk, pv;
 #pragma unroll
   for (int n = 0; n < kBlocks; ++n) dk[n] = dv[n] = Acc(0.0f);
   const float c = p.scale * kLog2e;
 
-  Poison<T, kBlocks> pk, pv;
   Stage<T, kRows, kDim, kThreads> sq(a.sq.token, p.dim), sg(a.sg.token, p.dim);
   float row_lse = 0.0f, row_delta = 0.0f;
   const auto fetch = [&](int it) {
@@ -153,12 +203,12 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
       rows[buffer][1][threadIdx.x] = row_delta;
     }
   };
-  if (count > 0) {
-    fetch(0);
-    keep(0);
+  if (begin < count) {
+    fetch(begin);
+    keep(begin & 1);
   }
   __syncthreads();
-  for (int it = 0; it < count; ++it) {
+  for (int it = begin; it < count; ++it) {
     if (it + 1 < count) fetch(it + 1);
     const T* qt = tiles[it & 1][0];
     const T* gt = tiles[it & 1][1];
@@ -166,13 +216,13 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
 #pragma unroll 1
     for (int h = 0; h < kRows / 32; ++h) {
       const int p0 = off + i0 + 32 * h, p1 = p0 + 31;  // positions
-      // Queries outside [from, to) belong to other segments.
       const bool inside = i0 + 32 * h >= from && i0 + 32 * h + 31 < to;
+      const int w1 = w0 + 31;
       const bool any = w0 <= p1 && w0 < length && i0 + 32 * h < to &&
-                       (w0 + 31 > p0 - p.window || w0 < p.sinks);
-      const bool all = inside && w0 + 31 <= p0 && w0 + 31 < length &&
-                       (w0 > p1 - p.window || w0 + 31 < p.sinks);
-      if (any) {
+                       (w1 > p0 - p.window || w0 < p.sinks);
+      const bool all = inside && w1 <= p0 && w1 < length &&
+                       (w0 > p1 - p.window || w1 < p.sinks);
+      if (__builtin_expect(any, 1)) {
         Acc s(0.0f), dp(0.0f);
 #pragma unroll
         for (int st = 0; st < kSteps; ++st)
@@ -186,8 +236,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
           const float lse = rows[it & 1][0][row], delta = rows[it & 1][1][row];
           s[r] = power<T>(s[r] * c - lse);
           dp[r] = s[r] * (dp[r] - delta);
+          if constexpr (std::is_same_v<T, f16>) dp[r] *= up;
         }
-        if (!all) {
+        if (__builtin_expect(!all, 0)) {
           const QuerySight sight(p, j, i0 + 32 * h + 4 * (lane >> 5), from, to, length);
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
@@ -196,25 +247,27 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
             dp[r] = see ? dp[r] : 0.0f;
           }
         }
-#pragma unroll
-        for (int st = 0; st < 2; ++st) {
-          const Frag<T> pf = acc_frag<T>(s, st), df = acc_frag<T>(dp, st);
+        // Two products that contract over the queries: of a tile's turned rows
+        // and the probabilities or their gradients.
+        const auto add = [&](const T* tile, const Acc& x, Poison<T, kBlocks>& poison,
+                             Acc (&acc)[kBlocks], int st) {
+          const Frag<T> xf = acc_frag<T>(x, st);
           Frag<T> f[kBlocks];
 #pragma unroll
           for (int n = 0; n < kBlocks; ++n)
-            f[n] = load_turned<T>(gt, kPitchT, 32 * h + 16 * st, 32 * n);
-          const QuerySight sight(p, j, i0 + 32 * h + 16 * st, from, to, length);
-          if (!all)
-            pv.guard(gt, kPitchT, 32 * h + 16 * st, f, pf, [&](int e) { return sight.sees(e); });
+            f[n] = load_turned<T>(tile, kPitchT, 32 * h + 16 * st, 32 * n);
+          if (__builtin_expect(!all, 0)) {
+            const QuerySight sight(p, j, i0 + 32 * h + 16 * st, from, to, length);
+            poison.guard(tile, kPitchT, 32 * h + 16 * st, f, xf,
+                         [&](int e) { return sight.sees(e); });
+          }
 #pragma unroll
-          for (int n = 0; n < kBlocks; ++n) mma(f[n], pf, dv[n]);
+          for (int n = 0; n < kBlocks; ++n) mma(f[n], xf, acc[n]);
+        };
 #pragma unroll
-          for (int n = 0; n < kBlocks; ++n)
-            f[n] = load_turned<T>(qt, kPitchT, 32 * h + 16 * st, 32 * n);
-          if (!all)
-            pk.guard(qt, kPitchT, 32 * h + 16 * st, f, df, [&](int e) { return sight.sees(e); });
-#pragma unroll
-          for (int n = 0; n < kBlocks; ++n) mma(f[n], df, dk[n]);
+        for (int st = 0; st < 2; ++st) {
+          add(gt, s, pv, dv, st);
+          add(qt, dp, pk, dk, st);
         }
       }
     }
@@ -223,27 +276,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
   }
   pk.apply(dk);
   pv.apply(dv);
-  if (part) {
-    float* at = a.parts + ((((int64_t(b) * p.kv_heads + kv) * a.sink_blocks + block) * a.segments +
-                            segment) * 2 * kBlockKeys + wave * 32 + (lane & 31)) * p.dim;
-#pragma unroll
-    for (int n = 0; n < kBlocks; ++n)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int d = 32 * n + 8 * g + 4 * (lane >> 5);
-        if (d >= p.dim) continue;
-        FloatVec<4> x, y;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          x[r] = dk[n][4 * g + r];
-          y[r] = dv[n][4 * g + r];
-        }
-        *reinterpret_cast<FloatVec<4>*>(at + d) = x;
-        *reinterpret_cast<FloatVec<4>*>(at + kBlockKeys * p.dim + d) = y;
-      }
-    return;
-  }
-  if (j >= p.keys) return;
+  float* part_at = part ? a.parts + (part_index(a, b, kv, block, segment) * 2 * kBlockKeys +
+                                     wave * 32 + (lane & 31)) * p.dim
+                        : nullptr;
+  if (!part && j >= p.keys) return;
   const int64_t row = ((int64_t(b) * p.keys + j) * p.kv_heads + kv) * p.dim;
 #pragma unroll
   for (int n = 0; n < kBlocks; ++n)
@@ -254,35 +290,44 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
       FloatVec<4> x, y;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        x[r] = dk[n][4 * g + r] * p.scale;
+        x[r] = dk[n][4 * g + r] * down;
         y[r] = dv[n][4 * g + r];
       }
-      *reinterpret_cast<Vec<T, 4>*>(static_cast<T*>(a.dk) + row + d) = from_float<T, 4>(x);
-      *reinterpret_cast<Vec<T, 4>*>(static_cast<T*>(a.dv) + row + d) = from_float<T, 4>(y);
+      if (part) {
+        *reinterpret_cast<FloatVec<4>*>(part_at + d) = x;
+        *reinterpret_cast<FloatVec<4>*>(part_at + kBlockKeys * p.dim + d) = y;
+      } else {
+        *reinterpret_cast<Vec<T, 4>*>(static_cast<T*>(a.dk) + row + d) = from_float<T, 4>(x * p.scale);
+        *reinterpret_cast<Vec<T, 4>*>(static_cast<T*>(a.dv) + row + d) = from_float<T, 4>(y);
+      }
     }
 }
 
-// The first tokens' blocks: their segments' sums in order.  One thread for each
-// element of [batch, kv_heads, sink_blocks, kBlockKeys, dim].
+// The blocks that left parts: their segments' sums in order.  One thread for
+// four elements of [batch, kv_heads, blocks, kBlockKeys, dim], of the blocks from
+// `first` on.
 template <typename T>
-__global__ __launch_bounds__(256) void attention_bwd_join_kernel(BackwardArgs a) {
+__global__ __launch_bounds__(256) void attention_bwd_join_kernel(BackwardArgs a, int first,
+                                                                 int blocks) {
   const Problem& p = a.p;
   const int64_t plane = int64_t(kBlockKeys) * p.dim;
-  const int64_t e = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (e >= int64_t(p.batch) * p.kv_heads * a.sink_blocks * plane) return;
-  const int64_t block = e / plane, in = e % plane;
-  const int j = int(block % a.sink_blocks) * kBlockKeys + int(in / p.dim);
+  const int64_t e = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 4;
+  if (e >= int64_t(p.batch) * p.kv_heads * blocks * plane) return;
+  const int64_t in = e % plane, at = e / plane;
+  const int block = first + int(at % blocks);
+  const int kv = int(at / blocks % p.kv_heads), b = int(at / blocks / p.kv_heads);
+  const int j = block * kBlockKeys + int(in / p.dim);
   if (j >= p.keys) return;
-  const int64_t kv = block / a.sink_blocks % p.kv_heads, b = block / a.sink_blocks / p.kv_heads;
-  const float* at = a.parts + block * a.segments * 2 * plane + in;
-  float dk = 0.0f, dv = 0.0f;
-  for (int s = 0; s < a.segments; ++s) {
-    dk += at[2 * s * plane];
-    dv += at[(2 * s + 1) * plane];
+  const float* part = a.parts + part_index(a, b, kv, block, 0) * 2 * plane + in;
+  const int pieces = block < a.sink_blocks ? a.sink_segments : a.segments;
+  FloatVec<4> dk(0.0f), dv(0.0f);
+  for (int s = 0; s < pieces; ++s) {
+    dk += *reinterpret_cast<const FloatVec<4>*>(part + 2 * s * plane);
+    dv += *reinterpret_cast<const FloatVec<4>*>(part + (2 * s + 1) * plane);
   }
-  const int64_t row = ((b * p.keys + j) * p.kv_heads + kv) * p.dim + in % p.dim;
-  static_cast<T*>(a.dk)[row] = T(dk * p.scale);
-  static_cast<T*>(a.dv)[row] = T(dv);
+  const int64_t row = ((int64_t(b) * p.keys + j) * p.kv_heads + kv) * p.dim + in % p.dim;
+  *reinterpret_cast<Vec<T, 4>*>(static_cast<T*>(a.dk) + row) = from_float<T, 4>(dk * p.scale);
+  *reinterpret_cast<Vec<T, 4>*>(static_cast<T*>(a.dv) + row) = from_float<T, 4>(dv);
 }
 
 // grad_q of a workgroup's queries: a wave holds 32, the keys that they see walk by.
@@ -320,7 +365,11 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
     }
   }
   const int64_t at = (int64_t(b) * p.heads + head) * p.queries + i;
-  const float lse = live ? a.lse[at] * kLog2e : 0.0f, delta = live ? a.delta[at] : 0.0f;
+  const int shift = gradient_shift<T>(a);
+  const float down = ldexpf(1.0f, -shift);
+  // P carries dS's power of two.
+  const float lse = live ? a.lse[at] * kLog2e - float(shift) : 0.0f;
+  const float delta = live ? a.delta[at] : 0.0f;
 
   const int first = p.offset() + block * kBlockQueries;
   const int last = min(p.offset() + min((block + 1) * kBlockQueries, p.queries), length) - 1;
@@ -358,7 +407,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
       const int j0 = (it < head_tiles ? it : tail + it) * kRows + 32 * h, j1 = j0 + 31;
       const bool any = j0 <= wave_last && j0 < length && (j1 > wave_first - p.window || j0 < p.sinks);
       const bool all = j1 <= wave_first && j1 < length && (j0 > wave_last - p.window || j1 < p.sinks);
-      if (any) {
+      if (__builtin_expect(any, 1)) {
         Acc s(0.0f), dp(0.0f);
 #pragma unroll
         for (int st = 0; st < kSteps; ++st)
@@ -368,7 +417,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
           mma(load_rows<T>(vt, kPitchT, 32 * h, 16 * st), g[st], dp);
 #pragma unroll
         for (int r = 0; r < 16; ++r) dp[r] = power<T>(s[r] * c - lse) * (dp[r] - delta);
-        if (!all) {
+        if (__builtin_expect(!all, 0)) {
           const KeySight sight(p, pos, j0 + 4 * (lane >> 5), length);
 #pragma unroll
           for (int r = 0; r < 16; ++r) dp[r] = sight.sees(acc_row_of_half(r)) ? dp[r] : 0.0f;
@@ -380,7 +429,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
 #pragma unroll
           for (int n = 0; n < kBlocks; ++n)
             f[n] = load_turned<T>(kt, kPitchT, 32 * h + 16 * st, 32 * n);
-          if (!all) {
+          if (__builtin_expect(!all, 0)) {
             const KeySight sight(p, pos, j0 + 16 * st, length);
             poison.guard(kt, kPitchT, 32 * h + 16 * st, f, df, [&](int e) { return sight.sees(e); });
           }
@@ -405,26 +454,34 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
       const int d = 32 * n + 8 * e + 4 * (lane >> 5);
       FloatVec<4> x;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) x[r] = dq[n][4 * e + r] * p.scale;
+      for (int r = 0; r < 4; ++r) x[r] = dq[n][4 * e + r] * (p.scale * down);
       if (d < p.dim) *reinterpret_cast<Vec<T, 4>*>(out + d) = from_float<T, 4>(x);
     }
 }
 
-// How the first tokens' walk is cut: segments of about as many queries as
-// another workgroup walks.
-void plan_segments(const Problem& p, BackwardArgs& a) {
-  const int blocks = (p.keys + kBlockKeys - 1) / kBlockKeys;
-  a.sink_blocks = std::min(blocks, (p.sinks + kBlockKeys - 1) / kBlockKeys);
-  // Segments start at a tile's first query.
-  a.segment = (p.window + kBlockKeys + 63) / 64 * 64;
-  a.segments = (p.queries + a.segment - 1) / a.segment;
-  if (a.segments <= 1) a.sink_blocks = 0;
+// How the walks are cut.  Where the blocks of keys are fewer than two for each
+// CU, into segments of at least two tiles that make up for it.  The first tokens'
+// walks into segments a quarter as long: most of their tiles are masked, and with
+// segments of the others' length they end last (40000 tokens: 2.41 ms, 1.81 with
+// a quarter).
+void plan_segments(const Problem& p, int32_t type, BackwardArgs& a) {
+  const int64_t blocks = key_blocks(p), rows = type == GS_F32 ? 32 : 64;
+  const int64_t group = p.heads / p.kv_heads;
+  const int64_t reach = std::min<int64_t>(p.queries, int64_t(p.window) + kBlockKeys);
+  const int64_t walk = std::max<int64_t>(1, (reach + rows - 1) / rows * group);
+  const int64_t items = std::max<int64_t>(1, blocks * p.kv_heads * p.batch);
+  a.segments = int(std::max<int64_t>(1, std::min<int64_t>(512 / items, walk / 2)));
+  a.sink_blocks = int(std::min<int64_t>(blocks, (p.sinks + kBlockKeys - 1) / kBlockKeys));
+  const int64_t long_walk = (int64_t(p.queries) + rows - 1) / rows * group;
+  const int64_t piece = std::max<int64_t>(1, walk / a.segments);
+  a.sink_segments = int(std::max<int64_t>(1, std::min<int64_t>(4 * long_walk / piece, 4096)));
 }
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 size_t delta_bytes(const Problem& p) {
-  return align256(size_t(p.batch) * size_t(p.heads) * size_t(p.queries) * sizeof(float));
+  return align256(size_t(p.batch) * size_t(p.heads) * size_t(p.queries) * sizeof(float) +
+                  sizeof(uint32_t));
 }
 
 }  // namespace
@@ -434,11 +491,12 @@ using namespace gs;
 
 extern "C" GS_API size_t gs_window_attention_bwd_workspace_bytes(const gs_attention* desc) {
   if (!desc || check_attention(*desc) != GS_OK) return 0;
-  const Problem p = make_problem(*desc, nullptr);
   BackwardArgs a{};
-  plan_segments(p, a);
-  return delta_bytes(p) + size_t(p.batch) * size_t(p.kv_heads) * size_t(a.sink_blocks) *
-                              size_t(a.segments) * 2 * kBlockKeys * size_t(p.dim) * sizeof(float);
+  a.p = make_problem(*desc, nullptr);
+  const Problem& p = a.p;
+  plan_segments(p, desc->type, a);
+  return delta_bytes(p) + size_t(p.batch) * size_t(p.kv_heads) * size_t(parts_per_head(a)) * 2 *
+                              kBlockKeys * size_t(p.dim) * sizeof(float);
 }
 
 extern "C" GS_API int gs_window_attention_bwd(const gs_attention* desc, const void* q,
@@ -488,15 +546,20 @@ extern "C" GS_API int gs_window_attention_bwd(const gs_attention* desc, const vo
   a.dq = grad_q;
   a.dk = grad_k;
   a.dv = grad_v;
-  plan_segments(a.p, a);
+  plan_segments(a.p, desc->type, a);
   a.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes(a.p));
   const Problem& p = a.p;
   const int64_t rows = int64_t(p.batch) * p.queries * p.heads;
-  const int64_t key_items = (int64_t(p.keys + kBlockKeys - 1) / kBlockKeys - a.sink_blocks +
-                             int64_t(a.sink_blocks) * a.segments) * p.kv_heads * p.batch;
+  a.largest = reinterpret_cast<uint32_t*>(a.delta + rows);
+  const int64_t blocks = key_blocks(p), others = blocks - a.sink_blocks;
+  const int64_t key_items = (int64_t(a.sink_blocks) * a.sink_segments + others * a.segments) *
+                            p.kv_heads * p.batch;
   const int64_t query_items =
       int64_t(p.queries + kBlockQueries - 1) / kBlockQueries * p.heads * p.batch;
-  const int64_t joined = int64_t(p.batch) * p.kv_heads * a.sink_blocks * kBlockKeys * p.dim;
+  // Blocks that leave parts: all, the first tokens' or the others.
+  const int join_first = a.sink_segments > 1 ? 0 : a.sink_blocks;
+  const int join_blocks = int((a.sink_segments > 1 ? a.sink_blocks : 0) + (a.segments > 1 ? others : 0));
+  const int64_t joined = int64_t(p.batch) * p.kv_heads * join_blocks * kBlockKeys * p.dim / 4;
   GS_REQUIRE(rows / 16 < (int64_t(1) << 30) && key_items < (int64_t(1) << 30) &&
                  query_items < (int64_t(1) << 30) && joined / 256 < (int64_t(1) << 30),
              GS_ERR_OVERFLOW, "attention problem too large");
@@ -504,6 +567,7 @@ extern "C" GS_API int gs_window_attention_bwd(const gs_attention* desc, const vo
   return seq::with_type(desc->type, [&](auto t) {
     using T = decltype(t);
     if (rows) {
+      if (std::is_same_v<T, f16>) attention_clear_kernel<<<1, 1, 0, s>>>(a.largest);
       attention_delta_kernel<T><<<unsigned((rows + 15) / 16), 256, 0, s>>>(a);
       GS_TRY(check_launch("window_attention backward"));
     }
@@ -516,7 +580,8 @@ extern "C" GS_API int gs_window_attention_bwd(const gs_attention* desc, const vo
       GS_TRY(check_launch("window_attention backward, keys"));
     }
     if (joined) {
-      attention_bwd_join_kernel<T><<<unsigned((joined + 255) / 256), 256, 0, s>>>(a);
+      attention_bwd_join_kernel<T><<<unsigned((joined + 255) / 256), 256, 0, s>>>(a, join_first,
+                                                                                  join_blocks);
       GS_TRY(check_launch("window_attention backward, first tokens"));
     }
     if (query_items) {

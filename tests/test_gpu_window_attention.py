@@ -186,6 +186,22 @@ def test_large_scores(dtype):
     _check((q * -6).to(dtype), k, v, 70, 1, scale=0.5)
 
 
+@pytest.mark.parametrize("size", [1e-4, 1e-2, 1e3])
+def test_float16_gradients_of_any_size(size):
+    """Gradients far below and above one: relative to their size the result is as
+    exact as for gradients near one."""
+    q, k, v = _inputs(1, 300, 300, 2, 1, 64, torch.float16)
+    grad = normal(q.shape, torch.float32, 9)
+    d = [t.to(DEV).requires_grad_(True) for t in (q, k, v)]
+    out = window_attention(*d, 200, 2)
+    got = torch.autograd.grad(out, d, (grad * size).half().to(DEV))
+    values, bounds = _dense(q, k, v, 200, 2, None, None, (grad * size).half())
+    # grad_out's own subnormals are in both; outputs may add half of one.
+    unit, unit_bounds = _dense(q, k, v, 200, 2, None, None, grad.half())
+    for name, x, y, b in zip(("dq", "dk", "dv"), got, values[1:], unit_bounds[1:]):
+        assert_within(x, y, b * size + 2 * TINY[torch.float16], name)
+
+
 def test_strides():
     """[batch, heads, tokens, dim] tensors, one block of a fused projection, an
     offset that no 16-byte access allows."""
