@@ -80,6 +80,7 @@ int device_flags(hipStream_t stream, uint32_t** flags);
 constexpr uint32_t kDeviceFlagSpinLimit = GS_DEVICE_SPIN_LIMIT;
 constexpr uint32_t kDeviceFlagWindow = GS_DEVICE_WINDOW_OVERFLOW;
 constexpr uint32_t kDeviceFlagSizes = GS_DEVICE_SIZE_MISMATCH;
+constexpr uint32_t kDeviceFlagScan = GS_DEVICE_SCAN_LIMIT;
 
 #define GS_REQUIRE(cond, code, ...)      \
   do {                                   \

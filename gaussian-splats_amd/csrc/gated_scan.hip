@@ -237,7 +237,7 @@ __device__ FloatVec<kChannels> look_back(const ScanArgs& a, int64_t b, int64_t p
     from += taken;
     if (taken == 0) {
       if (++spins > kSpinLimit) {
-        if ((threadIdx.x & 63) == 0) atomicOr(a.flags, kDeviceFlagSpinLimit);
+        if ((threadIdx.x & 63) == 0) atomicOr(a.flags, kDeviceFlagScan);
         return h;
       }
       __builtin_amdgcn_s_sleep(1);

@@ -366,22 +366,24 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_long_kernel(NormBwdArgs a) 
   }
 }
 
-// grad_w from the partial rows: a workgroup adds 64 columns, its four waves a
-// quarter of the rows each.
-__global__ __launch_bounds__(kThreads) void norm_weight_kernel(const float* __restrict__ partials,
-                                                               int count, int width, void* grad_w,
-                                                               int type) {
-  __shared__ float parts[kWaves][kWave];
+// grad_w from the partial rows: a workgroup adds 64 columns, its sixteen waves
+// every sixteenth row each.
+constexpr int kSumWaves = 16;
+__global__ __launch_bounds__(kSumWaves* kWave) void norm_weight_kernel(
+    const float* __restrict__ partials, int count, int width, void* grad_w, int type) {
+  __shared__ float parts[kSumWaves][kWave];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int c = blockIdx.x * kWave + lane;
   float sum = 0.0f;
-  if (c < width)
-    for (int i = wave; i < count; i += kWaves) sum += partials[int64_t(i) * width + c];
+  if (c < width) {
+#pragma unroll 8
+    for (int i = wave; i < count; i += kSumWaves) sum += partials[int64_t(i) * width + c];
+  }
   parts[wave][lane] = sum;
   __syncthreads();
   if (wave == 0 && c < width) {
 #pragma unroll
-    for (int i = 1; i < kWaves; ++i) sum += parts[i][lane];
+    for (int i = 1; i < kSumWaves; ++i) sum += parts[i][lane];
     store_from_float(grad_w, c, type, sum);
   }
 }
@@ -539,8 +541,8 @@ extern "C" GS_API int gs_add_rms_norm_bwd(const void* sum, const void* weight,
     }));
   }
   if (grad_weight) {
-    norm_weight_kernel<<<unsigned((width + kWave - 1) / kWave), kThreads, 0, as_stream(stream)>>>(
-        a.partials, blocks, a.width, grad_weight, weight_type);
+    norm_weight_kernel<<<unsigned((width + kWave - 1) / kWave), kSumWaves * kWave, 0,
+                         as_stream(stream)>>>(a.partials, blocks, a.width, grad_weight, weight_type);
     return check_launch("add_rms_norm weight gradient");
   }
   return GS_OK;

@@ -36,7 +36,7 @@ struct StepArgs {
 };
 
 template <typename T, int kDim>
-__global__ __launch_bounds__(kThreads) void attention_step_kernel(StepArgs a) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_step_kernel(StepArgs a) {
   constexpr int kPitchT = kPitch<T, kDim>;
   constexpr int kSteps = kDim / 16, kBlocks = kDim / 32;
   constexpr int kV = 16 / int(sizeof(T)), kPerRow = kDim / kV, kCount = kKeys * kPerRow / kWave;
@@ -230,7 +230,7 @@ int plan_splits(const gs_attention& d) {
   const int64_t capacity = d.sinks + d.window;
   const int64_t rows = d.batch * d.kv_heads * ((d.heads / d.kv_heads + 31) / 32);
   const int64_t most = (capacity + kWaves * kKeys - 1) / (kWaves * kKeys);
-  return int(std::max<int64_t>(1, std::min<int64_t>({most, 1024 / std::max<int64_t>(rows, 1), 256})));
+  return int(std::max<int64_t>(1, std::min<int64_t>({most, 1536 / std::max<int64_t>(rows, 1), 256})));
 }
 
 }  // namespace

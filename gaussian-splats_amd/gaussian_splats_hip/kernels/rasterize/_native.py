@@ -451,6 +451,7 @@ DEVICE_FLAGS = {
     1: "a look-back wait of a sort or binning pass hit its spin limit",
     2: "a binning workgroup's owner window exceeded its tile",
     4: "sizes passed to a binning pass differ from the plan's device totals",
+    8: "a wait of a gated scan hit its spin limit",
 }
 
 
@@ -459,8 +460,8 @@ def raise_device_flags(flags: int, where: str) -> None:
     if flags:
         what = "; ".join(text for bit, text in DEVICE_FLAGS.items() if flags & bit) or "unknown"
         raise RuntimeError(
-            f"{where}: a device-side check failed in a binning or sort call on this GPU "
-            f"(flags {flags:#x}: {what}); the intersection lists of that call are incomplete"
+            f"{where}: a device-side check failed in an earlier call on this GPU "
+            f"(flags {flags:#x}: {what}); the outputs of that call are incomplete"
         )
 
 

@@ -171,7 +171,6 @@ def window_attention(
     return _WindowAttention.apply(q, k, v, int(window), int(sinks), scale, lengths)
 
 
-@torch.no_grad()
 def window_attention_step(
     q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
     v_cache: torch.Tensor, positions: torch.Tensor, window: int, sinks: int = 0,

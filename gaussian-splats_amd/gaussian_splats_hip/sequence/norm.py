@@ -147,7 +147,6 @@ def add_rms_norm(
     return _AddRmsNorm.apply(x, residual, weight, eps)
 
 
-@torch.no_grad()
 def add_rms_norm_quant(
     x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float = 1e-6,
     format: str = "int8",

@@ -145,7 +145,6 @@ def gated_scan(
     return _GatedScan.apply(x, gate, state)
 
 
-@torch.no_grad()
 def gated_scan_step(
     x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, state_out: torch.Tensor | None = None
 ) -> tuple[torch.Tensor, torch.Tensor]:

@@ -135,6 +135,7 @@ GS_API int gs_disarm_launch_events(void);
 #define GS_DEVICE_SPIN_LIMIT 1u       /* a look-back wait hit its spin limit */
 #define GS_DEVICE_WINDOW_OVERFLOW 2u  /* a workgroup's owner window exceeded its tile */
 #define GS_DEVICE_SIZE_MISMATCH 4u    /* sizes passed by the host differ from the plan's */
+#define GS_DEVICE_SCAN_LIMIT 8u       /* a wait of a gated scan hit its spin limit */
 
 /* Reads the sticky word of the stream's GPU into *flags after the work
  * enqueued on `stream` so far has completed (this call synchronises the
