@@ -133,8 +133,8 @@ __device__ __forceinline__ float add_all(const Frag<float>& f, float sum) {
   return sum;
 }
 
-// A [kRows, kDim] tile on its way from global memory through a workgroup's
-// registers into LDS.  Rows outside [0, end) and columns from dim on are zeros.
+// A [kRows, kDim] tile on its way from global memory through the registers of
+// kThreads threads into LDS.  Rows outside [0, end) and columns from dim on are zeros.
 // A thread's places are the same in every tile, so a tile inside the tensor
 // takes no address arithmetic but the wave's.
 template <typename T, int kRows, int kDim, int kThreads>
@@ -150,8 +150,8 @@ struct Stage {
   uint32_t offset;  // of the thread's first chunk, in bytes
   int64_t stride;   // of a row, in bytes
 
-  __device__ __forceinline__ Stage(int64_t row_stride, int dim)
-      : row(threadIdx.x / kPerRow), col(threadIdx.x % kPerRow * kV), in(col < dim),
+  __device__ __forceinline__ Stage(int64_t row_stride, int dim, int thread)
+      : row(thread / kPerRow), col(thread % kPerRow * kV), in(col < dim),
         stride(row_stride * int64_t(sizeof(T))) {
     offset = uint32_t(row * stride) + uint32_t(col * sizeof(T));
 #pragma unroll
@@ -280,6 +280,39 @@ struct Problem {
     return lengths ? min(max(lengths[b], 0), keys) : keys;
   }
 };
+
+// The tiles of kKeys keys that queries from `query` on, `queries` of them, walk:
+// those that hold first tokens, then those of the window.
+template <int kKeys>
+struct KeyTiles {
+  int count, head, tail;
+  __device__ __forceinline__ KeyTiles(const Problem& p, int query, int queries, int length) {
+    const int first = p.offset() + query;
+    const int last = min(p.offset() + min(query + queries, p.queries), length) - 1;
+    tail = max(0, first - p.window + 1) / kKeys;
+    head = min((min(p.sinks, last + 1) + kKeys - 1) / kKeys, tail);
+    count = last < 0 ? 0 : head + max(0, last / kKeys - tail + 1);
+    tail -= head;
+  }
+  __device__ __forceinline__ int first_key(int it) const {
+    return (it < head ? it : tail + it) * kKeys;
+  }
+};
+
+// Fewer workgroups of 128 queries than this, and 32 queries a workgroup with the
+// keys shared out over its waves take over.  Forward, 128 a workgroup against 32,
+// us: heads of 64, 80 workgroups 19 and 15, 256 between 20 and 21 and 42 and 37,
+// 512 24 and 31; heads of 128, 64 workgroups 34 and 23, 128 between 27 and 29 and
+// 60 and 52, 256 43 and 82.
+inline int64_t split_below(int dim) { return dim <= 64 ? 256 : 160; }
+
+// What a wave's lanes wrote to LDS of their own is there for all of them: LDS
+// serves a wave in order, so only the compiler has to be held.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 
 // Which of the keys base + k a query at position p sees: comparisons of k,
 // known at compile time, with a few registers.

@@ -30,205 +30,252 @@ struct ForwardArgs {
 
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
-constexpr int kKeys = 64;  // of a tile
 
-// kTiles: tiles of 32 queries that a wave holds.
-template <typename T, int kDim, int kTiles>
-constexpr int kWavesPerSimd = sizeof(T) == 2 && sizeof(T) == 2 && kDim * kTiles <= 64 ? 4 : sizeof(T) == 2 && kDim * kTiles <= 128 ? 2 : 1;
+// 32 queries of a wave, a query for each pair of lanes: what their walk over the
+// keys carries.
+template <typename T, int kDim>
+struct Queries {
+  static constexpr int kSteps = kDim / 16, kBlocks = kDim / 32;
+  static constexpr int kPitchT = kPitch<T, kDim>;
+  Frag<T> q[kSteps];
+  float top = -INFINITY, sum = 0.0f;
+  Acc o[kBlocks];
+  Poison<T, kBlocks> poison;
+  int first, pos, length;  // position of the wave's first query and of the lane's
 
-template <typename T, int kDim, int kTiles>
-__global__ __launch_bounds__(kThreads, (kWavesPerSimd<T, kDim, kTiles>)) void attention_fwd_kernel(
-    ForwardArgs a) {
-  constexpr int kPitchT = kPitch<T, kDim>;
-  constexpr int kSteps = kDim / 16, kBlocks = kDim / 32;
-  constexpr int kQueries = 32 * kTiles * kWaves;  // of a workgroup
-  __shared__ __align__(16) T tiles[2][2][kKeys * kPitchT];
-  const Problem& p = a.p;
-  const int blocks = (p.queries + kQueries - 1) / kQueries;
-  const int64_t id = xcd_order(blockIdx.x, int64_t(blocks) * p.heads * p.batch);
-  if (id >= int64_t(blocks) * p.heads * p.batch) return;
-  // The heads that share keys side by side.
-  const int group = p.heads / p.kv_heads;
-  const int of = int(id % group);
-  const int block = int(id / group % blocks);
-  const int kv = int(id / group / blocks % p.kv_heads);
-  const int b = int(id / group / blocks / p.kv_heads);
-  const int head = kv * group + of;
-  const int length = p.length(b);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-
-  const int i0 = block * kQueries + wave * 32 * kTiles + (lane & 31);  // the lane's first query
-  const int pos = p.offset() + i0;
-  Frag<T> q[kTiles][kSteps];
-#pragma unroll
-  for (int t = 0; t < kTiles; ++t) {
-    const int i = i0 + 32 * t;
+  __device__ __forceinline__ Queries(const ForwardArgs& a, int b, int head, int query, int length_)
+      : first(a.p.offset() + query), length(length_) {
+    const int lane = threadIdx.x & 63, i = query + (lane & 31);
+    pos = a.p.offset() + i;
     const T* row = static_cast<const T*>(a.q) + b * a.sq.batch + i * a.sq.token + head * a.sq.head;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       const int d = 16 * s + 8 * (lane >> 5);
-      q[t][s] = load_global<T>(row + d, i < p.queries && d < p.dim);
+      q[s] = load_global<T>(row + d, i < a.p.queries && d < a.p.dim);
+    }
+#pragma unroll
+    for (int n = 0; n < kBlocks; ++n) o[n] = Acc(0.0f);
+  }
+
+  // 32 keys from j0 on, rows row0 .. of the LDS tiles kt and vt; c: the scale in
+  // powers of two.
+  __device__ __forceinline__ void take(const Problem& p, const T* kt, const T* vt, int row0, int j0,
+                                       float c) {
+    const int lane = threadIdx.x & 63, last = first + 31, j1 = j0 + 31;
+    const bool any = j0 <= last && j0 < length && (j1 > first - p.window || j0 < p.sinks);
+    const bool all = j1 <= first && j1 < length && (j0 > last - p.window || j1 < p.sinks);
+    if (__builtin_expect(!any, 0)) return;
+    Acc s(0.0f);
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st) mma(load_rows<T>(kt, kPitchT, row0, 16 * st), q[st], s);
+    if (__builtin_expect(!all, 0)) {
+      const KeySight sight(p, pos, j0 + 4 * (lane >> 5), length);
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (!sight.sees(acc_row_of_half(r))) s[r] = -INFINITY;
+    }
+    float m = s[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) m = fmaxf(m, s[r]);
+    m *= c;
+    // The maximum that exponents are taken against follows the true one at a
+    // distance of up to 2^8, so that most tiles rescale nothing, and need nothing
+    // of the scores that the lane's other half holds.
+    if (__builtin_expect(__any(m > top + 8.0f), 0)) {
+      const float whole = fmaxf(m, __shfl_xor(m, 32, 64));
+      const float up = whole > top + 8.0f ? whole : top;
+      float shrink = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - up);
+      asm volatile("" : "+v"(shrink));  // or the compiler rescales without the branch
+      sum *= shrink;
+#pragma unroll
+      for (int n = 0; n < kBlocks; ++n) o[n] *= shrink;
+      top = up;
+    }
+    const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      Frag<T> vf[kBlocks];
+#pragma unroll
+      for (int n = 0; n < kBlocks; ++n) vf[n] = load_turned<T>(vt, kPitchT, row0 + 16 * st, 32 * n);
+#pragma unroll
+      for (int r = 8 * st; r < 8 * st + 8; ++r) s[r] = power<T>(s[r] * c - base);
+      const Frag<T> pf = acc_frag<T>(s, st);
+      sum = add_all(pf, sum);
+      if (__builtin_expect(!all, 0)) {
+        const KeySight sight(p, pos, j0 + 16 * st, length);
+        poison.guard(vt, kPitchT, row0 + 16 * st, vf, pf, [&](int e) { return sight.sees(e); });
+      }
+#pragma unroll
+      for (int n = 0; n < kBlocks; ++n) mma(vf[n], pf, o[n]);
     }
   }
-  const T* kbase = static_cast<const T*>(a.k) + b * a.sk.batch + kv * a.sk.head;
-  const T* vbase = static_cast<const T*>(a.v) + b * a.sv.batch + kv * a.sv.head;
+};
 
-  // Tiles of the first tokens, then those of the window.
-  const int first = p.offset() + block * kQueries;
-  const int last = min(p.offset() + min((block + 1) * kQueries, p.queries), length) - 1;
-  int tail = max(0, first - p.window + 1) / kKeys;
-  const int head_tiles = min((min(p.sinks, last + 1) + kKeys - 1) / kKeys, tail);
-  const int count = last < 0 ? 0 : head_tiles + max(0, last / kKeys - tail + 1);
-  tail -= head_tiles;
-
-  const float c = p.scale * kLog2e;
-  const int wave_first = first + wave * 32 * kTiles, wave_last = wave_first + 32 * kTiles - 1;
-  float top[kTiles], sum[kTiles];
-  Acc o[kTiles][kBlocks];
-  Poison<T, kBlocks> poison[kTiles];
-#pragma unroll
-  for (int t = 0; t < kTiles; ++t) {
-    top[t] = -INFINITY;
-    sum[t] = 0.0f;
-#pragma unroll
-    for (int n = 0; n < kBlocks; ++n) o[t][n] = Acc(0.0f);
+// Which heads and queries a workgroup has: the heads that share keys side by side.
+struct Place {
+  int b, kv, head, block;
+  __device__ __forceinline__ Place(const Problem& p, int64_t id, int blocks) {
+    const int group = p.heads / p.kv_heads;
+    block = int(id / group % blocks);
+    kv = int(id / group / blocks % p.kv_heads);
+    b = int(id / group / blocks / p.kv_heads);
+    head = kv * group + int(id % group);
   }
+};
 
-  Stage<T, kKeys, kDim, kThreads> sk(a.sk.token, p.dim), sv(a.sv.token, p.dim);
+// 128 queries a workgroup, whose waves share tiles of 64 keys in LDS.
+template <typename T, int kDim>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : kDim <= 64 ? 4 : 2) void attention_fwd_kernel(
+    ForwardArgs a) {
+  constexpr int kKeys = 64, kQueries = 32 * kWaves;
+  constexpr int kBlocks = kDim / 32;
+  __shared__ __align__(16) T tiles[2][2][kKeys * kPitch<T, kDim>];
+  const Problem& p = a.p;
+  const int blocks = (p.queries + kQueries - 1) / kQueries;
+  const int64_t id = xcd_order(blockIdx.x, int64_t(blocks) * p.heads * p.batch);
+  if (id >= int64_t(blocks) * p.heads * p.batch) return;
+  const Place at(p, id, blocks);
+  const int length = p.length(at.b);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const T* kbase = static_cast<const T*>(a.k) + at.b * a.sk.batch + at.kv * a.sk.head;
+  const T* vbase = static_cast<const T*>(a.v) + at.b * a.sv.batch + at.kv * a.sv.head;
+  Queries<T, kDim> w(a, at.b, at.head, at.block * kQueries + wave * 32, length);
+  const KeyTiles<kKeys> walk(p, at.block * kQueries, kQueries, length);
+  const float c = p.scale * kLog2e;
+
+  Stage<T, kKeys, kDim, kThreads> sk(a.sk.token, p.dim, threadIdx.x), sv(a.sv.token, p.dim, threadIdx.x);
   const auto fetch = [&](int it) {
-    const int j0 = (it < head_tiles ? it : tail + it) * kKeys;
-    sk.load(kbase, j0, length);
-    sv.load(vbase, j0, length);
+    sk.load(kbase, walk.first_key(it), length);
+    sv.load(vbase, walk.first_key(it), length);
   };
-  if (count > 0) {
+  if (walk.count > 0) {
     fetch(0);
     sk.store(tiles[0][0]);
     sv.store(tiles[0][1]);
   }
   __syncthreads();
-  for (int it = 0; it < count; ++it) {
-    if (it + 1 < count) fetch(it + 1);
-    const T* kt = tiles[it & 1][0];
-    const T* vt = tiles[it & 1][1];
+  for (int it = 0; it < walk.count; ++it) {
+    if (it + 1 < walk.count) fetch(it + 1);
 #pragma unroll
-    for (int h = 0; h < kKeys / 32; ++h) {
-      const int j0 = (it < head_tiles ? it : tail + it) * kKeys + 32 * h, j1 = j0 + 31;
-      const bool any = j0 <= wave_last && j0 < length && (j1 > wave_first - p.window || j0 < p.sinks);
-      const bool all = j1 <= wave_first && j1 < length && (j0 > wave_last - p.window || j1 < p.sinks);
-      if (__builtin_expect(any, 1)) {
-        Acc s[kTiles];
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) s[t] = Acc(0.0f);
-#pragma unroll
-        for (int st = 0; st < kSteps; ++st) {
-          const Frag<T> kf = load_rows<T>(kt, kPitchT, 32 * h, 16 * st);
-#pragma unroll
-          for (int t = 0; t < kTiles; ++t) mma(kf, q[t][st], s[t]);
-        }
-        if (__builtin_expect(!all, 0)) {
-#pragma unroll
-          for (int t = 0; t < kTiles; ++t) {
-            const KeySight sight(p, pos + 32 * t, j0 + 4 * (lane >> 5), length);
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              if (!sight.sees(acc_row_of_half(r))) s[t][r] = -INFINITY;
-          }
-        }
-        float m[kTiles];
-        bool grows = false;
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-          m[t] = s[t][0];
-#pragma unroll
-          for (int r = 1; r < 16; ++r) m[t] = fmaxf(m[t], s[t][r]);
-          m[t] *= c;
-          grows |= m[t] > top[t] + 8.0f;
-        }
-        // The maximum that exponents are taken against follows the true one at a
-        // distance of up to 2^8, so that most tiles rescale nothing, and need
-        // nothing of the half of the scores that the lane's other half holds.
-        if (__builtin_expect(__any(grows), 0)) {
-#pragma unroll
-          for (int t = 0; t < kTiles; ++t) {
-            const float whole = fmaxf(m[t], __shfl_xor(m[t], 32, 64));
-            const float up = whole > top[t] + 8.0f ? whole : top[t];
-            float shrink = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[t] - up);
-            asm volatile("" : "+v"(shrink));  // or the compiler rescales without the branch
-            sum[t] *= shrink;
-#pragma unroll
-            for (int n = 0; n < kBlocks; ++n) o[t][n] *= shrink;
-            top[t] = up;
-          }
-        }
-#pragma unroll
-        for (int st = 0; st < 2; ++st) {
-          Frag<T> pf[kTiles], vf[kBlocks];
-#pragma unroll
-          for (int n = 0; n < kBlocks; ++n)
-            vf[n] = load_turned<T>(vt, kPitchT, 32 * h + 16 * st, 32 * n);
-#pragma unroll
-          for (int t = 0; t < kTiles; ++t) {
-            const float base = top[t] == -INFINITY ? 0.0f : top[t];
-#pragma unroll
-            for (int r = 8 * st; r < 8 * st + 8; ++r) s[t][r] = power<T>(s[t][r] * c - base);
-            pf[t] = acc_frag<T>(s[t], st);
-            sum[t] = add_all(pf[t], sum[t]);
-          }
-          if (__builtin_expect(!all, 0)) {
-            if (__builtin_expect(any_not_finite<T>(vf), 0)) {
-#pragma unroll
-              for (int t = 0; t < kTiles; ++t) {
-                const KeySight sight(p, pos + 32 * t, j0 + 16 * st, length);
-                poison[t].mark(vt, kPitchT, 32 * h + 16 * st, pf[t],
-                               [&](int e) { return sight.sees(e); });
-              }
-              drop_not_finite<T>(vf);
-            }
-          }
-#pragma unroll
-          for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-            for (int n = 0; n < kBlocks; ++n) mma(vf[n], pf[t], o[t][n]);
-        }
-      }
-    }
-    if (it + 1 < count) {
+    for (int h = 0; h < kKeys / 32; ++h)
+      w.take(p, tiles[it & 1][0], tiles[it & 1][1], 32 * h, walk.first_key(it) + 32 * h, c);
+    if (it + 1 < walk.count) {
       sk.store(tiles[(it + 1) & 1][0]);
       sv.store(tiles[(it + 1) & 1][1]);
     }
     __syncthreads();
   }
+  w.poison.apply(w.o);
+  const int i = at.block * kQueries + wave * 32 + (lane & 31);
+  const float l = w.sum + __shfl_xor(w.sum, 32, 64);
+  if (i >= p.queries) return;
+  const float inverse = w.top == -INFINITY && l == 0.0f ? 0.0f : 1.0f / l;
+  T* out = static_cast<T*>(a.out) + ((int64_t(at.b) * p.queries + i) * p.heads + at.head) * p.dim;
 #pragma unroll
-  for (int t = 0; t < kTiles; ++t) {
-    const int i = i0 + 32 * t;
-    poison[t].apply(o[t]);
-    const float l = sum[t] + __shfl_xor(sum[t], 32, 64);
-    if (i >= p.queries) continue;
-    const float inverse = top[t] == -INFINITY && l == 0.0f ? 0.0f : 1.0f / l;
-    T* out = static_cast<T*>(a.out) + ((int64_t(b) * p.queries + i) * p.heads + head) * p.dim;
+  for (int n = 0; n < kBlocks; ++n)
 #pragma unroll
-    for (int n = 0; n < kBlocks; ++n)
+    for (int g = 0; g < 4; ++g) {
+      const int d = 32 * n + 8 * g + 4 * (lane >> 5);
+      FloatVec<4> f;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int d = 32 * n + 8 * g + 4 * (lane >> 5);
-        FloatVec<4> f;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) f[r] = o[t][n][4 * g + r] * inverse;
-        if (d < p.dim) *reinterpret_cast<Vec<T, 4>*>(out + d) = from_float<T, 4>(f);
-      }
-    if (lane < 32)
-      a.lse[(int64_t(b) * p.heads + head) * p.queries + i] =
-          top[t] == -INFINITY ? -INFINITY : (top[t] + __builtin_amdgcn_logf(l)) / kLog2e;
-  }
+      for (int r = 0; r < 4; ++r) f[r] = w.o[n][4 * g + r] * inverse;
+      if (d < p.dim) *reinterpret_cast<Vec<T, 4>*>(out + d) = from_float<T, 4>(f);
+    }
+  if (lane < 32)
+    a.lse[(int64_t(at.b) * p.heads + at.head) * p.queries + i] =
+        w.top == -INFINITY ? -INFINITY : (w.top + __builtin_amdgcn_logf(l)) / kLog2e;
 }
 
-template <typename T, int kDim, int kTiles>
+// 32 queries a workgroup: every wave has all of them and every fourth tile of 32
+// keys, which it loads by itself, and the waves join at the end.  For calls that
+// would leave most of the GPU idle with 128 queries a workgroup.
+template <typename T, int kDim>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fwd_split_kernel(
+    ForwardArgs a) {
+  constexpr int kKeys = 32, kQueries = 32;
+  constexpr int kBlocks = kDim / 32;
+  __shared__ __align__(16) T tiles[kWaves][2][kKeys * kPitch<T, kDim>];
+  __shared__ float joined[32][kDim + 1];
+  __shared__ float tops[kWaves][32], sums[kWaves][32];
+  const Problem& p = a.p;
+  const int blocks = (p.queries + kQueries - 1) / kQueries;
+  const int64_t id = xcd_order(blockIdx.x, int64_t(blocks) * p.heads * p.batch);
+  if (id >= int64_t(blocks) * p.heads * p.batch) return;
+  const Place at(p, id, blocks);
+  const int length = p.length(at.b);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const T* kbase = static_cast<const T*>(a.k) + at.b * a.sk.batch + at.kv * a.sk.head;
+  const T* vbase = static_cast<const T*>(a.v) + at.b * a.sv.batch + at.kv * a.sv.head;
+  Queries<T, kDim> w(a, at.b, at.head, at.block * kQueries, length);
+  const KeyTiles<kKeys> walk(p, at.block * kQueries, kQueries, length);
+  const float c = p.scale * kLog2e;
+  Stage<T, kKeys, kDim, kWave> sk(a.sk.token, p.dim, lane), sv(a.sv.token, p.dim, lane);
+  const auto fetch = [&](int it) {
+    sk.load(kbase, walk.first_key(it), length);
+    sv.load(vbase, walk.first_key(it), length);
+  };
+  if (wave < walk.count) fetch(wave);
+  for (int it = wave; it < walk.count; it += kWaves) {
+    sk.store(tiles[wave][0]);
+    sv.store(tiles[wave][1]);
+    if (it + kWaves < walk.count) fetch(it + kWaves);
+    wave_sync();
+    w.take(p, tiles[wave][0], tiles[wave][1], 0, walk.first_key(it), c);
+    wave_sync();
+  }
+  w.poison.apply(w.o);
+  // The waves join: the largest maximum, then the sums one wave after the other.
+  const float l = w.sum + __shfl_xor(w.sum, 32, 64);
+  if (lane < 32) {
+    tops[wave][lane] = w.top;
+    sums[wave][lane] = l;
+  }
+  __syncthreads();
+  const int col = lane & 31;
+  float top = tops[0][col], whole = 0.0f;
+#pragma unroll
+  for (int k = 1; k < kWaves; ++k) top = fmaxf(top, tops[k][col]);
+  const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+  for (int k = 0; k < kWaves; ++k)
+    whole += sums[k][col] * __builtin_amdgcn_exp2f(tops[k][col] - base);
+  const float inverse = top == -INFINITY && whole == 0.0f ? 0.0f : 1.0f / whole;
+  const float shrink = __builtin_amdgcn_exp2f(w.top - base) * inverse;
+  for (int k = 0; k < kWaves; ++k) {
+    if (wave == k) {
+#pragma unroll
+      for (int n = 0; n < kBlocks; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          float& sum = joined[col][32 * n + acc_row(r)];
+          const float v = w.top == -INFINITY ? 0.0f : w.o[n][r] * shrink;
+          sum = k ? sum + v : v;
+        }
+    }
+    __syncthreads();
+  }
+  const int i0 = at.block * kQueries;
+  T* out = static_cast<T*>(a.out) + ((int64_t(at.b) * p.queries + i0) * p.heads + at.head) * p.dim;
+  for (int e = threadIdx.x; e < 32 * kDim; e += kThreads) {
+    const int row = e / kDim, d = e % kDim;
+    if (i0 + row < p.queries && d < p.dim)
+      out[int64_t(row) * p.heads * p.dim + d] = T(joined[row][d]);
+  }
+  if (threadIdx.x < 32 && i0 + col < p.queries)
+    a.lse[(int64_t(at.b) * p.heads + at.head) * p.queries + i0 + col] =
+        top == -INFINITY ? -INFINITY : (top + __builtin_amdgcn_logf(whole)) / kLog2e;
+}
+
+template <typename T, int kDim>
 int launch_forward(const ForwardArgs& a, hipStream_t s) {
-  constexpr int kQueries = 32 * kTiles * kWaves;
-  const int64_t items =
-      (int64_t(a.p.queries) + kQueries - 1) / kQueries * a.p.heads * a.p.batch;
-  GS_REQUIRE(items < (int64_t(1) << 30), GS_ERR_OVERFLOW, "attention problem too large");
-  attention_fwd_kernel<T, kDim, kTiles><<<unsigned(xcd_grid(items)), kThreads, 0, s>>>(a);
+  const auto items = [&](int queries) {
+    return (int64_t(a.p.queries) + queries - 1) / queries * a.p.heads * a.p.batch;
+  };
+  GS_REQUIRE(items(32) < (int64_t(1) << 30), GS_ERR_OVERFLOW, "attention problem too large");
+  if (items(32 * kWaves) < split_below(a.p.dim))
+    attention_fwd_split_kernel<T, kDim><<<unsigned(xcd_grid(items(32))), kThreads, 0, s>>>(a);
+  else
+    attention_fwd_kernel<T, kDim><<<unsigned(xcd_grid(items(32 * kWaves))), kThreads, 0, s>>>(a);
   return check_launch("window_attention");
 }
 
@@ -305,7 +352,7 @@ extern "C" GS_API int gs_window_attention_fwd(const gs_attention* desc, const vo
                 out, lse};
   return seq::with_type(desc->type, [&](auto t) {
     using T = decltype(t);
-    if (desc->head_dim <= 64) return launch_forward<T, 64, 1>(a, as_stream(stream));
-    return launch_forward<T, 128, 1>(a, as_stream(stream));
+    if (desc->head_dim <= 64) return launch_forward<T, 64>(a, as_stream(stream));
+    return launch_forward<T, 128>(a, as_stream(stream));
   });
 }

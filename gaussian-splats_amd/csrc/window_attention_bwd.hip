@@ -181,7 +181,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
   for (int n = 0; n < kBlocks; ++n) dk[n] = dv[n] = Acc(0.0f);
   const float c = p.scale * kLog2e;
 
-  Stage<T, kRows, kDim, kThreads> sq(a.sq.token, p.dim), sg(a.sg.token, p.dim);
+  Stage<T, kRows, kDim, kThreads> sq(a.sq.token, p.dim, threadIdx.x),
+      sg(a.sg.token, p.dim, threadIdx.x);
   float row_lse = 0.0f, row_delta = 0.0f;
   const auto fetch = [&](int it) {
     const int head = kv * group + it / tiles_per_head;
@@ -321,6 +322,7 @@ __global__ __launch_bounds__(256) void attention_bwd_join_kernel(BackwardArgs a,
   const float* part = a.parts + part_index(a, b, kv, block, 0) * 2 * plane + in;
   const int pieces = block < a.sink_blocks ? a.sink_segments : a.segments;
   FloatVec<4> dk(0.0f), dv(0.0f);
+#pragma unroll 4
   for (int s = 0; s < pieces; ++s) {
     dk += *reinterpret_cast<const FloatVec<4>*>(part + 2 * s * plane);
     dv += *reinterpret_cast<const FloatVec<4>*>(part + (2 * s + 1) * plane);
@@ -330,31 +332,25 @@ __global__ __launch_bounds__(256) void attention_bwd_join_kernel(BackwardArgs a,
   *reinterpret_cast<Vec<T, 4>*>(static_cast<T*>(a.dv) + row) = from_float<T, 4>(dv);
 }
 
-// grad_q of a workgroup's queries: a wave holds 32, the keys that they see walk by.
+// grad_q of a wave's 32 queries: what their walk over the keys carries.
 template <typename T, int kDim>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) void attention_bwd_queries_kernel(BackwardArgs a) {
-  constexpr int kRows = kTileRows<T, kDim>;
-  constexpr int kPitchT = kPitch<T, kDim>;
-  constexpr int kSteps = kDim / 16, kBlocks = kDim / 32;
-  __shared__ __align__(16) T tiles[2][2][kRows * kPitchT];
-  const Problem& p = a.p;
-  const int blocks = (p.queries + kBlockQueries - 1) / kBlockQueries;
-  const int64_t total = int64_t(blocks) * p.heads * p.batch;
-  const int64_t id = xcd_order(blockIdx.x, total);
-  if (id >= total) return;
-  const int group = p.heads / p.kv_heads;
-  const int of = int(id % group);
-  const int block = int(id / group % blocks);
-  const int kv = int(id / group / blocks % p.kv_heads);
-  const int b = int(id / group / blocks / p.kv_heads);
-  const int head = kv * group + of;
-  const int length = p.length(b);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int i = block * kBlockQueries + wave * 32 + (lane & 31);
-  const int pos = p.offset() + i;
-  const bool live = i < p.queries;
+struct GradQueries {
+  static constexpr int kSteps = kDim / 16, kBlocks = kDim / 32;
+  static constexpr int kPitchT = kPitch<T, kDim>;
   Frag<T> q[kSteps], g[kSteps];
-  {
+  float lse, delta;  // lse in powers of two; P carries dS's power of two
+  float factor;      // of the result
+  Acc dq[kBlocks];
+  Poison<T, kBlocks> poison;
+  int first, pos, length;  // position of the wave's first query and of the lane's
+
+  __device__ __forceinline__ GradQueries(const BackwardArgs& a, int b, int head, int query,
+                                         int length_)
+      : first(a.p.offset() + query), length(length_) {
+    const Problem& p = a.p;
+    const int lane = threadIdx.x & 63, i = query + (lane & 31);
+    pos = p.offset() + i;
+    const bool live = i < p.queries;
     const T* qr = static_cast<const T*>(a.q) + b * a.sq.batch + i * a.sq.token + head * a.sq.head;
     const T* gr = static_cast<const T*>(a.grad) + b * a.sg.batch + i * a.sg.token + head * a.sg.head;
 #pragma unroll
@@ -363,90 +359,107 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
       q[s] = load_global<T>(qr + d, live && d < p.dim);
       g[s] = load_global<T>(gr + d, live && d < p.dim);
     }
-  }
-  const int64_t at = (int64_t(b) * p.heads + head) * p.queries + i;
-  const int shift = gradient_shift<T>(a);
-  const float down = ldexpf(1.0f, -shift);
-  // P carries dS's power of two.
-  const float lse = live ? a.lse[at] * kLog2e - float(shift) : 0.0f;
-  const float delta = live ? a.delta[at] : 0.0f;
-
-  const int first = p.offset() + block * kBlockQueries;
-  const int last = min(p.offset() + min((block + 1) * kBlockQueries, p.queries), length) - 1;
-  int tail = max(0, first - p.window + 1) / kRows;
-  const int head_tiles = min((min(p.sinks, last + 1) + kRows - 1) / kRows, tail);
-  const int count = last < 0 ? 0 : head_tiles + max(0, last / kRows - tail + 1);
-  tail -= head_tiles;
-  const int wave_first = first + wave * 32, wave_last = wave_first + 31;
-  const float c = p.scale * kLog2e;
-  Acc dq[kBlocks];
+    const int64_t at = (int64_t(b) * p.heads + head) * p.queries + i;
+    const int shift = gradient_shift<T>(a);
+    lse = live ? a.lse[at] * kLog2e - float(shift) : 0.0f;
+    delta = live ? a.delta[at] : 0.0f;
+    factor = ldexpf(p.scale, -shift);
 #pragma unroll
-  for (int n = 0; n < kBlocks; ++n) dq[n] = Acc(0.0f);
+    for (int n = 0; n < kBlocks; ++n) dq[n] = Acc(0.0f);
+  }
 
-  const T* kbase = static_cast<const T*>(a.k) + b * a.sk.batch + kv * a.sk.head;
-  const T* vbase = static_cast<const T*>(a.v) + b * a.sv.batch + kv * a.sv.head;
-  Poison<T, kBlocks> poison;
-  Stage<T, kRows, kDim, kThreads> sk(a.sk.token, p.dim), sv(a.sv.token, p.dim);
+  // 32 keys from j0 on, rows row0 .. of the LDS tiles kt and vt.
+  __device__ __forceinline__ void take(const Problem& p, const T* kt, const T* vt, int row0, int j0,
+                                       float c) {
+    const int lane = threadIdx.x & 63, last = first + 31, j1 = j0 + 31;
+    const bool any = j0 <= last && j0 < length && (j1 > first - p.window || j0 < p.sinks);
+    const bool all = j1 <= first && j1 < length && (j0 > last - p.window || j1 < p.sinks);
+    if (__builtin_expect(!any, 0)) return;
+    Acc s(0.0f), dp(0.0f);
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st) mma(load_rows<T>(kt, kPitchT, row0, 16 * st), q[st], s);
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st) mma(load_rows<T>(vt, kPitchT, row0, 16 * st), g[st], dp);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dp[r] = power<T>(s[r] * c - lse) * (dp[r] - delta);
+    if (__builtin_expect(!all, 0)) {
+      const KeySight sight(p, pos, j0 + 4 * (lane >> 5), length);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dp[r] = sight.sees(acc_row_of_half(r)) ? dp[r] : 0.0f;
+    }
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      const Frag<T> df = acc_frag<T>(dp, st);
+      Frag<T> f[kBlocks];
+#pragma unroll
+      for (int n = 0; n < kBlocks; ++n) f[n] = load_turned<T>(kt, kPitchT, row0 + 16 * st, 32 * n);
+      if (__builtin_expect(!all, 0)) {
+        const KeySight sight(p, pos, j0 + 16 * st, length);
+        poison.guard(kt, kPitchT, row0 + 16 * st, f, df, [&](int e) { return sight.sees(e); });
+      }
+#pragma unroll
+      for (int n = 0; n < kBlocks; ++n) mma(f[n], df, dq[n]);
+    }
+  }
+};
+
+// The heads that share keys side by side.
+struct QueryPlace {
+  int b, kv, head, block;
+  __device__ __forceinline__ QueryPlace(const Problem& p, int64_t id, int blocks) {
+    const int group = p.heads / p.kv_heads;
+    block = int(id / group % blocks);
+    kv = int(id / group / blocks % p.kv_heads);
+    b = int(id / group / blocks / p.kv_heads);
+    head = kv * group + int(id % group);
+  }
+};
+
+// 128 queries a workgroup, whose waves share tiles of keys in LDS.
+template <typename T, int kDim>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) void
+attention_bwd_queries_kernel(BackwardArgs a) {
+  constexpr int kRows = kTileRows<T, kDim>, kBlocks = kDim / 32;
+  __shared__ __align__(16) T tiles[2][2][kRows * kPitch<T, kDim>];
+  const Problem& p = a.p;
+  const int blocks = (p.queries + kBlockQueries - 1) / kBlockQueries;
+  const int64_t id = xcd_order(blockIdx.x, int64_t(blocks) * p.heads * p.batch);
+  if (id >= int64_t(blocks) * p.heads * p.batch) return;
+  const QueryPlace at(p, id, blocks);
+  const int length = p.length(at.b);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int query = at.block * kBlockQueries + wave * 32;
+  GradQueries<T, kDim> w(a, at.b, at.head, query, length);
+  const KeyTiles<kRows> walk(p, at.block * kBlockQueries, kBlockQueries, length);
+  const float c = p.scale * kLog2e;
+  const T* kbase = static_cast<const T*>(a.k) + at.b * a.sk.batch + at.kv * a.sk.head;
+  const T* vbase = static_cast<const T*>(a.v) + at.b * a.sv.batch + at.kv * a.sv.head;
+  Stage<T, kRows, kDim, kThreads> sk(a.sk.token, p.dim, threadIdx.x), sv(a.sv.token, p.dim, threadIdx.x);
   const auto fetch = [&](int it) {
-    const int j0 = (it < head_tiles ? it : tail + it) * kRows;
-    sk.load(kbase, j0, length);
-    sv.load(vbase, j0, length);
+    sk.load(kbase, walk.first_key(it), length);
+    sv.load(vbase, walk.first_key(it), length);
   };
-  if (count > 0) {
+  if (walk.count > 0) {
     fetch(0);
     sk.store(tiles[0][0]);
     sv.store(tiles[0][1]);
   }
   __syncthreads();
-  for (int it = 0; it < count; ++it) {
-    if (it + 1 < count) fetch(it + 1);
-    const T* kt = tiles[it & 1][0];
-    const T* vt = tiles[it & 1][1];
+  for (int it = 0; it < walk.count; ++it) {
+    if (it + 1 < walk.count) fetch(it + 1);
 #pragma unroll 1
-    for (int h = 0; h < kRows / 32; ++h) {
-      const int j0 = (it < head_tiles ? it : tail + it) * kRows + 32 * h, j1 = j0 + 31;
-      const bool any = j0 <= wave_last && j0 < length && (j1 > wave_first - p.window || j0 < p.sinks);
-      const bool all = j1 <= wave_first && j1 < length && (j0 > wave_last - p.window || j1 < p.sinks);
-      if (__builtin_expect(any, 1)) {
-        Acc s(0.0f), dp(0.0f);
-#pragma unroll
-        for (int st = 0; st < kSteps; ++st)
-          mma(load_rows<T>(kt, kPitchT, 32 * h, 16 * st), q[st], s);
-#pragma unroll
-        for (int st = 0; st < kSteps; ++st)
-          mma(load_rows<T>(vt, kPitchT, 32 * h, 16 * st), g[st], dp);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) dp[r] = power<T>(s[r] * c - lse) * (dp[r] - delta);
-        if (__builtin_expect(!all, 0)) {
-          const KeySight sight(p, pos, j0 + 4 * (lane >> 5), length);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) dp[r] = sight.sees(acc_row_of_half(r)) ? dp[r] : 0.0f;
-        }
-#pragma unroll
-        for (int st = 0; st < 2; ++st) {
-          const Frag<T> df = acc_frag<T>(dp, st);
-          Frag<T> f[kBlocks];
-#pragma unroll
-          for (int n = 0; n < kBlocks; ++n)
-            f[n] = load_turned<T>(kt, kPitchT, 32 * h + 16 * st, 32 * n);
-          if (__builtin_expect(!all, 0)) {
-            const KeySight sight(p, pos, j0 + 16 * st, length);
-            poison.guard(kt, kPitchT, 32 * h + 16 * st, f, df, [&](int e) { return sight.sees(e); });
-          }
-#pragma unroll
-          for (int n = 0; n < kBlocks; ++n) mma(f[n], df, dq[n]);
-        }
-      }
-    }
-    if (it + 1 < count) {
+    for (int h = 0; h < kRows / 32; ++h)
+      w.take(p, tiles[it & 1][0], tiles[it & 1][1], 32 * h, walk.first_key(it) + 32 * h, c);
+    if (it + 1 < walk.count) {
       sk.store(tiles[(it + 1) & 1][0]);
       sv.store(tiles[(it + 1) & 1][1]);
     }
     __syncthreads();
   }
-  poison.apply(dq);
-  if (!live) return;
-  T* out = static_cast<T*>(a.dq) + ((int64_t(b) * p.queries + i) * p.heads + head) * p.dim;
+  w.poison.apply(w.dq);
+  const int i = query + (lane & 31);
+  if (i >= p.queries) return;
+  T* out = static_cast<T*>(a.dq) + ((int64_t(at.b) * p.queries + i) * p.heads + at.head) * p.dim;
 #pragma unroll
   for (int n = 0; n < kBlocks; ++n)
 #pragma unroll
@@ -454,16 +467,85 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
       const int d = 32 * n + 8 * e + 4 * (lane >> 5);
       FloatVec<4> x;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) x[r] = dq[n][4 * e + r] * (p.scale * down);
+      for (int r = 0; r < 4; ++r) x[r] = w.dq[n][4 * e + r] * w.factor;
       if (d < p.dim) *reinterpret_cast<Vec<T, 4>*>(out + d) = from_float<T, 4>(x);
     }
 }
 
+// 32 queries a workgroup: every wave has all of them and every fourth tile of 32
+// keys, which it loads by itself; the waves' sums are added one after the other.
+template <typename T, int kDim>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void
+attention_bwd_queries_split_kernel(BackwardArgs a) {
+  constexpr int kKeys = 32, kQueries = 32, kBlocks = kDim / 32;
+  __shared__ __align__(16) T tiles[kWaves][2][kKeys * kPitch<T, kDim>];
+  __shared__ float joined[32][kDim + 1];
+  const Problem& p = a.p;
+  const int blocks = (p.queries + kQueries - 1) / kQueries;
+  const int64_t id = xcd_order(blockIdx.x, int64_t(blocks) * p.heads * p.batch);
+  if (id >= int64_t(blocks) * p.heads * p.batch) return;
+  const QueryPlace at(p, id, blocks);
+  const int length = p.length(at.b);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  GradQueries<T, kDim> w(a, at.b, at.head, at.block * kQueries, length);
+  const KeyTiles<kKeys> walk(p, at.block * kQueries, kQueries, length);
+  const float c = p.scale * kLog2e;
+  const T* kbase = static_cast<const T*>(a.k) + at.b * a.sk.batch + at.kv * a.sk.head;
+  const T* vbase = static_cast<const T*>(a.v) + at.b * a.sv.batch + at.kv * a.sv.head;
+  Stage<T, kKeys, kDim, kWave> sk(a.sk.token, p.dim, lane), sv(a.sv.token, p.dim, lane);
+  const auto fetch = [&](int it) {
+    sk.load(kbase, walk.first_key(it), length);
+    sv.load(vbase, walk.first_key(it), length);
+  };
+  if (wave < walk.count) fetch(wave);
+  for (int it = wave; it < walk.count; it += kWaves) {
+    sk.store(tiles[wave][0]);
+    sv.store(tiles[wave][1]);
+    if (it + kWaves < walk.count) fetch(it + kWaves);
+    wave_sync();
+    w.take(p, tiles[wave][0], tiles[wave][1], 0, walk.first_key(it), c);
+    wave_sync();
+  }
+  w.poison.apply(w.dq);
+  for (int k = 0; k < kWaves; ++k) {
+    if (wave == k) {
+#pragma unroll
+      for (int n = 0; n < kBlocks; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          float& sum = joined[lane & 31][32 * n + acc_row(r)];
+          sum = k ? sum + w.dq[n][r] : w.dq[n][r];
+        }
+    }
+    __syncthreads();
+  }
+  const int i0 = at.block * kQueries;
+  T* out = static_cast<T*>(a.dq) + ((int64_t(at.b) * p.queries + i0) * p.heads + at.head) * p.dim;
+  for (int e = threadIdx.x; e < 32 * kDim; e += kThreads) {
+    const int row = e / kDim, d = e % kDim;
+    if (i0 + row < p.queries && d < p.dim)
+      out[int64_t(row) * p.heads * p.dim + d] = T(joined[row][d] * w.factor);
+  }
+}
+
+template <typename T, int kDim>
+void launch_queries(const BackwardArgs& a, hipStream_t s) {
+  const auto items = [&](int queries) {
+    return (int64_t(a.p.queries) + queries - 1) / queries * a.p.heads * a.p.batch;
+  };
+  if (items(kBlockQueries) < split_below(a.p.dim))
+    attention_bwd_queries_split_kernel<T, kDim>
+        <<<unsigned(xcd_grid(items(32))), kThreads, 0, s>>>(a);
+  else
+    attention_bwd_queries_kernel<T, kDim>
+        <<<unsigned(xcd_grid(items(kBlockQueries))), kThreads, 0, s>>>(a);
+}
+
 // How the walks are cut.  Where the blocks of keys are fewer than two for each
-// CU, into segments of at least two tiles that make up for it.  The first tokens'
-// walks into segments a quarter as long: most of their tiles are masked, and with
-// segments of the others' length they end last (40000 tokens: 2.41 ms, 1.81 with
-// a quarter).
+// CU, into segments of at least two tiles that make up for it, and the first
+// tokens' walks into as long ones.  Else the first tokens' alone, into segments a
+// quarter as long as the others' walks: most of their tiles are masked, and at the
+// others' length they end last (40000 tokens: 2.41 ms, 1.81 with a quarter).
 void plan_segments(const Problem& p, int32_t type, BackwardArgs& a) {
   const int64_t blocks = key_blocks(p), rows = type == GS_F32 ? 32 : 64;
   const int64_t group = p.heads / p.kv_heads;
@@ -473,8 +555,8 @@ void plan_segments(const Problem& p, int32_t type, BackwardArgs& a) {
   a.segments = int(std::max<int64_t>(1, std::min<int64_t>(512 / items, walk / 2)));
   a.sink_blocks = int(std::min<int64_t>(blocks, (p.sinks + kBlockKeys - 1) / kBlockKeys));
   const int64_t long_walk = (int64_t(p.queries) + rows - 1) / rows * group;
-  const int64_t piece = std::max<int64_t>(1, walk / a.segments);
-  a.sink_segments = int(std::max<int64_t>(1, std::min<int64_t>(4 * long_walk / piece, 4096)));
+  const int64_t piece = a.segments > 1 ? walk / a.segments : std::max<int64_t>(1, walk / 4);
+  a.sink_segments = int(std::max<int64_t>(1, std::min<int64_t>(long_walk / piece, 4096)));
 }
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
@@ -554,14 +636,12 @@ extern "C" GS_API int gs_window_attention_bwd(const gs_attention* desc, const vo
   const int64_t blocks = key_blocks(p), others = blocks - a.sink_blocks;
   const int64_t key_items = (int64_t(a.sink_blocks) * a.sink_segments + others * a.segments) *
                             p.kv_heads * p.batch;
-  const int64_t query_items =
-      int64_t(p.queries + kBlockQueries - 1) / kBlockQueries * p.heads * p.batch;
   // Blocks that leave parts: all, the first tokens' or the others.
   const int join_first = a.sink_segments > 1 ? 0 : a.sink_blocks;
   const int join_blocks = int((a.sink_segments > 1 ? a.sink_blocks : 0) + (a.segments > 1 ? others : 0));
   const int64_t joined = int64_t(p.batch) * p.kv_heads * join_blocks * kBlockKeys * p.dim / 4;
   GS_REQUIRE(rows / 16 < (int64_t(1) << 30) && key_items < (int64_t(1) << 30) &&
-                 query_items < (int64_t(1) << 30) && joined / 256 < (int64_t(1) << 30),
+                 joined / 256 < (int64_t(1) << 30),
              GS_ERR_OVERFLOW, "attention problem too large");
   const hipStream_t s = as_stream(stream);
   return seq::with_type(desc->type, [&](auto t) {
@@ -584,12 +664,11 @@ extern "C" GS_API int gs_window_attention_bwd(const gs_attention* desc, const vo
                                                                                   join_blocks);
       GS_TRY(check_launch("window_attention backward, first tokens"));
     }
-    if (query_items) {
-      const unsigned grid = unsigned(xcd_grid(query_items));
+    if (rows) {
       if (p.dim <= 64)
-        attention_bwd_queries_kernel<T, 64><<<grid, kThreads, 0, s>>>(a);
+        launch_queries<T, 64>(a, s);
       else
-        attention_bwd_queries_kernel<T, 128><<<grid, kThreads, 0, s>>>(a);
+        launch_queries<T, 128>(a, s);
     }
     return check_launch("window_attention backward, queries");
   });

@@ -107,15 +107,12 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_st
     Acc s(0.0f);
 #pragma unroll
     for (int st = 0; st < kSteps; ++st) mma(kf[st], q[st], s);
-    // The tile is the wave's own, and LDS serves a wave in order.
 #pragma unroll
     for (int i = 0; i < kCount; ++i) {
       const int chunk = i * kWave + lane;
       *reinterpret_cast<Vec<T, kV>*>(tile + chunk / kPerRow * kPitchT + chunk % kPerRow * kV) = vr[i];
     }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    wave_sync();
     if (j0 + kWaves * kKeys < hi) fetch(j0 + kWaves * kKeys);
     if (j0 + kKeys > hi) {
 #pragma unroll
@@ -146,9 +143,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_st
 #pragma unroll
       for (int n = 0; n < kBlocks; ++n) mma(load_turned<T>(tile, kPitchT, 16 * st, 32 * n), pf, o[n]);
     }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    wave_sync();
   }
   // The waves join: the largest maximum, then the sums one wave after the other.
   sum += __shfl_xor(sum, 32, 64);
