@@ -57,26 +57,45 @@ struct Queries {
     for (int n = 0; n < kBlocks; ++n) o[n] = Acc(0.0f);
   }
 
-  // 32 keys from j0 on, rows row0 .. of the LDS tiles kt and vt; c: the scale in
-  // powers of two.
+  // Whether every query sees each of `keys` keys from j0 on.
+  __device__ __forceinline__ bool sees_all(const Problem& p, int j0, int keys) const {
+    const int last = first + 31, j1 = j0 + keys - 1;
+    return j1 <= first && j1 < length && (j0 > last - p.window || j1 < p.sinks);
+  }
+
+  // 32 kHalves keys from j0 on, rows row0 .. of the LDS tiles kt and vt; c: the
+  // scale in powers of two.  kFull: every query sees all of them.
+  template <bool kFull, int kHalves>
   __device__ __forceinline__ void take(const Problem& p, const T* kt, const T* vt, int row0, int j0,
                                        float c) {
-    const int lane = threadIdx.x & 63, last = first + 31, j1 = j0 + 31;
-    const bool any = j0 <= last && j0 < length && (j1 > first - p.window || j0 < p.sinks);
-    const bool all = j1 <= first && j1 < length && (j0 > last - p.window || j1 < p.sinks);
-    if (__builtin_expect(!any, 0)) return;
-    Acc s(0.0f);
+    const int lane = threadIdx.x & 63;
+    const bool all = kFull || sees_all(p, j0, 32 * kHalves);
+    if constexpr (!kFull) {
+      if (j0 > first + 31 || j0 >= length ||
+          (j0 + 32 * kHalves - 1 <= first - p.window && j0 >= p.sinks))
+        return;
+    }
+    Acc s[kHalves];
 #pragma unroll
-    for (int st = 0; st < kSteps; ++st) mma(load_rows<T>(kt, kPitchT, row0, 16 * st), q[st], s);
-    if (__builtin_expect(!all, 0)) {
+    for (int h = 0; h < kHalves; ++h) {
+      s[h] = Acc(0.0f);
+#pragma unroll
+      for (int st = 0; st < kSteps; ++st)
+        mma(load_rows<T>(kt, kPitchT, row0 + 32 * h, 16 * st), q[st], s[h]);
+    }
+    if (!all) {
       const KeySight sight(p, pos, j0 + 4 * (lane >> 5), length);
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (!sight.sees(acc_row_of_half(r))) s[r] = -INFINITY;
-    }
-    float m = s[0];
+      for (int h = 0; h < kHalves; ++h)
 #pragma unroll
-    for (int r = 1; r < 16; ++r) m = fmaxf(m, s[r]);
+        for (int r = 0; r < 16; ++r)
+          if (!sight.sees(32 * h + acc_row_of_half(r))) s[h][r] = -INFINITY;
+    }
+    float m = s[0][0];
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) m = fmaxf(m, s[h][r]);
     m *= c;
     // The maximum that exponents are taken against follows the true one at a
     // distance of up to 2^8, so that most tiles rescale nothing, and need nothing
@@ -93,21 +112,25 @@ struct Queries {
     }
     const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-    for (int st = 0; st < 2; ++st) {
-      Frag<T> vf[kBlocks];
+    for (int h = 0; h < kHalves; ++h)
 #pragma unroll
-      for (int n = 0; n < kBlocks; ++n) vf[n] = load_turned<T>(vt, kPitchT, row0 + 16 * st, 32 * n);
+      for (int st = 0; st < 2; ++st) {
+        Frag<T> vf[kBlocks];
 #pragma unroll
-      for (int r = 8 * st; r < 8 * st + 8; ++r) s[r] = power<T>(s[r] * c - base);
-      const Frag<T> pf = acc_frag<T>(s, st);
-      sum = add_all(pf, sum);
-      if (__builtin_expect(!all, 0)) {
-        const KeySight sight(p, pos, j0 + 16 * st, length);
-        poison.guard(vt, kPitchT, row0 + 16 * st, vf, pf, [&](int e) { return sight.sees(e); });
+        for (int n = 0; n < kBlocks; ++n)
+          vf[n] = load_turned<T>(vt, kPitchT, row0 + 32 * h + 16 * st, 32 * n);
+#pragma unroll
+        for (int r = 8 * st; r < 8 * st + 8; ++r) s[h][r] = power<T>(s[h][r] * c - base);
+        const Frag<T> pf = acc_frag<T>(s[h], st);
+        sum = add_all(pf, sum);
+        if (!all) {
+          const KeySight sight(p, pos, j0 + 32 * h + 16 * st, length);
+          poison.guard(vt, kPitchT, row0 + 32 * h + 16 * st, vf, pf,
+                       [&](int e) { return sight.sees(e); });
+        }
+#pragma unroll
+        for (int n = 0; n < kBlocks; ++n) mma(vf[n], pf, o[n]);
       }
-#pragma unroll
-      for (int n = 0; n < kBlocks; ++n) mma(vf[n], pf, o[n]);
-    }
   }
 };
 
@@ -154,16 +177,28 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : kDim <= 64 ? 4 : 2) 
     sv.store(tiles[0][1]);
   }
   __syncthreads();
-  for (int it = 0; it < walk.count; ++it) {
+  const auto turn = [&](int it, auto full) {
     if (it + 1 < walk.count) fetch(it + 1);
-#pragma unroll
-    for (int h = 0; h < kKeys / 32; ++h)
-      w.take(p, tiles[it & 1][0], tiles[it & 1][1], 32 * h, walk.first_key(it) + 32 * h, c);
+    const T* kt = tiles[it & 1][0];
+    const T* vt = tiles[it & 1][1];
+    if constexpr (full) {
+      w.template take<true, kKeys / 32>(p, kt, vt, 0, walk.first_key(it), c);
+    } else {
+#pragma unroll 1
+      for (int h = 0; h < kKeys / 32; ++h)
+        w.template take<false, 1>(p, kt, vt, 32 * h, walk.first_key(it) + 32 * h, c);
+    }
     if (it + 1 < walk.count) {
       sk.store(tiles[(it + 1) & 1][0]);
       sv.store(tiles[(it + 1) & 1][1]);
     }
     __syncthreads();
+  };
+  // Runs of tiles that the wave's queries see whole in a loop of their own:
+  // without branches the compiler lays products over exponentials.
+  for (int it = 0; it < walk.count;) {
+    while (it < walk.count && !w.sees_all(p, walk.first_key(it), kKeys)) turn(it++, std::false_type{});
+    while (it < walk.count && w.sees_all(p, walk.first_key(it), kKeys)) turn(it++, std::true_type{});
   }
   w.poison.apply(w.o);
   const int i = at.block * kQueries + wave * 32 + (lane & 31);
@@ -220,7 +255,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
     sv.store(tiles[wave][1]);
     if (it + kWaves < walk.count) fetch(it + kWaves);
     wave_sync();
-    w.take(p, tiles[wave][0], tiles[wave][1], 0, walk.first_key(it), c);
+    w.template take<false, 1>(p, tiles[wave][0], tiles[wave][1], 0, walk.first_key(it), c);
     wave_sync();
   }
   w.poison.apply(w.o);

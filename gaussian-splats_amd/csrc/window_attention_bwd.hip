@@ -209,71 +209,88 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
     keep(begin & 1);
   }
   __syncthreads();
-  for (int it = begin; it < count; ++it) {
+  // One tile of queries.  `full` (known at compile time): every query of it sees
+  // all of the wave's keys; otherwise each half looks for itself.
+  const auto turn = [&](int it, auto full) {
     if (it + 1 < count) fetch(it + 1);
     const T* qt = tiles[it & 1][0];
     const T* gt = tiles[it & 1][1];
     const int i0 = (first_tile + it % tiles_per_head) * kRows;
-#pragma unroll 1
-    for (int h = 0; h < kRows / 32; ++h) {
+    const auto half = [&](int h) {
       const int p0 = off + i0 + 32 * h, p1 = p0 + 31;  // positions
       const bool inside = i0 + 32 * h >= from && i0 + 32 * h + 31 < to;
       const int w1 = w0 + 31;
-      const bool any = w0 <= p1 && w0 < length && i0 + 32 * h < to &&
-                       (w1 > p0 - p.window || w0 < p.sinks);
-      const bool all = inside && w1 <= p0 && w1 < length &&
-                       (w0 > p1 - p.window || w1 < p.sinks);
-      if (__builtin_expect(any, 1)) {
-        Acc s(0.0f), dp(0.0f);
+      const bool any = full || (w0 <= p1 && w0 < length && i0 + 32 * h < to &&
+                                (w1 > p0 - p.window || w0 < p.sinks));
+      const bool all = full || (inside && w1 <= p0 && w1 < length &&
+                                (w0 > p1 - p.window || w1 < p.sinks));
+      if (!any) return;
+      Acc s(0.0f), dp(0.0f);
 #pragma unroll
-        for (int st = 0; st < kSteps; ++st)
-          mma(load_rows<T>(qt, kPitchT, 32 * h, 16 * st), kf[st], s);
+      for (int st = 0; st < kSteps; ++st)
+        mma(load_rows<T>(qt, kPitchT, 32 * h, 16 * st), kf[st], s);
 #pragma unroll
-        for (int st = 0; st < kSteps; ++st)
-          mma(load_rows<T>(gt, kPitchT, 32 * h, 16 * st), vf[st], dp);
+      for (int st = 0; st < kSteps; ++st)
+        mma(load_rows<T>(gt, kPitchT, 32 * h, 16 * st), vf[st], dp);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int row = 32 * h + acc_row(r);
+        const float lse = rows[it & 1][0][row], delta = rows[it & 1][1][row];
+        s[r] = power<T>(s[r] * c - lse);
+        dp[r] = s[r] * (dp[r] - delta);
+        if constexpr (std::is_same_v<T, f16>) dp[r] *= up;
+      }
+      if (!all) {
+        const QuerySight sight(p, j, i0 + 32 * h + 4 * (lane >> 5), from, to, length);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int row = 32 * h + acc_row(r);
-          const float lse = rows[it & 1][0][row], delta = rows[it & 1][1][row];
-          s[r] = power<T>(s[r] * c - lse);
-          dp[r] = s[r] * (dp[r] - delta);
-          if constexpr (std::is_same_v<T, f16>) dp[r] *= up;
-        }
-        if (__builtin_expect(!all, 0)) {
-          const QuerySight sight(p, j, i0 + 32 * h + 4 * (lane >> 5), from, to, length);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const bool see = sight.sees(acc_row_of_half(r));
-            s[r] = see ? s[r] : 0.0f;
-            dp[r] = see ? dp[r] : 0.0f;
-          }
-        }
-        // Two products that contract over the queries: of a tile's turned rows
-        // and the probabilities or their gradients.
-        const auto add = [&](const T* tile, const Acc& x, Poison<T, kBlocks>& poison,
-                             Acc (&acc)[kBlocks], int st) {
-          const Frag<T> xf = acc_frag<T>(x, st);
-          Frag<T> f[kBlocks];
-#pragma unroll
-          for (int n = 0; n < kBlocks; ++n)
-            f[n] = load_turned<T>(tile, kPitchT, 32 * h + 16 * st, 32 * n);
-          if (__builtin_expect(!all, 0)) {
-            const QuerySight sight(p, j, i0 + 32 * h + 16 * st, from, to, length);
-            poison.guard(tile, kPitchT, 32 * h + 16 * st, f, xf,
-                         [&](int e) { return sight.sees(e); });
-          }
-#pragma unroll
-          for (int n = 0; n < kBlocks; ++n) mma(f[n], xf, acc[n]);
-        };
-#pragma unroll
-        for (int st = 0; st < 2; ++st) {
-          add(gt, s, pv, dv, st);
-          add(qt, dp, pk, dk, st);
+          const bool see = sight.sees(acc_row_of_half(r));
+          s[r] = see ? s[r] : 0.0f;
+          dp[r] = see ? dp[r] : 0.0f;
         }
       }
+      // Two products that contract over the queries: of a tile's turned rows and
+      // the probabilities or their gradients.
+      const auto add = [&](const T* tile, const Acc& x, Poison<T, kBlocks>& poison,
+                           Acc (&acc)[kBlocks], int st) {
+        const Frag<T> xf = acc_frag<T>(x, st);
+        Frag<T> f[kBlocks];
+#pragma unroll
+        for (int n = 0; n < kBlocks; ++n)
+          f[n] = load_turned<T>(tile, kPitchT, 32 * h + 16 * st, 32 * n);
+        if (!all) {
+          const QuerySight sight(p, j, i0 + 32 * h + 16 * st, from, to, length);
+          poison.guard(tile, kPitchT, 32 * h + 16 * st, f, xf, [&](int e) { return sight.sees(e); });
+        }
+#pragma unroll
+        for (int n = 0; n < kBlocks; ++n) mma(f[n], xf, acc[n]);
+      };
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        add(gt, s, pv, dv, st);
+        add(qt, dp, pk, dk, st);
+      }
+    };
+    if constexpr (full) {
+#pragma unroll
+      for (int h = 0; h < kRows / 32; ++h) half(h);
+    } else {
+#pragma unroll 1
+      for (int h = 0; h < kRows / 32; ++h) half(h);
     }
     if (it + 1 < count) keep((it + 1) & 1);
     __syncthreads();
+  };
+  const auto full_tile = [&](int it) {
+    const int i0 = (first_tile + it % tiles_per_head) * kRows;
+    return i0 >= from && i0 + kRows <= to && w0 + 31 <= off + i0 && w0 + 31 < length &&
+           (w0 > off + i0 + kRows - 1 - p.window || w0 + 31 < p.sinks);
+  };
+  // Runs of full tiles in a loop of their own: without branches the compiler
+  // lays the products of one half over the exponentials of the other.
+  for (int it = begin; it < count;) {
+    while (it < count && !full_tile(it)) turn(it++, std::false_type{});
+    while (it < count && full_tile(it)) turn(it++, std::true_type{});
   }
   pk.apply(dk);
   pv.apply(dv);
@@ -368,13 +385,22 @@ struct GradQueries {
     for (int n = 0; n < kBlocks; ++n) dq[n] = Acc(0.0f);
   }
 
-  // 32 keys from j0 on, rows row0 .. of the LDS tiles kt and vt.
+  // Whether every query sees each of `keys` keys from j0 on.
+  __device__ __forceinline__ bool sees_all(const Problem& p, int j0, int keys) const {
+    const int last = first + 31, j1 = j0 + keys - 1;
+    return j1 <= first && j1 < length && (j0 > last - p.window || j1 < p.sinks);
+  }
+
+  // 32 keys from j0 on, rows row0 .. of the LDS tiles kt and vt.  kFull: every
+  // query sees all of them.
+  template <bool kFull>
   __device__ __forceinline__ void take(const Problem& p, const T* kt, const T* vt, int row0, int j0,
                                        float c) {
-    const int lane = threadIdx.x & 63, last = first + 31, j1 = j0 + 31;
-    const bool any = j0 <= last && j0 < length && (j1 > first - p.window || j0 < p.sinks);
-    const bool all = j1 <= first && j1 < length && (j0 > last - p.window || j1 < p.sinks);
-    if (__builtin_expect(!any, 0)) return;
+    const int lane = threadIdx.x & 63;
+    const bool all = kFull || sees_all(p, j0, 32);
+    if constexpr (!kFull) {
+      if (j0 > first + 31 || j0 >= length || (j0 + 31 <= first - p.window && j0 >= p.sinks)) return;
+    }
     Acc s(0.0f), dp(0.0f);
 #pragma unroll
     for (int st = 0; st < kSteps; ++st) mma(load_rows<T>(kt, kPitchT, row0, 16 * st), q[st], s);
@@ -382,7 +408,7 @@ struct GradQueries {
     for (int st = 0; st < kSteps; ++st) mma(load_rows<T>(vt, kPitchT, row0, 16 * st), g[st], dp);
 #pragma unroll
     for (int r = 0; r < 16; ++r) dp[r] = power<T>(s[r] * c - lse) * (dp[r] - delta);
-    if (__builtin_expect(!all, 0)) {
+    if (!all) {
       const KeySight sight(p, pos, j0 + 4 * (lane >> 5), length);
 #pragma unroll
       for (int r = 0; r < 16; ++r) dp[r] = sight.sees(acc_row_of_half(r)) ? dp[r] : 0.0f;
@@ -393,7 +419,7 @@ struct GradQueries {
       Frag<T> f[kBlocks];
 #pragma unroll
       for (int n = 0; n < kBlocks; ++n) f[n] = load_turned<T>(kt, kPitchT, row0 + 16 * st, 32 * n);
-      if (__builtin_expect(!all, 0)) {
+      if (!all) {
         const KeySight sight(p, pos, j0 + 16 * st, length);
         poison.guard(kt, kPitchT, row0 + 16 * st, f, df, [&](int e) { return sight.sees(e); });
       }
@@ -445,16 +471,29 @@ attention_bwd_queries_kernel(BackwardArgs a) {
     sv.store(tiles[0][1]);
   }
   __syncthreads();
-  for (int it = 0; it < walk.count; ++it) {
+  const auto turn = [&](int it, auto full) {
     if (it + 1 < walk.count) fetch(it + 1);
+    const T* kt = tiles[it & 1][0];
+    const T* vt = tiles[it & 1][1];
+    if constexpr (full) {
+#pragma unroll
+      for (int h = 0; h < kRows / 32; ++h)
+        w.template take<true>(p, kt, vt, 32 * h, walk.first_key(it) + 32 * h, c);
+    } else {
 #pragma unroll 1
-    for (int h = 0; h < kRows / 32; ++h)
-      w.take(p, tiles[it & 1][0], tiles[it & 1][1], 32 * h, walk.first_key(it) + 32 * h, c);
+      for (int h = 0; h < kRows / 32; ++h)
+        w.template take<false>(p, kt, vt, 32 * h, walk.first_key(it) + 32 * h, c);
+    }
     if (it + 1 < walk.count) {
       sk.store(tiles[(it + 1) & 1][0]);
       sv.store(tiles[(it + 1) & 1][1]);
     }
     __syncthreads();
+  };
+  // Runs of tiles that the wave's queries see whole in a loop of their own.
+  for (int it = 0; it < walk.count;) {
+    while (it < walk.count && !w.sees_all(p, walk.first_key(it), kRows)) turn(it++, std::false_type{});
+    while (it < walk.count && w.sees_all(p, walk.first_key(it), kRows)) turn(it++, std::true_type{});
   }
   w.poison.apply(w.dq);
   const int i = query + (lane & 31);
@@ -503,7 +542,7 @@ attention_bwd_queries_split_kernel(BackwardArgs a) {
     sv.store(tiles[wave][1]);
     if (it + kWaves < walk.count) fetch(it + kWaves);
     wave_sync();
-    w.take(p, tiles[wave][0], tiles[wave][1], 0, walk.first_key(it), c);
+    w.template take<false>(p, tiles[wave][0], tiles[wave][1], 0, walk.first_key(it), c);
     wave_sync();
   }
   w.poison.apply(w.dq);
