@@ -17,6 +17,12 @@
 //
 // A lane holds two neighbouring channels of a 16-bit type where rows allow
 // 4-byte accesses.
+//
+// Bound by memory in principle.  Measured, bfloat16, [1, 160000, 768]: forward 191
+// us for 0.74 GB (3.9 TB/s, where a large copy moves 5.2), backward 311 us for 1.23
+// GB (4.0 TB/s): a workgroup fills a CU, and its items' loads run ahead by one item,
+// but what a look back waits for is not all hidden.  Three kernels that read the
+// inputs twice (maps, walk, run) took 375 and 500 us.
 #include "sequence.h"
 
 namespace gs {

@@ -11,6 +11,14 @@
 // one exchange with the other half, and the exponentials are the next product's
 // operand in place.  Probabilities are rounded to the inputs' type for that
 // product and for the sum alike, so that a row's weights add up to one.
+//
+// Measured, bfloat16, 40000 tokens, 12 heads of 64 on 4, window 5000: 0.78 ms, 740
+// TFLOP/s, where a large square matrix product reaches 1126.  Matrix cores are
+// busy 40 % of the time, a SIMD issues vector instructions (half of them the
+// exponentials' path) for about 45 %, LDS serves for 40 %: what is left is the
+// latency from one to the other, which four waves a SIMD hide in part.  64
+// queries a wave would halve the LDS reads but leave two waves a SIMD: 0.90 ms.
+// float16, 2 x 8160 tokens, 16 heads of 128: 0.34 ms, 670 TFLOP/s at two waves.
 #include "attention_tile.h"
 
 namespace gs {

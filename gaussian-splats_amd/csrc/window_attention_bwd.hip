@@ -14,6 +14,10 @@
 // than a window, is cut into segments of about the others' length, each a
 // workgroup of its own that leaves float32 sums, which a last kernel adds in the
 // order of the segments.  Where there are few keys the other walks are cut too.
+// Measured, bfloat16, 40000 tokens, 12 heads of 64 on 4, window 5000: keys 1.57 ms
+// (730 TFLOP/s, two waves a SIMD, 212 registers), queries 1.01 ms (850 TFLOP/s,
+// three waves); bound as the forward is.  64 keys a wave: 2.57 ms, one wave a SIMD.
+//
 // dS is an operand of products in the inputs' type.  float16 would lose small
 // values of it below its normal range and large ones above it, as gradients come
 // in any size (and P is about one over the window): there dS carries a power of

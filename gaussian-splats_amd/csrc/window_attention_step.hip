@@ -9,6 +9,9 @@
 // workgroups a second kernel joins those, both in a fixed order.  The new token's
 // key and value come from the call's own inputs, not from the cache: the one
 // workgroup whose share holds their slot writes them there, and no other reads it.
+//
+// Measured, bfloat16, 32 streams of up to 8176 slots, 32 heads of 128 on 8: 189 us
+// for 975 MB, 5.1 TB/s, where a large copy moves 5.2; the join 5.5 us.
 #include "attention_tile.h"
 
 namespace gs {
@@ -219,8 +222,10 @@ __global__ __launch_bounds__(128) void attention_step_join_kernel(StepArgs a) {
   static_cast<T*>(a.out)[row * a.dim + d] = T(none ? 0.0f : o / sum);
 }
 
-// Workgroups of one stream and key head: as many as fill the GPU a few times
-// over, with a tile for each of their waves.
+// Workgroups of one stream and key head: as many as fill the GPU three times over
+// (512 at a time; streams of different lengths even out), with a tile for each of
+// their waves.  The case above with 1024 workgroups: 202 us, 1536: 189, 2048: 196,
+// 3072: 272.
 int plan_splits(const gs_attention& d) {
   const int64_t capacity = d.sinks + d.window;
   const int64_t rows = d.batch * d.kv_heads * ((d.heads / d.kv_heads + 31) / 32);

@@ -126,7 +126,7 @@ GS_API int gs_camera_rotation(float w, float x, float y, float z, float* rotatio
 GS_API int gs_arm_launch_events(void* start_event, void* stop_event);
 GS_API int gs_disarm_launch_events(void);
 
-/* Device-side check failures.  The binning and sort kernels validate what
+/* Device-side check failures.  The binning, sort and scan kernels validate what
  * they cannot check on the host (sizes passed between calls against the
  * plan's device totals, the bounded spin of their look-back waits, owner
  * windows) and, on a failure, leave their outputs incomplete and OR one of
