@@ -54,16 +54,17 @@ struct Gate {
 template <typename T>
 __device__ __forceinline__ Gate gate_of(float g) {
   // With e = exp(-g), a = 1 / (1 + e) and 1 - a = e a lose no bits near 0 or 1.
-  // Where e overflows a is 0 and e a a NaN, of which the minimum makes 1; a NaN
-  // of g stays in a.  float32 inputs get the library's exp; for 16-bit ones the
-  // instruction's error is far below their rounding.
+  // Where e is huge a may be 0 (the reciprocal instruction's results have no
+  // subnormals) and e a anything: 1 - a is 1 there.  A NaN of g stays in both.
+  // float32 inputs get the library's exp; for 16-bit ones the instruction's error
+  // is far below their rounding.
   float e;
   if constexpr (sizeof(T) == 4)
     e = expf(-g);
   else
     e = __builtin_amdgcn_exp2f(g * -1.44269504f);
   const float a = __builtin_amdgcn_rcpf(1.0f + e);
-  return {a, fminf(e * a, 1.0f)};
+  return {a, e > 1e30f ? 1.0f : e * a};
 }
 
 // N channels of one lane.

@@ -436,11 +436,14 @@ int check_norm(int64_t rows, int64_t width, int32_t x_type, int32_t r_type, int3
   return GS_OK;
 }
 
+// Whether rows `stride` apart allow accesses to eight elements at once.
+bool fits(const void* p, int32_t type, int64_t stride) {
+  const size_t bytes = 8 * size_t(type_bytes(type));
+  return !p || (aligned_to(p, bytes) && (stride * type_bytes(type)) % int64_t(bytes) == 0);
+}
+
 int run_norm(NormArgs a, int32_t x_type, int32_t r_type, void* stream) {
   if (a.rows == 0) return GS_OK;
-  const auto fits = [&](const void* p, int32_t type, int64_t stride) {
-    return !p || (aligned_to(p, 16) && (stride * type_bytes(type)) % 16 == 0);
-  };
   const bool vec = a.width % 8 == 0 && fits(a.x, x_type, a.x_stride) &&
                    fits(a.residual, r_type, a.residual_stride) && fits(a.sum, r_type, 8) &&
                    fits(a.weight, a.weight_type, 8) && fits(a.y, x_type, 8);
@@ -521,13 +524,10 @@ extern "C" GS_API int gs_add_rms_norm_bwd(const void* sum, const void* weight,
                 grad_residual, grad_weight ? static_cast<float*>(workspace) : nullptr};
   const int blocks = rows ? partial_rows(rows, int(width)) : 0;
   if (rows) {
-    const auto fits = [&](const void* p, int32_t type, int64_t stride) {
-      return !p || (aligned_to(p, 16) && (stride * type_bytes(type)) % 16 == 0);
-    };
     const bool vec = width % 8 == 0 && fits(sum, residual_type, sum_stride) &&
                      fits(weight, weight_type, 8) && fits(grad_y, x_type, 8) &&
                      fits(grad_sum, residual_type, 8) && fits(grad_x, x_type, 8) &&
-                     fits(grad_residual, residual_type, 8) && aligned_to(workspace, 16);
+                     fits(grad_residual, residual_type, 8) && fits(workspace, GS_F32, 8);
     GS_TRY(with_types(x_type, residual_type, [&](auto x, auto r) {
       using TX = decltype(x);
       using TR = decltype(r);

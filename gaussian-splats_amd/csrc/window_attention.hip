@@ -367,6 +367,9 @@ int check_rows(const void* p, const int64_t* strides, int32_t type, const char* 
   GS_REQUIRE(seq::aligned_to(p, 16) && strides[0] % unit == 0 && strides[1] % unit == 0 &&
                  strides[2] % unit == 0,
              GS_ERR_INVALID_ARGUMENT, "%s must have rows on 16-byte boundaries", name);
+  // A tile's rows lie within 32 bits of its first one.
+  GS_REQUIRE(strides[1] >= 0 && strides[1] < (int64_t(1) << 24), GS_ERR_OVERFLOW,
+             "the tokens of %s lie too far apart (%lld elements)", name, (long long)strides[1]);
   return GS_OK;
 }
 

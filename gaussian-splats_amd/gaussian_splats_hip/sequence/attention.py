@@ -47,9 +47,11 @@ def _check_sizes(window: int, sinks: int, heads: int, kv_heads: int) -> None:
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
     """Rows that start on 16-byte boundaries, neighbouring elements side by
-    side; a copy where the strides do not give that."""
+    side and tokens less than 2^24 elements apart; a copy where the strides do
+    not give that."""
     unit = 16 // t.element_size()
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % unit for s in t.stride()[:-1]):
+    if (t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % unit for s in t.stride()[:-1])
+            or t.stride(1) >= 1 << 24):
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()

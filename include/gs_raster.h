@@ -734,7 +734,8 @@ typedef struct gs_attention {
 } gs_attention;
 
 /* strides, host memory: batch, token and head stride of q, of k and of v;
- * rows start on 16-byte boundaries.  Writes out [batch, queries, heads,
+ * rows start on 16-byte boundaries, tokens lie less than 2^24 elements apart
+ * (GS_ERR_OVERFLOW otherwise).  Writes out [batch, queries, heads,
  * head_dim] and lse, the logarithm of each softmax's sum (float32 [batch,
  * heads, queries]; -inf where a query sees no key). */
 GS_API int gs_window_attention_fwd(

@@ -88,6 +88,38 @@ def test_gates_at_infinity(dtype):
     _check(x, gate, None, normal(shape, dtype, 3), normal((1, 10), torch.float32, 4))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gates_of_any_size(dtype):
+    """Gates far beyond what an exponential holds, and where it is about to
+    overflow: forgetting keeps x, remembering keeps h, a NaN stays in its channel."""
+    sizes = [-6e4, -120.0, -104.0, -90.0, -89.0, -88.5, -88.0, -87.5, -87.0, -80.0, -70.0, -69.0, -40.0,
+             -10.0, 0.0, 10.0, 40.0, 70.0, 80.0, 87.0, 88.0, 89.0, 104.0, 120.0, 6e4]
+    gate = torch.tensor(sizes).to(dtype).expand(1, 9, -1).contiguous()
+    x, state = normal(gate.shape, dtype, 1), normal((1, len(sizes)), torch.float32, 2)
+    _check(x, gate, state, normal(gate.shape, dtype, 3), normal((1, len(sizes)), torch.float32, 4))
+    row, _ = gated_scan_step(x[:, 0].to(DEV), gate[:, 0].to(DEV), state.to(DEV))
+    want, _ = orc.gated_scan(x[:, :1], gate[:, :1], state)
+    assert_within(row, want[:, 0], want[:, 0].abs() * UNIT[dtype] + 40 * U32 * 4, "step")
+    gate[0, 4, 3] = float("nan")
+    y, _ = gated_scan(x.to(DEV), gate.to(DEV), state.to(DEV))
+    bad = torch.isnan(y[0].cpu())
+    assert bad[4:, 3].all() and int(bad.sum()) == 5
+
+
+def test_offsets_beyond_32_bits():
+    """Sequences whose tensors lie more than 2^31 elements apart."""
+    apart, shape = (1 << 31) + 64, (2, 40, 16)
+    far = [torch.empty(apart + 640, dtype=torch.bfloat16, device=DEV).as_strided(shape, (apart, 16, 1))
+           for _ in range(3)]
+    near = [normal(shape, torch.bfloat16, i).to(DEV) for i in range(3)]
+    for a, b in zip(far, near):
+        a.copy_(b)
+    out = [gated_scan_forward(*t[:2]) for t in (far, near)]
+    grads = [gated_scan_backward(t[0], t[1], o[2], t[2], None) for t, o in zip((far, near), out)]
+    for a, b in zip((*out[0], *grads[0]), (*out[1], *grads[1])):
+        assert torch.equal(a, b)
+
+
 def test_strides_and_alignment():
     base = normal((3, 700, 300), torch.bfloat16, 1).to(DEV)
     for x in (base[:, :, 40:140], base[:, :, 1:100], base[:, ::2, 10:110], base[:, :, :7],
@@ -174,6 +206,33 @@ def test_same_bits_again_and_on_another_stream():
     torch.cuda.synchronize()
     for a, b in zip(first, second):
         assert torch.equal(a, b)
+
+
+def test_scan_in_a_graph():
+    """Replays of a captured scan and its backward on new inputs, with eager work
+    between them, equal eager calls."""
+    shape = (2, 700, 130)
+    x, gate, dy = (normal(shape, torch.bfloat16, i).to(DEV) for i in range(3))
+
+    def both():
+        y, last, starts = gated_scan_forward(x, gate)
+        return y, last, *gated_scan_backward(x, gate, starts, dy, last)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = both()
+    for t in range(4):
+        for i, v in enumerate((x, gate, dy)):
+            v.copy_(normal(shape, torch.bfloat16, 10 * t + i))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, both()):
+            assert torch.equal(a, b), t
 
 
 def test_empty():

@@ -288,6 +288,36 @@ def test_empty():
     assert out.shape == q.shape and not dk.any() and not dv.any()
 
 
+def test_offsets_beyond_32_bits():
+    """Sequences and cache rows that lie more than 2^31 elements apart."""
+    apart = (1 << 31) + 64
+
+    def spread(t):
+        flat = torch.empty(apart + t[0].numel(), dtype=t.dtype, device=DEV)
+        far = flat.as_strided(t.shape, (apart, *t.stride()[1:]))
+        far.copy_(t)
+        return far
+
+    near = [t.to(DEV) for t in _inputs(2, 70, 70, 2, 1, 64, torch.bfloat16)]
+    far = [spread(t) for t in near]
+    out = [window_attention_forward(*t, 30, 2) for t in (near, far)]
+    grads = [window_attention_backward(*t, *o, near[0], 30, 2) for t, o in zip((near, far), out)]
+    for a, b in zip((*out[0], *grads[0]), (*out[1], *grads[1])):
+        assert torch.equal(a, b)
+    # A window's tokens far apart: copied together first.
+    wide = spread(near[1][:, :2].transpose(0, 1).contiguous()).transpose(0, 1)
+    assert torch.equal(window_attention_forward(near[0][:, :2], wide, near[2][:, :2], 30)[0],
+                       window_attention_forward(near[0][:, :2], near[1][:, :2], near[2][:, :2], 30)[0])
+    del far, wide
+    cache = [t.clone() for t in near[1:]]
+    far = [spread(t) for t in near[1:]]
+    q, kv = near[0][:, 0].contiguous(), near[1][:, 1].contiguous()
+    at = torch.tensor([69, 200], dtype=torch.int32, device=DEV)
+    a = window_attention_step(q, kv, kv, *cache, at, 66, 4)
+    b = window_attention_step(q, kv, kv, *far, at, 66, 4)
+    assert torch.equal(a, b) and all(torch.equal(x, y) for x, y in zip(cache, far))
+
+
 def _step_bound(q, k_cache, v_cache, want, positions, dtype):
     d = q.shape[-1]
     size = float(q.double().norm(dim=-1).max() * k_cache.double().norm(dim=-1).max()) / math.sqrt(d)

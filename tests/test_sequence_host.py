@@ -181,6 +181,8 @@ def test_attention_c_abi_checks():
     assert fwd(q=ctypes.c_void_p(8)) == nat.GS_ERR_INVALID_ARGUMENT
     odd = (ctypes.c_int64 * 12)(*[65] * 12)
     assert fwd(strides=odd) == nat.GS_ERR_INVALID_ARGUMENT and b"16-byte" in lib.gs_last_error()
+    far = (ctypes.c_int64 * 12)(*[1 << 24] * 12)
+    assert fwd(strides=far) == nat.GS_ERR_OVERFLOW and b"far apart" in lib.gs_last_error()
     assert fwd(batch=0) == nat.GS_OK and fwd(queries=0) == nat.GS_OK
     d = _attention()
     ws = lib.gs_window_attention_bwd_workspace_bytes(ctypes.byref(d))
