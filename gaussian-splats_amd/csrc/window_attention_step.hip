@@ -225,7 +225,7 @@ __global__ __launch_bounds__(128) void attention_step_join_kernel(StepArgs a) {
 // Workgroups of one stream and key head: as many as fill the GPU three times over
 // (512 at a time; streams of different lengths even out), with a tile for each of
 // their waves.  The case above with 1024 workgroups: 202 us, 1536: 189, 2048: 196,
-// 3072: 272.
+// twice 1536: 272.
 int plan_splits(const gs_attention& d) {
   const int64_t capacity = d.sinks + d.window;
   const int64_t rows = d.batch * d.kv_heads * ((d.heads / d.kv_heads + 31) / 32);
