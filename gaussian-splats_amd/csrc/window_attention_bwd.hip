@@ -689,8 +689,9 @@ extern "C" GS_API int gs_window_attention_bwd(const gs_attention* desc, const vo
   const hipStream_t s = as_stream(stream);
   return seq::with_type(desc->type, [&](auto t) {
     using T = decltype(t);
+    // Without queries the keys' kernel reads it all the same.
+    if (std::is_same_v<T, f16>) attention_clear_kernel<<<1, 1, 0, s>>>(a.largest);
     if (rows) {
-      if (std::is_same_v<T, f16>) attention_clear_kernel<<<1, 1, 0, s>>>(a.largest);
       attention_delta_kernel<T><<<unsigned((rows + 15) / 16), 256, 0, s>>>(a);
       GS_TRY(check_launch("window_attention backward"));
     }

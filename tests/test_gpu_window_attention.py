@@ -399,3 +399,16 @@ def test_step_in_a_graph():
         torch.cuda.synchronize()
         assert torch.equal(out, twin.step(q, k, v)), t
         assert torch.equal(cache.k, twin.k) and torch.equal(cache.positions, twin.positions)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_no_queries(dtype):
+    """Keys without a query get zeros, whatever the workspace held before."""
+    q, k, v = (t.to(DEV) for t in _inputs(2, 0, 70, 2, 1, 64, dtype))
+    out, lse = window_attention_forward(q, k, v, 4, 1)
+    torch.cuda.empty_cache()
+    old = [torch.full((1 << 17,), -1.0, device=DEV) for _ in range(4)]
+    del old  # small allocations are cut from these
+    _, dk, dv = window_attention_backward(q, k, v, out, lse, out, 4, 1)
+    for t in (dk, dv):
+        assert torch.isfinite(t).all() and not t.any()
