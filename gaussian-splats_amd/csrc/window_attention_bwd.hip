@@ -19,10 +19,13 @@
 // three waves); bound as the forward is.  64 keys a wave: 2.57 ms, one wave a SIMD.
 //
 // dS is an operand of products in the inputs' type.  float16 would lose small
-// values of it below its normal range and large ones above it, as gradients come
-// in any size (and P is about one over the window): there dS carries a power of
-// two that brings the largest |grad_out| to between 4 and 8, taken out of the
-// sums in float32.
+// values of it below its normal range and large ones above it, as gradients and
+// values come in any size (and P is about one over the window): there dS carries
+// a power of two, taken out of the sums in float32.  |dP - delta| is at most
+// B = 2 max|grad_out_i| max|v_j| over the rows of a sequence that share a key
+// head; the power brings B to between 2^13 and 2^15, half of what the type holds,
+// so nothing overflows, and what is lost is below 2^-24 / 2^13 of B.  Each
+// sequence and key head has its own, so none takes bits of another.
 #include "attention_tile.h"
 
 namespace gs {
@@ -49,7 +52,9 @@ struct BackwardArgs {
   Strides sq, sk, sv, sg;
   const float* lse;
   float* delta;  // [batch, heads, queries]
-  uint32_t* largest;  // float16: the bits of the largest finite |grad_out|
+  // float16, [batch, kv_heads, 2]: the bits of the largest |grad_out_i|^2 and
+  // |v_j|^2, of rows that count, without elements that are not finite.
+  uint32_t* sizes;
   void* dq;
   void* dk;
   void* dv;
@@ -78,24 +83,66 @@ __device__ __forceinline__ int64_t part_index(const BackwardArgs& a, int b, int 
 
 // The power of two that dS carries.
 template <typename T>
-__device__ __forceinline__ int gradient_shift(const BackwardArgs& a) {
+__device__ __forceinline__ int gradient_shift(const BackwardArgs& a, int b, int kv) {
   if constexpr (std::is_same_v<T, f16>) {
-    const uint32_t bits = *a.largest;
-    if (bits != 0) return 129 - int(bits >> 23);  // 2^(bits >> 23 - 127) to 2^2
+    const uint32_t* sizes = a.sizes + (int64_t(b) * a.p.kv_heads + kv) * 2;
+    const uint32_t grad = sizes[0], value = sizes[1];
+    // A square below 2^e: B = 2 sqrt(their product) is below 2^(1 + half the sum of
+    // the exponents, rounded up).
+    if (grad != 0 && value != 0) return 14 - ((int(grad >> 23) + int(value >> 23) - 252 + 1) >> 1);
   }
   return 0;
 }
 
-__global__ void attention_clear_kernel(uint32_t* largest) { *largest = 0; }
+__global__ __launch_bounds__(256) void attention_clear_kernel(uint32_t* words, int64_t count) {
+  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (i < count) words[i] = 0;
+}
 
-// delta, a group of 16 lanes for each row.
+// Sum of the finite elements' squares.
+__device__ __forceinline__ float square(const Frag<f16>& f) {
+  float sum = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float x = float(f[e]);
+    sum = finite(x) ? sum + x * x : sum;
+  }
+  return sum;
+}
+// A row's square, of which 16 lanes hold a part each, into the largest one.  A
+// maximum does not depend on the order; most rows find a larger one there.
+__device__ __forceinline__ void note_size(uint32_t* largest, float part, bool counts) {
+#pragma unroll
+  for (int s = 8; s > 0; s >>= 1) part += __shfl_xor(part, s, 64);
+  const uint32_t bits = __float_as_uint(part);
+  if (counts && (threadIdx.x & 15) == 0 &&
+      bits > __hip_atomic_load(largest, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
+    atomicMax(largest, bits);
+}
+
+// delta, a group of 16 lanes for each row; float16: the sizes of grad_out's rows
+// and, in the workgroups from row_blocks on, those of v's.
 template <typename T>
-__global__ __launch_bounds__(256) void attention_delta_kernel(BackwardArgs a) {
+__global__ __launch_bounds__(256) void attention_delta_kernel(BackwardArgs a, unsigned row_blocks) {
   const Problem& p = a.p;
   const int64_t rows = int64_t(p.batch) * p.queries * p.heads;
-  const int64_t row = int64_t(blockIdx.x) * 16 + (threadIdx.x >> 4);
   const int d = (threadIdx.x & 15) * 8;
-  float sum = 0.0f, top = 0.0f;
+  if constexpr (std::is_same_v<T, f16>) {
+    if (blockIdx.x >= row_blocks) {
+      const int64_t at = int64_t(blockIdx.x - row_blocks) * 16 + (threadIdx.x >> 4);
+      const bool in = at < int64_t(p.batch) * p.keys * p.kv_heads;
+      const int kv = in ? int(at % p.kv_heads) : 0;
+      const int64_t j = in ? at / p.kv_heads % p.keys : 0, b = in ? at / p.kv_heads / p.keys : 0;
+      const bool counts = in && j < p.length(int(b));
+      const Frag<T> v = load_global<T>(static_cast<const T*>(a.v) + b * a.sv.batch +
+                                           j * a.sv.token + kv * a.sv.head + d,
+                                       counts && d < p.dim);
+      note_size(a.sizes + (b * p.kv_heads + kv) * 2 + 1, square(v), counts);
+      return;
+    }
+  }
+  const int64_t row = int64_t(blockIdx.x) * 16 + (threadIdx.x >> 4);
+  float sum = 0.0f, size = 0.0f;
   const int head = int(row % p.heads);
   const int64_t i = row / p.heads % p.queries, b = row / p.heads / p.queries;
   if (row < rows && d < p.dim) {
@@ -103,18 +150,14 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(BackwardArgs a) {
     const Frag<T> g = load_global<T>(static_cast<const T*>(a.grad) + b * a.sg.batch +
                                          i * a.sg.token + head * a.sg.head + d, true);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      sum += float(o[e]) * float(g[e]);
-      const float size = fabsf(float(g[e]));
-      top = finite(size) ? fmaxf(top, size) : top;
-    }
+    for (int e = 0; e < 8; ++e) sum += float(o[e]) * float(g[e]);
+    if constexpr (std::is_same_v<T, f16>) size = square(g);
   }
   if constexpr (std::is_same_v<T, f16>) {
-#pragma unroll
-    for (int s = 32; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
-    // A maximum does not depend on the order; most waves find a larger one there.
-    if ((threadIdx.x & 63) == 0 && __float_as_uint(top) > *a.largest)
-      atomicMax(a.largest, __float_as_uint(top));
+    // A query that sees nothing has no dS.
+    const bool counts = row < rows && a.lse[(b * p.heads + head) * p.queries + i] != -INFINITY;
+    const int64_t kv = head / (p.heads / p.kv_heads);
+    note_size(a.sizes + (counts ? (b * p.kv_heads + kv) * 2 : 0), size, counts);
   }
 #pragma unroll
   for (int s = 8; s > 0; s >>= 1) sum += __shfl_xor(sum, s, 64);
@@ -177,7 +220,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
   const int64_t walk = int64_t(tiles_per_head) * group;
   const int begin = int(walk * segment / pieces), count = int(walk * (segment + 1) / pieces);
 
-  const int shift = gradient_shift<T>(a);
+  const int shift = gradient_shift<T>(a, b, kv);
   const float up = ldexpf(1.0f, shift), down = ldexpf(1.0f, -shift);
   Acc dk[kBlocks], dv[kBlocks];
   Poison<T, kBlocks> pk, pv;
@@ -381,7 +424,7 @@ struct GradQueries {
       g[s] = load_global<T>(gr + d, live && d < p.dim);
     }
     const int64_t at = (int64_t(b) * p.heads + head) * p.queries + i;
-    const int shift = gradient_shift<T>(a);
+    const int shift = gradient_shift<T>(a, b, head / (p.heads / p.kv_heads));
     lse = live ? a.lse[at] * kLog2e - float(shift) : 0.0f;
     delta = live ? a.delta[at] : 0.0f;
     factor = ldexpf(p.scale, -shift);
@@ -604,9 +647,10 @@ void plan_segments(const Problem& p, int32_t type, BackwardArgs& a) {
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
+// delta and, behind it, float16's sizes.
 size_t delta_bytes(const Problem& p) {
-  return align256(size_t(p.batch) * size_t(p.heads) * size_t(p.queries) * sizeof(float) +
-                  sizeof(uint32_t));
+  return align256(size_t(p.batch) * (size_t(p.heads) * size_t(p.queries) + 2 * size_t(p.kv_heads)) *
+                  sizeof(float));
 }
 
 }  // namespace
@@ -675,7 +719,8 @@ extern "C" GS_API int gs_window_attention_bwd(const gs_attention* desc, const vo
   a.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes(a.p));
   const Problem& p = a.p;
   const int64_t rows = int64_t(p.batch) * p.queries * p.heads;
-  a.largest = reinterpret_cast<uint32_t*>(a.delta + rows);
+  a.sizes = reinterpret_cast<uint32_t*>(a.delta + rows);
+  const int64_t value_rows = desc->type == GS_F16 ? int64_t(p.batch) * p.keys * p.kv_heads : 0;
   const int64_t blocks = key_blocks(p), others = blocks - a.sink_blocks;
   const int64_t key_items = (int64_t(a.sink_blocks) * a.sink_segments + others * a.segments) *
                             p.kv_heads * p.batch;
@@ -683,16 +728,21 @@ extern "C" GS_API int gs_window_attention_bwd(const gs_attention* desc, const vo
   const int join_first = a.sink_segments > 1 ? 0 : a.sink_blocks;
   const int join_blocks = int((a.sink_segments > 1 ? a.sink_blocks : 0) + (a.segments > 1 ? others : 0));
   const int64_t joined = int64_t(p.batch) * p.kv_heads * join_blocks * kBlockKeys * p.dim / 4;
-  GS_REQUIRE(rows / 16 < (int64_t(1) << 30) && key_items < (int64_t(1) << 30) &&
+  GS_REQUIRE((rows + value_rows) / 16 < (int64_t(1) << 30) && key_items < (int64_t(1) << 30) &&
                  joined / 256 < (int64_t(1) << 30),
              GS_ERR_OVERFLOW, "attention problem too large");
   const hipStream_t s = as_stream(stream);
   return seq::with_type(desc->type, [&](auto t) {
     using T = decltype(t);
-    // Without queries the keys' kernel reads it all the same.
-    if (std::is_same_v<T, f16>) attention_clear_kernel<<<1, 1, 0, s>>>(a.largest);
+    // Without queries the keys' kernel reads them all the same.
+    if (std::is_same_v<T, f16>) {
+      const int64_t words = int64_t(p.batch) * p.kv_heads * 2;
+      attention_clear_kernel<<<unsigned((words + 255) / 256), 256, 0, s>>>(a.sizes, words);
+    }
     if (rows) {
-      attention_delta_kernel<T><<<unsigned((rows + 15) / 16), 256, 0, s>>>(a);
+      const unsigned row_blocks = unsigned((rows + 15) / 16);
+      const unsigned blocks = row_blocks + unsigned((value_rows + 15) / 16);
+      attention_delta_kernel<T><<<blocks, 256, 0, s>>>(a, row_blocks);
       GS_TRY(check_launch("window_attention backward"));
     }
     if (key_items) {

@@ -412,3 +412,59 @@ def test_no_queries(dtype):
     _, dk, dv = window_attention_backward(q, k, v, out, lse, out, 4, 1)
     for t in (dk, dv):
         assert torch.isfinite(t).all() and not t.any()
+
+
+@pytest.mark.parametrize("values,size", [(100.0, 1.0), (1000.0, 1.0), (3000.0, 0.1), (300.0, 1e-3), (1e-3, 1e-3)])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("window", [1, 200])
+def test_float16_values_of_any_size(window, dim, values, size):
+    """Large and small values beside gradients of one sign.  dS carries a power of
+    two that brings B = 2 max|g| max|v| over the rows to 2^13 .. 2^15, so that it
+    loses up to max(1, B / 2^13) half subnormals."""
+    q, k, v = _inputs(1, 300, 300, 2, 1, dim, torch.float16)
+    v = (v.float() * values).half()
+    grad = (normal(q.shape, torch.float32, 9).abs() * size).half()
+    d = [t.to(DEV).requires_grad_(True) for t in (q, k, v)]
+    got = torch.autograd.grad(window_attention(*d, window, 2), d, grad.to(DEV))
+    want, bounds = _dense(q, k, v, window, 2, None, None, grad)
+    top = 2 * float(grad.double().norm(dim=-1).max() * v.double().norm(dim=-1).max())
+    lost = TINY[torch.float16] * max(1.0, top / 2**13) / math.sqrt(dim)
+    for name, x, y, b, t in zip(("dq", "dk", "dv"), got, want[1:], bounds[1:], (k, q, None)):
+        more = 0 if t is None else 300 * lost * float(t.double().abs().max()) * (1 if name == "dq" else 2)
+        assert_within(x, y, b + more, name)
+
+
+def test_float16_opposite_values():
+    """Two equal keys with values of +256 and -256 and gradients of one: dS is
+    16384, dk 16384 q / sqrt(128) and dq zero."""
+    q = normal((1, 2, 1, 128), torch.float16, 1)
+    k = normal((1, 1, 1, 128), torch.float16, 2).expand(1, 2, 1, 128).contiguous()
+    v = torch.full((1, 2, 1, 128), 256.0).half()
+    v[:, 1] = -256.0
+    grad = torch.zeros(q.shape).half()
+    grad[:, 1] = 1.0
+    d = [t.to(DEV).requires_grad_(True) for t in (q, k, v)]
+    dq, dk, dv = torch.autograd.grad(window_attention(*d, 2), d, grad.to(DEV))
+    want = 16384 / math.sqrt(128) * q[0, 1, 0].double()
+    u = UNIT[torch.float16]
+    assert_within(dk[0, 0, 0], want, 4 * u * want.abs(), "dk")
+    assert_within(dk[0, 1, 0], -want, 4 * u * want.abs(), "dk")
+    assert_within(dv[0, :, 0], torch.full((2, 128), 0.5), 2 * u, "dv")
+    # Two terms that cancel, each within the bound on dS.
+    assert_within(dq[0, 1, 0], torch.zeros(128), 8 * u * 16384 / math.sqrt(128) * k[0, 0, 0].double().abs(), "dq")
+
+
+def test_float16_sequences_apart():
+    """One sequence's large values and gradients take no bits of another's small
+    ones."""
+    q, k, v = _inputs(2, 300, 300, 2, 1, 64, torch.float16)
+    grad = normal(q.shape, torch.float16, 9)
+
+    def run(q, k, v, grad):
+        q, k, v, grad = (t.to(DEV) for t in (q, k, v, grad))
+        return window_attention_backward(q, k, v, *window_attention_forward(q, k, v, 200, 2), grad, 200, 2)
+
+    alone = run(q[:1], k[:1], v[:1], grad[:1])
+    v[1], grad[1] = v[1] * 4000, grad[1] * 4000
+    for a, b in zip(alone, run(q, k, v, grad)):
+        assert torch.equal(a[0], b[0])
