@@ -25,7 +25,9 @@
 // B = 2 max|grad_out_i| max|v_j| over the rows of a sequence that share a key
 // head; the power brings B to between 2^13 and 2^15, half of what the type holds,
 // so nothing overflows, and what is lost is below 2^-24 / 2^13 of B.  Each
-// sequence and key head has its own, so none takes bits of another.
+// sequence and key head has its own, so none takes bits of another.  P, grad_v's
+// operand and about one at most, carries 2^14 there: a window of a million keys leaves
+// probabilities of 2^-20, of which float16 keeps four bits.
 #include "attention_tile.h"
 
 namespace gs {
@@ -80,6 +82,10 @@ __device__ __forceinline__ int64_t part_index(const BackwardArgs& a, int b, int 
   const int64_t before = a.sink_segments > 1 ? int64_t(a.sink_blocks) * a.sink_segments : 0;
   return head + before + int64_t(block - a.sink_blocks) * a.segments + segment;
 }
+
+// The power of two that P carries as an operand.
+template <typename T>
+constexpr int kProbabilityShift = std::is_same_v<T, f16> ? 14 : 0;
 
 // The power of two that dS carries.
 template <typename T>
@@ -221,7 +227,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
   const int begin = int(walk * segment / pieces), count = int(walk * (segment + 1) / pieces);
 
   const int shift = gradient_shift<T>(a, b, kv);
-  const float up = ldexpf(1.0f, shift), down = ldexpf(1.0f, -shift);
+  // P comes out of the exponential with its power of two, and dS with P's.
+  const float up = ldexpf(1.0f, shift - kProbabilityShift<T>), down = ldexpf(1.0f, -shift);
   Acc dk[kBlocks], dv[kBlocks];
   Poison<T, kBlocks> pk, pv;
 #pragma unroll
@@ -239,7 +246,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
     if (threadIdx.x < kRows) {
       const int i = i0 + threadIdx.x;
       const int64_t at = (int64_t(b) * p.heads + head) * p.queries + i;
-      row_lse = i < p.queries ? a.lse[at] * kLog2e : 0.0f;
+      row_lse = i < p.queries ? a.lse[at] * kLog2e - float(kProbabilityShift<T>) : 0.0f;
       row_delta = i < p.queries ? a.delta[at] : 0.0f;
     }
   };
@@ -356,7 +363,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && kDim <= 64 ? 2 : 1) voi
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         x[r] = dk[n][4 * g + r] * down;
-        y[r] = dv[n][4 * g + r];
+        y[r] = dv[n][4 * g + r] * (1.0f / float(1 << kProbabilityShift<T>));
       }
       if (part) {
         *reinterpret_cast<FloatVec<4>*>(part_at + d) = x;

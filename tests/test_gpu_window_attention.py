@@ -468,3 +468,24 @@ def test_float16_sequences_apart():
     v[1], grad[1] = v[1] * 4000, grad[1] * 4000
     for a, b in zip(alone, run(q, k, v, grad)):
         assert torch.equal(a[0], b[0])
+
+
+def test_float16_long_uniform_window():
+    """Equal scores over a window of 1.6 million keys: probabilities of ten
+    subnormals of float16.  dv_j = sum_i g_i / n_i, within (2 u + 2 e + 2 N U) of
+    sum P |g|, N the 64 queries, and its own rounding."""
+    keys, queries = 1597830, 64
+    q = torch.zeros(1, queries, 1, 8).half()
+    k, v = normal((1, keys, 1, 8), torch.float16, 2), normal((1, keys, 1, 8), torch.float16, 3)
+    grad = normal(q.shape, torch.float16, 9, 500.0)
+    d = [t.to(DEV).requires_grad_(True) for t in (q, k, v)]
+    (dv,) = torch.autograd.grad(window_attention(*d, keys), d[2:], grad.to(DEV))
+    p = 1 / (keys - queries + 1 + torch.arange(queries, dtype=torch.float64))[:, None]
+    g = grad[0, :, 0].double()
+    want, size = (p * g).sum(0), (p * g.abs()).sum(0)
+    u = UNIT[torch.float16]
+    # The sums over the keys that lse holds are of equal terms; n U with n the keys
+    # bounds their chains, which are cut over lanes, waves and tiles of 32.
+    bound = (2 * u + 2 * (32 + keys / 256) * U32 + 2 * queries * U32) * size + u * want.abs() + TINY[torch.float16]
+    seen = dv[0, :keys - queries + 1, 0].cpu().double()
+    assert_within(seen, want.expand_as(seen), bound.expand_as(seen), "dv")
