@@ -226,7 +226,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : kDim <= 64 ? 4 : 2) 
     }
   if (lane < 32)
     a.lse[(int64_t(at.b) * p.heads + at.head) * p.queries + i] =
-        w.top == -INFINITY ? -INFINITY : (w.top + __builtin_amdgcn_logf(l)) / kLog2e;
+        w.top == -INFINITY && l == 0.0f ? -INFINITY : (w.top + __builtin_amdgcn_logf(l)) / kLog2e;
 }
 
 // 32 queries a workgroup: every wave has all of them and every fourth tile of 32
@@ -268,6 +268,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
   }
   w.poison.apply(w.o);
   // The waves join: the largest maximum, then the sums one wave after the other.
+  // No maximum and no sum: the query sees nothing.  NaN scores leave no maximum
+  // either, but a sum of NaN, which reaches the result.
   const float l = w.sum + __shfl_xor(w.sum, 32, 64);
   if (lane < 32) {
     tops[wave][lane] = w.top;
@@ -291,7 +293,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           float& sum = joined[col][32 * n + acc_row(r)];
-          const float v = w.top == -INFINITY ? 0.0f : w.o[n][r] * shrink;
+          const float v = w.o[n][r] * shrink;  // zero of a wave that saw nothing
           sum = k ? sum + v : v;
         }
     }
@@ -306,7 +308,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fw
   }
   if (threadIdx.x < 32 && i0 + col < p.queries)
     a.lse[(int64_t(at.b) * p.heads + at.head) * p.queries + i0 + col] =
-        top == -INFINITY ? -INFINITY : (top + __builtin_amdgcn_logf(whole)) / kLog2e;
+        top == -INFINITY && whole == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(whole)) / kLog2e;
 }
 
 template <typename T, int kDim>

@@ -489,3 +489,19 @@ def test_float16_long_uniform_window():
     bound = (2 * u + 2 * (32 + keys / 256) * U32 + 2 * queries * U32) * size + u * want.abs() + TINY[torch.float16]
     seen = dv[0, :keys - queries + 1, 0].cpu().double()
     assert_within(seen, want.expand_as(seen), bound.expand_as(seen), "dv")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("batch", [1, 40])
+def test_nan_scores_give_nan(dtype, batch):
+    """A query of NaN, and one that sees NaN keys alone, give NaN and a NaN lse,
+    few workgroups (one sequence) or many; every other query stays as it is."""
+    q, k, v = _inputs(batch, 300, 300, 4, 2, 64, dtype)
+    clean = window_attention_forward(q.to(DEV), k.to(DEV), v.to(DEV), 8)
+    q[0, 100], k[0, 200:208] = float("nan"), float("nan")
+    out, lse = window_attention_forward(q.to(DEV), k.to(DEV), v.to(DEV), 8)
+    assert torch.isnan(out[0, 100]).all() and torch.isnan(lse[0, :, 100]).all()
+    assert torch.isnan(out[0, 200:215]).all() and torch.isnan(lse[0, :, 200:215]).all()
+    rows = [i for i in range(300) if i != 100 and not 200 <= i < 215]
+    assert torch.equal(out[0, rows], clean[0][0, rows]) and torch.equal(out[1:], clean[0][1:])
+    assert torch.equal(lse[0][:, rows], clean[1][0][:, rows]) and torch.equal(lse[1:], clean[1][1:])
