@@ -45,13 +45,22 @@ def _check_sizes(window: int, sinks: int, heads: int, kv_heads: int) -> None:
         raise ValueError(f"{heads} heads cannot share {kv_heads} key heads")
 
 
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """Rows that start on 16-byte boundaries, neighbouring elements side by
-    side and tokens less than 2^24 elements apart; a copy where the strides do
-    not give that."""
+def _strides(t: torch.Tensor) -> list[int]:
+    """Strides of all dimensions but the last, 0 for one of a single element,
+    whose stride no address depends on and can be anything."""
+    return [s if n > 1 else 0 for n, s in zip(t.shape[:-1], t.stride())]
+
+
+def _on_16_bytes(t: torch.Tensor) -> bool:
+    """Rows start on 16-byte boundaries, neighbouring elements side by side."""
     unit = 16 // t.element_size()
-    if (t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % unit for s in t.stride()[:-1])
-            or t.stride(1) >= 1 << 24):
+    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(s % unit for s in _strides(t))
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """Rows on 16-byte boundaries and tokens less than 2^24 elements apart; a
+    copy where the strides do not give that."""
+    if not _on_16_bytes(t) or _strides(t)[1] >= 1 << 24:
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
@@ -91,7 +100,7 @@ def window_attention_forward(
     b, tq, h, _ = q.shape
     out = torch.empty(q.shape, dtype=q.dtype, device=device)
     lse = torch.empty((b, h, tq), dtype=torch.float32, device=device)
-    strides = _Strides[9](*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
+    strides = _Strides[9](*_strides(q), *_strides(k), *_strides(v))
     nat.check(
         nat.library().gs_window_attention_fwd(
             _byref(problem), q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, nat.ptr(lengths),
@@ -128,8 +137,7 @@ def window_attention_backward(
     lib = nat.library()
     ws_bytes = lib.gs_window_attention_bwd_workspace_bytes(_byref(problem))
     ws = nat.workspace(ws_bytes, device)
-    strides = _Strides[12](*q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
-                           *grad_out.stride()[:3])
+    strides = _Strides[12](*_strides(q), *_strides(k), *_strides(v), *_strides(grad_out))
     nat.check(
         lib.gs_window_attention_bwd(
             _byref(problem), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
@@ -201,10 +209,9 @@ def window_attention_step(
     if positions.shape != (b,):
         raise ValueError(f"positions {tuple(positions.shape)} does not fit a batch of {b}")
     device = nat.require_gpu(q, k, v, k_cache, v_cache, positions)
-    unit = 16 // q.element_size()
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
         # Written in place, so no aligned copy can stand in for them.
-        if t.stride(3) != 1 or t.data_ptr() % 16 or any(s % unit for s in t.stride()[:3]):
+        if not _on_16_bytes(t):
             raise ValueError(f"{name} must have its rows on 16-byte boundaries")
     problem = nat.GsAttention(b, 1, 0, window, sinks, h, hk, d, nat.TYPES[q.dtype], _scale(scale, d))
     q, k, v = nat.prepare(q, q.dtype), nat.prepare(k, q.dtype), nat.prepare(v, q.dtype)
@@ -213,7 +220,7 @@ def window_attention_step(
     lib = nat.library()
     ws_bytes = lib.gs_window_attention_step_workspace_bytes(_byref(problem))
     ws = nat.workspace(ws_bytes, device)
-    strides = _Strides[6](*k_cache.stride()[:3], *v_cache.stride()[:3])
+    strides = _Strides[6](*_strides(k_cache), *_strides(v_cache))
     nat.check(
         lib.gs_window_attention_step(
             _byref(problem), q.data_ptr(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(),

@@ -505,3 +505,23 @@ def test_nan_scores_give_nan(dtype, batch):
     rows = [i for i in range(300) if i != 100 and not 200 <= i < 215]
     assert torch.equal(out[0, rows], clean[0][0, rows]) and torch.equal(out[1:], clean[0][1:])
     assert torch.equal(lse[0][:, rows], clean[1][0][:, rows]) and torch.equal(lse[1:], clean[1][1:])
+
+
+def test_one_token_of_a_wide_row():
+    """Dimensions of one element, whose stride no address depends on: one token of
+    a fused projection of odd width, a cache of one stream."""
+    fused = normal((1, 1, 3 * 64 + 1), torch.bfloat16, 1).to(DEV)
+    q, k, v = fused[:, :, None, :192].split(64, -1)
+    assert q.stride(1) % 8 and q.is_contiguous()
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    out = window_attention(*leaves, 4, 1)
+    assert torch.equal(out, v)
+    _, _, dv = torch.autograd.grad(out, leaves, q)
+    assert torch.equal(dv, q)
+    far = [t.as_strided(t.shape, (t.stride(0), 1 << 25, 64, 1)) for t in leaves]
+    assert torch.equal(window_attention(*far, 4, 1), v)
+    caches = [torch.zeros(9 * 64 + 1, dtype=torch.bfloat16, device=DEV).as_strided((1, 9, 1, 64), (577, 64, 64, 1))
+              for _ in range(2)]
+    at = torch.zeros(1, dtype=torch.int32, device=DEV)
+    assert torch.equal(window_attention_step(q[0], k[0], v[0], *caches, at, 8, 1), v[0])
+    assert torch.equal(caches[0][:, 0], k[0]) and torch.equal(caches[1][:, 0], v[0])
