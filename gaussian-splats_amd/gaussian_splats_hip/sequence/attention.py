@@ -45,26 +45,29 @@ def _check_sizes(window: int, sinks: int, heads: int, kv_heads: int) -> None:
         raise ValueError(f"{heads} heads cannot share {kv_heads} key heads")
 
 
-def _strides(t: torch.Tensor) -> list[int]:
-    """Strides of all dimensions but the last, 0 for one of a single element,
+def _strides(t: torch.Tensor) -> tuple[int, int, int]:
+    """Strides of the first three dimensions, 0 for one of a single element,
     whose stride no address depends on and can be anything."""
-    return [s if n > 1 else 0 for n, s in zip(t.shape[:-1], t.stride())]
+    (a, b, c, _), (i, j, k, _) = t.stride(), t.shape
+    return a if i > 1 else 0, b if j > 1 else 0, c if k > 1 else 0
 
 
-def _on_16_bytes(t: torch.Tensor) -> bool:
+def _on_16_bytes(t: torch.Tensor, strides: tuple[int, int, int]) -> bool:
     """Rows start on 16-byte boundaries, neighbouring elements side by side."""
-    unit = 16 // t.element_size()
-    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(s % unit for s in _strides(t))
+    a, b, c = strides
+    return t.stride(3) == 1 and not ((a | b | c) * t.element_size() | t.data_ptr()) & 15
 
 
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """Rows on 16-byte boundaries and tokens less than 2^24 elements apart; a
-    copy where the strides do not give that."""
-    if not _on_16_bytes(t) or _strides(t)[1] >= 1 << 24:
+def _aligned(t: torch.Tensor) -> tuple[torch.Tensor, tuple[int, int, int]]:
+    """A tensor and its strides: rows on 16-byte boundaries and tokens less than
+    2^24 elements apart, a copy where the strides do not give that."""
+    strides = _strides(t)
+    if strides[1] >= 1 << 24 or not _on_16_bytes(t, strides):
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
-    return t
+        strides = _strides(t)
+    return t, strides
 
 
 def _problem(q, k, v, window, sinks, scale, lengths) -> nat.GsAttention:
@@ -95,12 +98,12 @@ def window_attention_forward(
     :func:`window_attention_backward` needs."""
     problem = _problem(q, k, v, window, sinks, scale, lengths)
     device = nat.require_gpu(q, k, v) if lengths is None else nat.require_gpu(q, k, v, lengths)
-    q, k, v = _aligned(q), _aligned(k), _aligned(v)
+    (q, sq), (k, sk), (v, sv) = _aligned(q), _aligned(k), _aligned(v)
     lengths = None if lengths is None else lengths.contiguous()
     b, tq, h, _ = q.shape
     out = torch.empty(q.shape, dtype=q.dtype, device=device)
     lse = torch.empty((b, h, tq), dtype=torch.float32, device=device)
-    strides = _Strides[9](*_strides(q), *_strides(k), *_strides(v))
+    strides = _Strides[9](*sq, *sk, *sv)
     nat.check(
         nat.library().gs_window_attention_fwd(
             _byref(problem), q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, nat.ptr(lengths),
@@ -129,7 +132,7 @@ def window_attention_backward(
         raise ValueError(f"out {tuple(out.shape)} {out.dtype} does not fit q")
     if lse.shape != (q.shape[0], q.shape[2], q.shape[1]) or lse.dtype != torch.float32:
         raise ValueError(f"lse {tuple(lse.shape)} {lse.dtype} does not fit q")
-    q, k, v, grad_out = _aligned(q), _aligned(k), _aligned(v), _aligned(grad_out)
+    (q, sq), (k, sk), (v, sv), (grad_out, sg) = _aligned(q), _aligned(k), _aligned(v), _aligned(grad_out)
     out, lse = nat.prepare(out, out.dtype), lse.contiguous()
     dq = torch.empty(q.shape, dtype=q.dtype, device=device)
     dk = torch.empty(k.shape, dtype=q.dtype, device=device)
@@ -137,7 +140,7 @@ def window_attention_backward(
     lib = nat.library()
     ws_bytes = lib.gs_window_attention_bwd_workspace_bytes(_byref(problem))
     ws = nat.workspace(ws_bytes, device)
-    strides = _Strides[12](*_strides(q), *_strides(k), *_strides(v), *_strides(grad_out))
+    strides = _Strides[12](*sq, *sk, *sv, *sg)
     nat.check(
         lib.gs_window_attention_bwd(
             _byref(problem), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
@@ -209,9 +212,10 @@ def window_attention_step(
     if positions.shape != (b,):
         raise ValueError(f"positions {tuple(positions.shape)} does not fit a batch of {b}")
     device = nat.require_gpu(q, k, v, k_cache, v_cache, positions)
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+    sk, sv = _strides(k_cache), _strides(v_cache)
+    for name, t, s in (("k_cache", k_cache, sk), ("v_cache", v_cache, sv)):
         # Written in place, so no aligned copy can stand in for them.
-        if not _on_16_bytes(t):
+        if not _on_16_bytes(t, s):
             raise ValueError(f"{name} must have its rows on 16-byte boundaries")
     problem = nat.GsAttention(b, 1, 0, window, sinks, h, hk, d, nat.TYPES[q.dtype], _scale(scale, d))
     q, k, v = nat.prepare(q, q.dtype), nat.prepare(k, q.dtype), nat.prepare(v, q.dtype)
@@ -220,7 +224,7 @@ def window_attention_step(
     lib = nat.library()
     ws_bytes = lib.gs_window_attention_step_workspace_bytes(_byref(problem))
     ws = nat.workspace(ws_bytes, device)
-    strides = _Strides[6](*_strides(k_cache), *_strides(v_cache))
+    strides = _Strides[6](*sk, *sv)
     nat.check(
         lib.gs_window_attention_step(
             _byref(problem), q.data_ptr(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(),
