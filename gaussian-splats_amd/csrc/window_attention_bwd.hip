@@ -638,7 +638,15 @@ void launch_queries(const BackwardArgs& a, hipStream_t s) {
 // CU, into segments of at least two tiles that make up for it, and the first
 // tokens' walks into as long ones.  Else the first tokens' alone, into segments a
 // quarter as long as the others' walks: most of their tiles are masked, and at the
-// others' length they end last (40000 tokens: 2.41 ms, 1.81 with a quarter).
+// others' length they end last (40000 tokens: 2.41 ms, 1.81 with a quarter).  The
+// first tokens' segments are about 1024 at most over all their blocks, four for
+// each CU, which bounds the parts to 128 MiB for heads of 128.  Backward in ms
+// with at most 512, 1024, 2048 and without a bound: 40000 tokens, 12 heads of 64 on
+// 4, window 64, 2500 first ones 2.51, 2.16, 1.63 and 3.36 (4.6 GiB of parts); 16
+// heads of 128, window 300, 1200 first ones 3.94, 3.73, 3.64 and 9.51 (12 GiB); 9600,
+// 8 heads of 64, window 1200, 1200 first ones 0.22, 0.25, 0.26 and 0.27.
+constexpr int64_t kSinkParts = 1024;
+
 void plan_segments(const Problem& p, int32_t type, BackwardArgs& a) {
   const int64_t blocks = key_blocks(p), rows = type == GS_F32 ? 32 : 64;
   const int64_t group = p.heads / p.kv_heads;
@@ -649,7 +657,9 @@ void plan_segments(const Problem& p, int32_t type, BackwardArgs& a) {
   a.sink_blocks = int(std::min<int64_t>(blocks, (p.sinks + kBlockKeys - 1) / kBlockKeys));
   const int64_t long_walk = (int64_t(p.queries) + rows - 1) / rows * group;
   const int64_t piece = a.segments > 1 ? walk / a.segments : std::max<int64_t>(1, walk / 4);
-  a.sink_segments = int(std::max<int64_t>(1, std::min<int64_t>(long_walk / piece, 4096)));
+  const int64_t sink_items = std::max<int64_t>(1, int64_t(a.sink_blocks) * p.kv_heads * p.batch);
+  a.sink_segments =
+      int(std::max<int64_t>(1, std::min<int64_t>(long_walk / piece, kSinkParts / sink_items)));
 }
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }

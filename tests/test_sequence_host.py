@@ -213,3 +213,16 @@ def test_first_tokens_workspace_is_bounded():
     delta = 12 * 40000 * 4
     parts = lib.gs_window_attention_bwd_workspace_bytes(ctypes.byref(d)) - delta
     assert 0 < parts <= 64 << 20
+
+
+@pytest.mark.parametrize("tokens,window,sinks,heads,kv_heads,dim", [
+    (40000, 64, 2500, 12, 4, 64), (40000, 300, 1200, 16, 16, 128), (40000, 16, 40000, 12, 4, 64),
+    (16320, 8160, 8160, 16, 4, 128), (160000, 300, 1200, 8, 8, 64)])
+def test_workspace_of_many_first_tokens_is_bounded(tokens, window, sinks, heads, kv_heads, dim):
+    """First tokens that are a whole view: parts for at most 1536 workgroups (1024
+    on the first tokens, 512 on the others), each two float32 tiles of 128 keys."""
+    lib = nat.library()
+    d = _attention(batch=1, queries=tokens, keys=tokens, window=window, sinks=sinks, heads=heads,
+                   kv_heads=kv_heads, head_dim=dim)
+    delta = heads * tokens * 4 + 4096
+    assert lib.gs_window_attention_bwd_workspace_bytes(ctypes.byref(d)) <= delta + 1536 * 2 * 128 * dim * 4
