@@ -115,44 +115,52 @@ __device__ __forceinline__ float square(const Frag<f16>& f) {
   }
   return sum;
 }
-// A row's square, of which 16 lanes hold a part each, into the largest one.  A
-// maximum does not depend on the order; most rows find a larger one there.
+// The rows' squares of a workgroup, of which 16 lanes hold a part each, into the
+// largest one.  A maximum does not depend on the order.
 __device__ __forceinline__ void note_size(uint32_t* largest, float part, bool counts) {
+  __shared__ float tops[4];
 #pragma unroll
   for (int s = 8; s > 0; s >>= 1) part += __shfl_xor(part, s, 64);
-  const uint32_t bits = __float_as_uint(part);
-  if (counts && (threadIdx.x & 15) == 0 &&
-      bits > __hip_atomic_load(largest, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
+  part = counts ? part : 0.0f;
+#pragma unroll
+  for (int s = 32; s > 8; s >>= 1) part = fmaxf(part, __shfl_xor(part, s, 64));
+  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = part;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  const uint32_t bits = __float_as_uint(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
+  // Most workgroups find a larger one there.
+  if (bits > __hip_atomic_load(largest, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
     atomicMax(largest, bits);
 }
 
-// delta, a group of 16 lanes for each row; float16: the sizes of grad_out's rows
-// and, in the workgroups from row_blocks on, those of v's.
+// delta, a workgroup for 16 queries of a head, 16 lanes each; float16: the sizes
+// of grad_out's rows and, in the workgroups from row_blocks on, those of v's.
 template <typename T>
 __global__ __launch_bounds__(256) void attention_delta_kernel(BackwardArgs a, unsigned row_blocks) {
   const Problem& p = a.p;
-  const int64_t rows = int64_t(p.batch) * p.queries * p.heads;
-  const int d = (threadIdx.x & 15) * 8;
+  const int d = (threadIdx.x & 15) * 8, row = threadIdx.x >> 4;
   if constexpr (std::is_same_v<T, f16>) {
     if (blockIdx.x >= row_blocks) {
-      const int64_t at = int64_t(blockIdx.x - row_blocks) * 16 + (threadIdx.x >> 4);
-      const bool in = at < int64_t(p.batch) * p.keys * p.kv_heads;
-      const int kv = in ? int(at % p.kv_heads) : 0;
-      const int64_t j = in ? at / p.kv_heads % p.keys : 0, b = in ? at / p.kv_heads / p.keys : 0;
-      const bool counts = in && j < p.length(int(b));
+      const unsigned at = blockIdx.x - row_blocks, blocks = unsigned(p.keys + 15) / 16;
+      const int kv = int(at % p.kv_heads), b = int(at / p.kv_heads / blocks);
+      const int j = int(at / p.kv_heads % blocks) * 16 + row;
+      const bool counts = j < p.length(b);
       const Frag<T> v = load_global<T>(static_cast<const T*>(a.v) + b * a.sv.batch +
                                            j * a.sv.token + kv * a.sv.head + d,
                                        counts && d < p.dim);
-      note_size(a.sizes + (b * p.kv_heads + kv) * 2 + 1, square(v), counts);
+      note_size(a.sizes + (int64_t(b) * p.kv_heads + kv) * 2 + 1, square(v), counts);
       return;
     }
   }
-  const int64_t row = int64_t(blockIdx.x) * 16 + (threadIdx.x >> 4);
+  const unsigned blocks = unsigned(p.queries + 15) / 16;
+  const int head = int(blockIdx.x % p.heads), b = int(blockIdx.x / p.heads / blocks);
+  const int i = int(blockIdx.x / p.heads % blocks) * 16 + row;
+  const int64_t at = (int64_t(b) * p.heads + head) * p.queries + i;
   float sum = 0.0f, size = 0.0f;
-  const int head = int(row % p.heads);
-  const int64_t i = row / p.heads % p.queries, b = row / p.heads / p.queries;
-  if (row < rows && d < p.dim) {
-    const Frag<T> o = load_global<T>(static_cast<const T*>(a.out) + row * p.dim + d, true);
+  if (i < p.queries && d < p.dim) {
+    const Frag<T> o = load_global<T>(static_cast<const T*>(a.out) +
+                                         ((int64_t(b) * p.queries + i) * p.heads + head) * p.dim + d,
+                                     true);
     const Frag<T> g = load_global<T>(static_cast<const T*>(a.grad) + b * a.sg.batch +
                                          i * a.sg.token + head * a.sg.head + d, true);
 #pragma unroll
@@ -161,13 +169,13 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(BackwardArgs a, un
   }
   if constexpr (std::is_same_v<T, f16>) {
     // A query that sees nothing has no dS.
-    const bool counts = row < rows && a.lse[(b * p.heads + head) * p.queries + i] != -INFINITY;
-    const int64_t kv = head / (p.heads / p.kv_heads);
-    note_size(a.sizes + (counts ? (b * p.kv_heads + kv) * 2 : 0), size, counts);
+    const bool counts = i < p.queries && a.lse[at] != -INFINITY;
+    const int kv = head / (p.heads / p.kv_heads);
+    note_size(a.sizes + (int64_t(b) * p.kv_heads + kv) * 2, size, counts);
   }
 #pragma unroll
   for (int s = 8; s > 0; s >>= 1) sum += __shfl_xor(sum, s, 64);
-  if (row < rows && (threadIdx.x & 15) == 0) a.delta[(b * p.heads + head) * p.queries + i] = sum;
+  if (i < p.queries && (threadIdx.x & 15) == 0) a.delta[at] = sum;
 }
 
 // grad_k and grad_v of a workgroup's keys: a wave holds 32, queries walk by.
@@ -737,7 +745,9 @@ extern "C" GS_API int gs_window_attention_bwd(const gs_attention* desc, const vo
   const Problem& p = a.p;
   const int64_t rows = int64_t(p.batch) * p.queries * p.heads;
   a.sizes = reinterpret_cast<uint32_t*>(a.delta + rows);
-  const int64_t value_rows = desc->type == GS_F16 ? int64_t(p.batch) * p.keys * p.kv_heads : 0;
+  const int64_t row_blocks = int64_t(p.batch) * p.heads * ((int64_t(p.queries) + 15) / 16);
+  const int64_t value_blocks =
+      desc->type == GS_F16 ? int64_t(p.batch) * p.kv_heads * ((int64_t(p.keys) + 15) / 16) : 0;
   const int64_t blocks = key_blocks(p), others = blocks - a.sink_blocks;
   const int64_t key_items = (int64_t(a.sink_blocks) * a.sink_segments + others * a.segments) *
                             p.kv_heads * p.batch;
@@ -745,7 +755,7 @@ extern "C" GS_API int gs_window_attention_bwd(const gs_attention* desc, const vo
   const int join_first = a.sink_segments > 1 ? 0 : a.sink_blocks;
   const int join_blocks = int((a.sink_segments > 1 ? a.sink_blocks : 0) + (a.segments > 1 ? others : 0));
   const int64_t joined = int64_t(p.batch) * p.kv_heads * join_blocks * kBlockKeys * p.dim / 4;
-  GS_REQUIRE((rows + value_rows) / 16 < (int64_t(1) << 30) && key_items < (int64_t(1) << 30) &&
+  GS_REQUIRE(row_blocks + value_blocks < (int64_t(1) << 30) && key_items < (int64_t(1) << 30) &&
                  joined / 256 < (int64_t(1) << 30),
              GS_ERR_OVERFLOW, "attention problem too large");
   const hipStream_t s = as_stream(stream);
@@ -757,9 +767,8 @@ extern "C" GS_API int gs_window_attention_bwd(const gs_attention* desc, const vo
       attention_clear_kernel<<<unsigned((words + 255) / 256), 256, 0, s>>>(a.sizes, words);
     }
     if (rows) {
-      const unsigned row_blocks = unsigned((rows + 15) / 16);
-      const unsigned blocks = row_blocks + unsigned((value_rows + 15) / 16);
-      attention_delta_kernel<T><<<blocks, 256, 0, s>>>(a, row_blocks);
+      attention_delta_kernel<T>
+          <<<unsigned(row_blocks + value_blocks), 256, 0, s>>>(a, unsigned(row_blocks));
       GS_TRY(check_launch("window_attention backward"));
     }
     if (key_items) {
