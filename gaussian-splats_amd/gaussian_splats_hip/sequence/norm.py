@@ -21,15 +21,19 @@ from ..kernels.rasterize import _native as nat
 _CODES = {"int8": (nat.TYPE_I8, torch.int8), "e4m3": (nat.TYPE_E4M3, torch.float8_e4m3fn)}
 
 
+def _check_rows(shape: torch.Size, dtype: torch.dtype, weight: torch.Tensor) -> None:
+    if dtype not in nat.TYPES:
+        raise TypeError(f"add_rms_norm expects float32, float16 or bfloat16, got {dtype}")
+    if len(shape) == 0 or shape[-1] == 0:
+        raise ValueError(f"add_rms_norm norms the last dimension, got shape {tuple(shape)}")
+    if weight.shape != shape[-1:]:
+        raise ValueError(f"weight {tuple(weight.shape)} does not fit rows of {shape[-1]}")
+    if weight.dtype != dtype and weight.dtype != torch.float32:
+        raise TypeError(f"weight is {weight.dtype}, expected {dtype} or torch.float32")
+
+
 def _check(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float) -> None:
-    if x.dtype not in nat.TYPES:
-        raise TypeError(f"add_rms_norm expects float32, float16 or bfloat16, got {x.dtype}")
-    if x.dim() == 0 or x.shape[-1] == 0:
-        raise ValueError(f"add_rms_norm norms the last dimension, got shape {tuple(x.shape)}")
-    if weight.shape != x.shape[-1:]:
-        raise ValueError(f"weight {tuple(weight.shape)} does not fit rows of {x.shape[-1]}")
-    if weight.dtype != x.dtype and weight.dtype != torch.float32:
-        raise TypeError(f"weight is {weight.dtype}, expected {x.dtype} or torch.float32")
+    _check_rows(x.shape, x.dtype, weight)
     if residual is not None:
         if residual.shape != x.shape:
             raise ValueError(f"x {tuple(x.shape)} and residual {tuple(residual.shape)} differ")
@@ -80,19 +84,23 @@ def add_rms_norm_backward(
 ) -> tuple[torch.Tensor | None, torch.Tensor | None, torch.Tensor | None]:
     """Backward kernels: gradients of x (of type ``dtype``), residual and
     weight.  The first two are one tensor where their types agree."""
-    device = nat.require_gpu(total, weight, inverse)
-    s2 = _rows(total)
-    weight = weight.contiguous()
-    rows, width = s2.shape
-    grads = []
+    _check_rows(total.shape, dtype, weight)
+    if total.dtype != dtype and total.dtype != torch.float32:
+        raise TypeError(f"total is {total.dtype}, expected {dtype} or torch.float32")
+    if inverse.dtype != torch.float32:
+        raise TypeError(f"inverse is {inverse.dtype}, expected torch.float32")
+    if inverse.dim() != 1 or inverse.shape[0] * total.shape[-1] != total.numel():
+        raise ValueError(f"inverse {tuple(inverse.shape)} is not that of the rows of {tuple(total.shape)}")
     for g, kind in ((grad_y, dtype), (grad_sum, total.dtype)):
-        if g is not None:
-            if g.shape != total.shape or g.dtype != kind:
-                raise ValueError(f"gradient {tuple(g.shape)} {g.dtype} does not fit "
-                                 f"{tuple(total.shape)} {kind}")
-            nat.require_gpu(total, g)
-            g = g.contiguous()
-        grads.append(g)
+        if g is not None and (g.shape != total.shape or g.dtype != kind):
+            raise ValueError(f"gradient {tuple(g.shape)} {g.dtype} does not fit "
+                             f"{tuple(total.shape)} {kind}")
+    given = [g for g in (grad_y, grad_sum) if g is not None]
+    device = nat.require_gpu(total, weight, inverse, *given)
+    s2 = _rows(total)
+    weight, inverse = weight.contiguous(), inverse.contiguous()
+    rows, width = s2.shape
+    grads = [None if g is None else g.contiguous() for g in (grad_y, grad_sum)]
     same = dtype == total.dtype
     grad_x = grad_residual = grad_weight = ws = None
     if need_x or (need_residual and same):

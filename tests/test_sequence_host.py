@@ -226,3 +226,27 @@ def test_workspace_of_many_first_tokens_is_bounded(tokens, window, sinks, heads,
                    kv_heads=kv_heads, head_dim=dim)
     delta = heads * tokens * 4 + 4096
     assert lib.gs_window_attention_bwd_workspace_bytes(ctypes.byref(d)) <= delta + 1536 * 2 * 128 * dim * 4
+
+
+def test_norm_backward_refuses():
+    """What the kernels would read beyond: a shorter weight or inverse, one of
+    another type."""
+    s, w, r = torch.zeros(2, 3, 8), torch.ones(8), torch.ones(6)
+    back = sequence.add_rms_norm_backward
+    with pytest.raises(ValueError, match="weight .* does not fit rows"):
+        back(s, w[:7], r, s, None, torch.float32)
+    with pytest.raises(TypeError, match="weight is torch.float16"):
+        back(s, w.half(), r, s, None, torch.float32)
+    with pytest.raises(TypeError, match="inverse is torch.bfloat16"):
+        back(s, w, r.bfloat16(), s, None, torch.float32)
+    for bad in (r[:5], r[:1], torch.ones(7), r.view(2, 3), torch.ones(())):
+        with pytest.raises(ValueError, match="inverse .* rows of"):
+            back(s, w, bad, s, None, torch.float32)
+    with pytest.raises(TypeError, match="total is torch.float16"):
+        back(s.half(), w.bfloat16(), r, s.bfloat16(), None, torch.bfloat16)
+    with pytest.raises(TypeError, match="float64"):
+        back(s, w, r, None, None, torch.float64)
+    with pytest.raises(ValueError, match="gradient"):
+        back(s, w, r, s[:1], None, torch.float32)
+    with pytest.raises(ValueError, match="ROCm GPU"):
+        back(s, w, r, s, None, torch.float32)
