@@ -80,23 +80,21 @@ def gated_scan_backward(
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
     """Backward kernels: gradients of x, gate and state; a gradient that is
     None counts as zeros."""
-    device = nat.require_gpu(x, gate, starts)
     _check(x, gate, None, 3, "gated_scan backward")
-    x, gate = _inner(x), _inner(gate)
     b, t, c = x.shape
     lib = nat.library()
+    if starts.dtype != torch.float32:
+        raise TypeError(f"starts is {starts.dtype}, expected torch.float32")
     if starts.shape != (b, lib.gs_gated_scan_chunks(t), c) or not starts.is_contiguous():
         raise ValueError(f"starts {tuple(starts.shape)} are not those of x {tuple(x.shape)}")
-    if grad_y is not None:
-        if grad_y.shape != x.shape or grad_y.dtype != x.dtype:
-            raise ValueError(f"grad_y {tuple(grad_y.shape)} {grad_y.dtype} does not fit x")
-        nat.require_gpu(x, grad_y)
-        grad_y = _inner(grad_y)
-    if grad_last is not None:
-        if grad_last.shape != (b, c) or grad_last.dtype != torch.float32:
-            raise ValueError(f"grad_last {tuple(grad_last.shape)} {grad_last.dtype} does not fit x")
-        nat.require_gpu(x, grad_last)
-        grad_last = grad_last.contiguous()
+    if grad_y is not None and (grad_y.shape != x.shape or grad_y.dtype != x.dtype):
+        raise ValueError(f"grad_y {tuple(grad_y.shape)} {grad_y.dtype} does not fit x")
+    if grad_last is not None and (grad_last.shape != (b, c) or grad_last.dtype != torch.float32):
+        raise ValueError(f"grad_last {tuple(grad_last.shape)} {grad_last.dtype} does not fit x")
+    device = nat.require_gpu(x, gate, starts, *(g for g in (grad_y, grad_last) if g is not None))
+    x, gate = _inner(x), _inner(gate)
+    grad_y = None if grad_y is None else _inner(grad_y)
+    grad_last = None if grad_last is None else grad_last.contiguous()
     grad_x = torch.empty((b, t, c), dtype=x.dtype, device=device)
     grad_gate = torch.empty((b, t, c), dtype=x.dtype, device=device)
     if t == 0:

@@ -250,3 +250,19 @@ def test_norm_backward_refuses():
         back(s, w, r, s[:1], None, torch.float32)
     with pytest.raises(ValueError, match="ROCm GPU"):
         back(s, w, r, s, None, torch.float32)
+
+
+def test_scan_backward_refuses():
+    x, starts = torch.zeros(2, 5, 8), torch.zeros(2, 1, 8)
+    back = sequence.gated_scan_backward
+    with pytest.raises(TypeError, match="starts is torch.bfloat16"):
+        back(x, x, starts.bfloat16(), x, None)
+    for bad in (starts[:1], starts[:, :, :7], torch.zeros(2, 2, 8), starts.expand(2, 1, 8)[:, :0]):
+        with pytest.raises(ValueError, match="starts .* are not those"):
+            back(x, x, bad, x, None)
+    with pytest.raises(ValueError, match="grad_y"):
+        back(x, x, starts, x[:1], None)
+    with pytest.raises(ValueError, match="grad_last"):
+        back(x, x, starts, x, torch.zeros(2, 8).half())
+    with pytest.raises(ValueError, match="ROCm GPU"):
+        back(x, x, starts, x, torch.zeros(2, 8))
