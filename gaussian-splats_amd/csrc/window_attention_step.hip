@@ -255,8 +255,10 @@ extern "C" GS_API int gs_window_attention_step(const gs_attention* desc, const v
   clear_error();
   GS_REQUIRE(desc, GS_ERR_INVALID_ARGUMENT, "null description");
   GS_TRY(check_attention(*desc));
-  GS_REQUIRE(desc->window < (int64_t(1) << 30) && desc->sinks < (int64_t(1) << 30),
-             GS_ERR_OVERFLOW, "cache too large");
+  // The kernel counts slots in 32 bits, up to a round of tiles beyond the last.
+  GS_REQUIRE(desc->window < (int64_t(1) << 30) && desc->sinks < (int64_t(1) << 30) - desc->window,
+             GS_ERR_OVERFLOW, "cache too large: %lld first tokens and a window of %lld",
+             (long long)desc->sinks, (long long)desc->window);
   if (desc->batch == 0) return GS_OK;
   const int64_t none[3] = {0, 0, 0};
   GS_REQUIRE(strides && positions, GS_ERR_INVALID_ARGUMENT, "null pointer");

@@ -762,7 +762,8 @@ GS_API int gs_window_attention_bwd(
  * memory) and attends from q [batch, heads, head_dim] to the slots that are
  * filled, its own among them; a stream at a negative position is left alone and
  * gets zeros.  strides: batch, token and head stride of k_cache and of v_cache;
- * q, k, v and out are contiguous. */
+ * q, k, v and out are contiguous; sinks + window is below 2^30 (GS_ERR_OVERFLOW
+ * otherwise). */
 GS_API size_t gs_window_attention_step_workspace_bytes(const gs_attention* attention);
 GS_API int gs_window_attention_step(
     const gs_attention* attention, const void* q, const void* k, const void* v,

@@ -266,3 +266,13 @@ def test_scan_backward_refuses():
         back(x, x, starts, x, torch.zeros(2, 8).half())
     with pytest.raises(ValueError, match="ROCm GPU"):
         back(x, x, starts, x, torch.zeros(2, 8))
+
+
+def test_step_refuses_caches_beyond_its_counters():
+    lib = nat.library()
+    strides = (ctypes.c_int64 * 6)(*[64] * 6)
+    for window, sinks in ((1 << 30, 0), ((1 << 30) - 1, 1), ((1 << 30) - 1, (1 << 30) - 1), (1, (1 << 63) - 1)):
+        d = _attention(window=window, sinks=sinks)
+        # Without positions: a call that the sizes do not turn away ends there.
+        assert lib.gs_window_attention_step(ctypes.byref(d), FAKE, FAKE, FAKE, FAKE, FAKE, strides, NULL, FAKE,
+                                            FAKE, 1 << 40, NULL) == nat.GS_ERR_OVERFLOW, (window, sinks)
