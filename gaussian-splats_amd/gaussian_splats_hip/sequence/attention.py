@@ -239,7 +239,8 @@ def window_attention_step(
 class WindowCache:
     """Keys and values of ``batch`` running streams for
     :func:`window_attention_step`: the first ``sinks`` tokens and a ring of the
-    last ``window`` ones, and each stream's next position."""
+    last ``window`` ones, and each stream's next position (negative: the stream
+    is not in use)."""
 
     def __init__(self, batch: int, kv_heads: int, dim: int, window: int, sinks: int = 0,
                  dtype: torch.dtype = torch.bfloat16, device: torch.device | str = "cuda"):
@@ -268,8 +269,9 @@ class WindowCache:
 
     def step(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
              scale: float | None = None) -> torch.Tensor:
-        """Attention of each stream's next token, which joins the cache."""
+        """Attention of each stream's next token, which joins the cache.  A stream
+        at a negative position stays there: zeros, and nothing joins."""
         out = window_attention_step(q, k, v, self.k, self.v, self.positions, self.window, self.sinks,
                                     scale)
-        self.positions.add_(1)
+        self.positions.add_(self.positions >= 0)
         return out

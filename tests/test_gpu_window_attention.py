@@ -525,3 +525,15 @@ def test_one_token_of_a_wide_row():
     at = torch.zeros(1, dtype=torch.int32, device=DEV)
     assert torch.equal(window_attention_step(q[0], k[0], v[0], *caches, at, 8, 1), v[0])
     assert torch.equal(caches[0][:, 0], k[0]) and torch.equal(caches[1][:, 0], v[0])
+
+
+def test_cache_leaves_inactive_streams_alone():
+    """A stream at a negative position stays there, step after step."""
+    cache = WindowCache(3, 1, 32, 8, 1, torch.float32, DEV)
+    cache.positions.copy_(torch.tensor([-1, 3, -5]))
+    q, k = torch.ones(3, 2, 32, device=DEV), torch.ones(3, 1, 32, device=DEV)
+    for t in range(2):
+        out = cache.step(q, k, k)
+        assert not out[0].any() and out[1].any() and not out[2].any()
+        assert cache.positions.tolist() == [-1, 4 + t, -5]
+    assert not cache.k[0].any() and not cache.k[2].any()
