@@ -45,6 +45,14 @@ def _check_sizes(window: int, sinks: int, heads: int, kv_heads: int) -> None:
         raise ValueError(f"{heads} heads cannot share {kv_heads} key heads")
 
 
+def _check_lengths(lengths: torch.Tensor | None, batch: int) -> None:
+    if lengths is not None:
+        if lengths.dtype != torch.int32:
+            raise TypeError(f"lengths is {lengths.dtype}, expected torch.int32")
+        if lengths.shape != (batch,):
+            raise ValueError(f"lengths {tuple(lengths.shape)} does not fit a batch of {batch}")
+
+
 def _strides(t: torch.Tensor) -> tuple[int, int, int]:
     """Strides of the first three dimensions, 0 for one of a single element,
     whose stride no address depends on and can be anything."""
@@ -80,11 +88,7 @@ def _problem(q, k, v, window, sinks, scale, lengths) -> nat.GsAttention:
     if k.shape[0] != b or k.shape[3] != d:
         raise ValueError(f"k {tuple(k.shape)} does not fit q {tuple(q.shape)}")
     _check_sizes(window, sinks, h, k.shape[2])
-    if lengths is not None:
-        if lengths.dtype != torch.int32:
-            raise TypeError(f"lengths is {lengths.dtype}, expected torch.int32")
-        if lengths.shape != (b,):
-            raise ValueError(f"lengths {tuple(lengths.shape)} does not fit a batch of {b}")
+    _check_lengths(lengths, b)
     return nat.GsAttention(b, tq, k.shape[1], window, sinks, h, k.shape[2], d, nat.TYPES[q.dtype],
                            _scale(scale, d))
 
@@ -252,13 +256,29 @@ class WindowCache:
         self.positions = torch.zeros(batch, dtype=torch.int32, device=device)
 
     @torch.no_grad()
-    def fill(self, k: torch.Tensor, v: torch.Tensor) -> None:
+    def fill(self, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor | None = None) -> None:
         """Starts every stream over with the tokens k, v [batch, tokens,
-        kv_heads, dim] of a prefill; only those that stay visible are kept."""
+        kv_heads, dim] of a prefill; only those that stay visible are kept.  Of
+        sequences that end early only the first ``lengths[batch]`` (int32; None:
+        all) are taken, and each stream goes on behind its own."""
         if k.shape != v.shape or k.dim() != 4 or k.shape[::2] != self.k.shape[::2] or k.shape[3] != self.k.shape[3]:
             raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not fit the cache "
                              f"{tuple(self.k.shape)}")
+        _check_lengths(lengths, k.shape[0])
         tokens = k.shape[1]
+        if lengths is not None:
+            lengths = lengths.clamp(0, tokens)
+            # The token of each slot: a first token's slot its own, the ring's slot s
+            # the last one of s, s + window, ..
+            slot = torch.arange(self.sinks + self.window, device=self.k.device)
+            behind = lengths[:, None] - 1 - slot
+            ring = slot + behind.div(self.window, rounding_mode="floor") * self.window
+            stream, at = (behind >= 0).nonzero(as_tuple=True)
+            token = torch.where(slot < self.sinks, slot, ring)[stream, at]
+            for cache, t in ((self.k, k), (self.v, v)):
+                cache[stream, at] = t[stream, token].to(cache.dtype)
+            self.positions.copy_(lengths)
+            return
         first = min(self.sinks, tokens)
         ring = torch.arange(max(first, tokens - self.window), tokens, device=self.k.device)
         slots = self.sinks + (ring - self.sinks) % self.window

@@ -537,3 +537,37 @@ def test_cache_leaves_inactive_streams_alone():
         assert not out[0].any() and out[1].any() and not out[2].any()
         assert cache.positions.tolist() == [-1, 4 + t, -5]
     assert not cache.k[0].any() and not cache.k[2].any()
+
+
+@pytest.mark.parametrize("tokens", [5, 31, 100, 131])
+def test_stream_continues_sequences_of_different_lengths(tokens):
+    """A prefill whose sequences end early, kept with their lengths, and steps
+    after it give the rows of attention over each whole sequence."""
+    window, sinks, dtype, steps = 28, 3, torch.bfloat16, 9
+    lengths = torch.tensor([tokens, tokens // 2, 2, 0], dtype=torch.int32)
+    q, k, v = _inputs(4, tokens + steps, tokens + steps, 4, 2, 64, dtype)
+    cache = WindowCache(4, 2, 64, window, sinks, dtype, DEV)
+    pk, pv = k[:, :tokens].clone(), v[:, :tokens].clone()
+    for i, n in enumerate(lengths.tolist()):
+        pk[i, n:], pv[i, n:] = float("nan"), float("nan")  # padding
+    cache.fill(pk.to(DEV), pv.to(DEV), lengths.to(DEV))
+    assert torch.equal(cache.positions.cpu(), lengths)
+    for t in range(steps):
+        at = lengths.long() + t
+        each = torch.arange(4)
+        out = cache.step(*(x[each, at].to(DEV) for x in (q, k, v)))
+        for i, p in enumerate(at.tolist()):
+            values, bounds = _dense(q[i:i + 1, :p + 1], k[i:i + 1, :p + 1], v[i:i + 1, :p + 1], window, sinks,
+                                    None, None, torch.zeros_like(q[i:i + 1, :p + 1]))
+            assert_within(out[i], values[0][0, p], bounds[0][0, p], f"sequence {i}, token {p}")
+
+
+def test_fill_refuses():
+    cache = WindowCache(2, 1, 32, 8, 1, torch.float32, DEV)
+    k = torch.ones(2, 4, 1, 32, device=DEV)
+    with pytest.raises(TypeError, match="lengths is"):
+        cache.fill(k, k, torch.zeros(2, dtype=torch.int64, device=DEV))
+    with pytest.raises(ValueError, match="batch of 2"):
+        cache.fill(k, k, torch.zeros(3, dtype=torch.int32, device=DEV))
+    with pytest.raises(ValueError, match="do not fit"):
+        cache.fill(k[:, :, :, :16], k[:, :, :, :16])
