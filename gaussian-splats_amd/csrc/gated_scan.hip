@@ -193,7 +193,9 @@ __device__ __forceinline__ int64_t end_row(const ScanArgs& a, int64_t b, int64_t
 // State before an item's chunk for the channels of one wave's lanes: the nearest
 // published one and the maps after it.  These are published by workgroups that
 // hold earlier tickets, so every wait ends; the spin limit turns a broken
-// invariant into an error flag.  `init` is the state before place 0.
+// invariant into an error flag and a state of NaN, as no call waits for the flag:
+// an output that misses what was waited for is NaN, never a wrong number (seen with
+// a limit of 0).  `init` is the state before place 0.
 template <bool kBackward, int kChannels>
 __device__ FloatVec<kChannels> look_back(const ScanArgs& a, int64_t b, int64_t place, int64_t c,
                                          FloatVec<kChannels> init) {
@@ -245,7 +247,7 @@ __device__ FloatVec<kChannels> look_back(const ScanArgs& a, int64_t b, int64_t p
     if (taken == 0) {
       if (++spins > kSpinLimit) {
         if ((threadIdx.x & 63) == 0) atomicOr(a.flags, kDeviceFlagScan);
-        return h;
+        return FloatVec<kChannels>(NAN);
       }
       __builtin_amdgcn_s_sleep(1);
     }

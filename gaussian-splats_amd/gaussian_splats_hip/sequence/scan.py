@@ -9,6 +9,10 @@ the recurrence by which front-to-back compositing accumulates colour.  h is
 float32 whatever the types; a state carries it from one call to the next, and
 ``gated_scan_step`` takes one token of a running stream.  A gate of -inf forgets
 what came before, one of +inf keeps it whole.
+
+Long scans wait for one another's chunks on the GPU.  A wait that hits its limit
+(none should) leaves NaN in what needs its state and a bit in the GPU's word of
+failed checks, which the next rasterizer call that synchronises raises.
 """
 
 from __future__ import annotations

@@ -690,7 +690,8 @@ GS_API int gs_add_rms_norm_bwd(
  * grad_y's after them).  gs_gated_scan_bwd writes the gradients of x, gate
  * and, unless NULL, state; grad_y NULL and grad_last NULL stand for zeros.
  * The results do not depend on the schedule.  With no token nothing is
- * written. */
+ * written.  Should a wait between workgroups ever hit its spin limit, the
+ * outputs that miss what it waited for are NaN, and GS_DEVICE_SCAN_LIMIT is set. */
 GS_API int64_t gs_gated_scan_chunks(int64_t tokens);
 GS_API size_t gs_gated_scan_workspace_bytes(
     int64_t batch, int64_t tokens, int64_t channels, int32_t backward);

@@ -243,3 +243,17 @@ def test_empty():
     assert y.shape == x.shape and torch.equal(last, state) and torch.equal(g, torch.ones_like(g))
     y, last = gated_scan(torch.zeros(0, 4, 5, device=DEV), torch.zeros(0, 4, 5, device=DEV))
     assert y.shape == (0, 4, 5) and last.shape == (0, 5)
+
+
+def test_waits_end_by_themselves():
+    """Long scans leave no bit of a failed wait behind."""
+    from gaussian_splats_hip.kernels.rasterize import _native as nat
+
+    nat.device_errors(DEV)
+    shape = (2, 40000, 512)
+    x, gate = (normal(shape, torch.bfloat16, i, s, m).to(DEV) for i, s, m in ((1, 1.0, 0.0), (2, 2.0, 3.0)))
+    y, last, starts = gated_scan_forward(x, gate)
+    grads = gated_scan_backward(x, gate, starts, x, last)
+    for t in (y, last, *grads):
+        assert torch.isfinite(t).all()
+    assert nat.device_errors(DEV) == 0
