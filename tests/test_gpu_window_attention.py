@@ -571,3 +571,26 @@ def test_fill_refuses():
         cache.fill(k, k, torch.zeros(3, dtype=torch.int32, device=DEV))
     with pytest.raises(ValueError, match="do not fit"):
         cache.fill(k[:, :, :, :16], k[:, :, :, :16])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_weights_add_up_to_one(dtype):
+    """Values that are the same for every key come back as they are, although
+    seven of eight probabilities round down by four tenths of a spacing: the sum
+    takes the rounded ones."""
+    b, h, d, n = 4, 16, 64, 600
+    spacing = UNIT[dtype]  # of the type from 0.5 to 1
+    scale = -math.log(0.5 + 0.4 * spacing)
+    q, k = torch.zeros(b, n, h, d).to(dtype), torch.zeros(b, n, h, d).to(dtype)
+    q[..., 0], k[..., 0] = 1, -1
+    k[:, ::8] = 0
+    value = 2 - 2 * spacing  # the largest below 2
+    v = torch.full((b, n, h, d), value).to(dtype)
+    assert float(v[0, 0, 0, 0]) == value
+    q, k, v = q.to(DEV), k.to(DEV), v.to(DEV)
+    for batch in (1, b):  # few workgroups and many
+        out, _ = window_attention_forward(q[:batch], k[:batch], v[:batch], n, 0, scale)
+        assert bool((out == value).all())
+    at = torch.full((b,), n - 1, dtype=torch.int32, device=DEV)
+    out = window_attention_step(q[:, -1], k[:, -1], v[:, -1], k.clone(), v.clone(), at, n, 0, scale)
+    assert bool((out == value).all())
