@@ -4,8 +4,8 @@
 //   G_t = grad_y_t + R_t,  R_{t-1} = a_t G_t,  R_T = grad_last,
 //   grad_x = (1 - a) G,  grad_gate = G (h_{t-1} - x) a (1 - a),  grad_state = R_0.
 // A step of either is the affine map h -> A h + B, and a run of steps composes
-// to one such map, so the tokens are cut into chunks of 128 that workgroups hold
-// in registers, a wave a run of tokens.  Each workgroup publishes its chunk's
+// to one such map, so the tokens are cut into chunks (240 forward, 120 backward)
+// that workgroups hold in registers, a wave a run of tokens.  Each workgroup publishes its chunk's
 // map, looks back for the nearest chunk whose end state is known, takes the maps
 // in between from there in order, publishes its own end state and runs its
 // tokens: every tensor is read and written once.  A chunk's state comes from the
@@ -18,11 +18,13 @@
 // A lane holds two neighbouring channels of a 16-bit type where rows allow
 // 4-byte accesses.
 //
-// Bound by memory in principle.  Measured, bfloat16, [1, 160000, 768]: forward 191
-// us for 0.74 GB (3.9 TB/s, where a large copy moves 5.2), backward 311 us for 1.23
-// GB (4.0 TB/s): a workgroup fills a CU, and its items' loads run ahead by one item,
+// Bound by memory in principle.  Measured, bfloat16, [1, 160000, 768]: forward 193
+// us for 0.74 GB (3.8 TB/s, where a large copy moves 5.2), backward 304-317 us for
+// 1.23 GB (3.9-4.0 TB/s): a workgroup fills a CU, and its items' loads run ahead by one item,
 // but what a look back waits for is not all hidden.  Three kernels that read the
-// inputs twice (maps, walk, run) took 375 and 500 us.
+// inputs twice (maps, walk, run) took 375 and 500 us.  [2, 8160, 1024]: 37 and 46 us
+// for 19 and 32 of bytes: 544 items forward on 256 workgroups, of which 32 take a
+// third one while the others wait.
 #include "sequence.h"
 
 namespace gs {
@@ -617,7 +619,10 @@ int64_t chunks_of(int64_t tokens) {
 }
 int64_t starts_of(int64_t tokens) { return (tokens + kStartTokens - 1) / kStartTokens; }
 
-// Two channels a lane where every row of every tensor allows 4-byte accesses.
+// Two channels a lane where every row of every tensor allows 4-byte accesses.  us
+// forward and backward with two and with one, bfloat16: [1, 160000, 768] 193 and 304,
+// 223 and 420; [2, 8160, 1024] 37 and 46, 39 and 57; [1, 2000, 256], of few workgroups,
+// 15.5 and 16.4, 14.4 and 14.8.
 bool pairs(const ScanArgs& a, int32_t type) {
   if (type == GS_F32 || a.channels % 2) return false;
   const int64_t strides = a.x_batch | a.x_token | a.gate_batch | a.gate_token | a.grad_batch |

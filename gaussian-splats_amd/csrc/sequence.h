@@ -73,12 +73,6 @@ __device__ __forceinline__ void store_from_float(void* p, int64_t i, int type, f
     static_cast<bf16*>(p)[i] = bf16(v);
 }
 
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
-
 // The larger one; NaN if either is NaN.
 __device__ __forceinline__ float max_nan(float a, float b) {
   return a != a ? a : (b != b ? b : fmaxf(a, b));

@@ -11,23 +11,26 @@
 // share keys are walked one after the other by their keys' workgroup.
 //
 // The first tokens are seen by every later query.  Their keys' walk, far longer
-// than a window, is cut into segments of about the others' length, each a
-// workgroup of its own that leaves float32 sums, which a last kernel adds in the
-// order of the segments.  Where there are few keys the other walks are cut too.
-// Measured, bfloat16, 40000 tokens, 12 heads of 64 on 4, window 5000: keys 1.57 ms
-// (730 TFLOP/s, two waves a SIMD, 212 registers), queries 1.01 ms (850 TFLOP/s,
+// than a window, is cut into segments, each a workgroup of its own that leaves
+// float32 sums, which a last kernel adds in the order of the segments.  Where there are few keys the other walks are cut too.
+// Measured, bfloat16, 40000 tokens, 12 heads of 64 on 4, window 5000: keys 1.51 ms
+// (760 TFLOP/s, two waves a SIMD, 232 registers), queries 0.98 ms (880 TFLOP/s,
 // three waves); bound as the forward is.  64 keys a wave: 2.57 ms, one wave a SIMD.
 //
-// dS is an operand of products in the inputs' type.  float16 would lose small
-// values of it below its normal range and large ones above it, as gradients and
-// values come in any size (and P is about one over the window): there dS carries
-// a power of two, taken out of the sums in float32.  |dP - delta| is at most
-// B = 2 max|grad_out_i| max|v_j| over the rows of a sequence that share a key
-// head; the power brings B to between 2^13 and 2^15, half of what the type holds,
-// so nothing overflows, and what is lost is below 2^-24 / 2^13 of B.  Each
+// P and dS are operands of products in the inputs' type, delta reads the rounded
+// out, and outputs are rounded once: relative to 64 bits the gradients are off by
+// 0.0025 in bfloat16 and 0.0003 in float16, where a single rounding leaves 0.0017 and
+// 0.0002.  Products with each rounding's rest would cost twice.
+//
+// float16 would lose small values of dS below its normal range and large ones
+// above it, as gradients and values come in any size (and P is about one over the
+// window): there dS carries a power of two, taken out of the sums in float32.
+// |dP - delta| is at most B = 2 max|grad_out_i| max|v_j| over the rows of a sequence
+// that share a key head; the power brings B to between 2^13 and 2^15, half of what
+// the type holds, so nothing overflows, and what is lost is below 2^-38 of B.  Each
 // sequence and key head has its own, so none takes bits of another.  P, grad_v's
-// operand and about one at most, carries 2^14 there: a window of a million keys leaves
-// probabilities of 2^-20, of which float16 keeps four bits.
+// operand and about one at most, carries 2^14 there: a window of a million keys
+// leaves probabilities of 2^-20, of which float16 itself keeps four bits.
 #include "attention_tile.h"
 
 namespace gs {
@@ -644,7 +647,11 @@ void launch_queries(const BackwardArgs& a, hipStream_t s) {
 
 // How the walks are cut.  Where the blocks of keys are fewer than two for each
 // CU, into segments of at least two tiles that make up for it, and the first
-// tokens' walks into as long ones.  Else the first tokens' alone, into segments a
+// tokens' walks into as long ones.  Backward in us, uncut and cut for 256, 512 and
+// 1024 workgroups: 4096 tokens, 8 heads of 64 on 2, window 1024 187, 138, 101 and 111;
+// 2 x 777, 6 heads of 40 on 2, float32 189, 80, 77 and 77; 1200, 8 heads of 64, window
+// 300 47, 42, 42 and 42; 2 x 2500, 8 heads of 128, window 1250 (320 blocks) 212, 212,
+// 212 and 231.  Else the first tokens' alone, into segments a
 // quarter as long as the others' walks: most of their tiles are masked, and at the
 // others' length they end last (40000 tokens: 2.41 ms, 1.81 with a quarter).  The
 // first tokens' segments are about 1024 at most over all their blocks, four for
