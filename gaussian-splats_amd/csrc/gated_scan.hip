@@ -302,7 +302,7 @@ __device__ __forceinline__ void await(uint32_t* counter, uint32_t count) {
 // waited for by later ones, and whoever holds the earliest unfinished one works
 // on it.
 __device__ __forceinline__ uint32_t next_ticket(const ScanArgs& a, uint32_t turn) {
-  return a.ticket ? atomicAdd(a.ticket, 1u) : turn ? a.items : blockIdx.x;
+  return a.ticket ? atomicAdd(a.ticket, 1u) : turn ? a.items : uint32_t(block_index());
 }
 
 // The looking wave: finds the state before each item's chunk, publishes the one
@@ -587,7 +587,7 @@ template <typename T, int kChannels>
 __global__ __launch_bounds__(256) void scan_step_kernel(const T* x, const T* gate,
                                                         const float* state, int64_t groups,
                                                         T* y, float* state_out) {
-  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t i = block_index() * 256 + threadIdx.x;
   if (i >= groups) return;
   const FloatVec<kChannels> xs = to_float<T, kChannels>(load_channels<T, kChannels>(x + i * kChannels));
   const FloatVec<kChannels> gs = to_float<T, kChannels>(load_channels<T, kChannels>(gate + i * kChannels));
@@ -690,9 +690,9 @@ int run_scan(ScanArgs& a, int32_t type, char* workspace, hipStream_t s) {
     using T = decltype(v);
     constexpr int kN = decltype(n)::value;
     if constexpr (kBackward)
-      scan_bwd_kernel<T, kN><<<unsigned(blocks), kThreads, 0, s>>>(a);
+      scan_bwd_kernel<T, kN><<<grid_of(blocks), kThreads, 0, s>>>(a);
     else
-      scan_fwd_kernel<T, kN><<<unsigned(blocks), kThreads, 0, s>>>(a);
+      scan_fwd_kernel<T, kN><<<grid_of(blocks), kThreads, 0, s>>>(a);
     return check_launch("gated_scan");
   });
 }
@@ -796,7 +796,7 @@ extern "C" GS_API int gs_gated_scan_step(const void* x, const void* gate, const 
                      constexpr int kN = decltype(k)::value;
                      const int64_t groups = n / kN;
                      scan_step_kernel<T, kN>
-                         <<<unsigned((groups + 255) / 256), 256, 0, as_stream(stream)>>>(
+                         <<<grid_of((groups + 255) / 256), 256, 0, as_stream(stream)>>>(
                              static_cast<const T*>(x), static_cast<const T*>(gate), state, groups,
                              static_cast<T*>(y), state_out);
                      return check_launch("gated_scan_step");

@@ -183,7 +183,7 @@ template <typename TX, typename TR, typename R>
 __global__ __launch_bounds__(kThreads) void norm_kernel(NormArgs a) {
   __shared__ float scratch[2][kWaves];
   const int t = threadIdx.x % R::kThreadsPerRow;
-  const int64_t row = int64_t(blockIdx.x) * R::kRows + threadIdx.x / R::kThreadsPerRow;
+  const int64_t row = block_index() * R::kRows + threadIdx.x / R::kThreadsPerRow;
   if (row >= a.rows) return;  // whole waves; workgroups of one row have no such row
   FloatVec<8> s[R::kCount], w[R::kCount];
   load_row<R>(static_cast<const TX*>(a.x) + row * a.x_stride, a.width, t, s);
@@ -225,7 +225,8 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(NormArgs a) {
 template <typename TX, typename TR>
 __global__ __launch_bounds__(kThreads) void norm_long_kernel(NormArgs a) {
   __shared__ float scratch[2][kWaves];
-  const int64_t row = blockIdx.x;
+  const int64_t row = block_index();
+  if (row >= a.rows) return;
   const TX* x = static_cast<const TX*>(a.x) + row * a.x_stride;
   const TR* res = static_cast<const TR*>(a.residual);
   if (res) res += row * a.residual_stride;
@@ -380,7 +381,7 @@ __global__ __launch_bounds__(kSumWaves* kWave) void norm_weight_kernel(
     const float* __restrict__ partials, int count, int width, void* grad_w, int type) {
   __shared__ float parts[kSumWaves][kWave];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int c = blockIdx.x * kWave + lane;
+  const int64_t c = block_index() * kWave + lane;
   float sum = 0.0f;
   if (c < width) {
 #pragma unroll 8
@@ -461,11 +462,11 @@ int run_norm(NormArgs a, int32_t x_type, int32_t r_type, void* stream) {
         a.width, vec,
         [&](auto row) {
           using R = decltype(row);
-          const unsigned blocks = unsigned((a.rows + R::kRows - 1) / R::kRows);
+          const dim3 blocks = grid_of((a.rows + R::kRows - 1) / R::kRows);
           norm_kernel<TX, TR, R><<<blocks, kThreads, 0, as_stream(stream)>>>(a);
         },
         [&] {
-          norm_long_kernel<TX, TR><<<unsigned(a.rows), kThreads, 0, as_stream(stream)>>>(a);
+          norm_long_kernel<TX, TR><<<grid_of(a.rows), kThreads, 0, as_stream(stream)>>>(a);
         });
     return check_launch("add_rms_norm");
   });
@@ -552,7 +553,7 @@ extern "C" GS_API int gs_add_rms_norm_bwd(const void* sum, const void* weight,
     }));
   }
   if (grad_weight) {
-    norm_weight_kernel<<<unsigned((width + kWave - 1) / kWave), kSumWaves * kWave, 0,
+    norm_weight_kernel<<<grid_of((width + kWave - 1) / kWave), kSumWaves * kWave, 0,
                          as_stream(stream)>>>(a.partials, blocks, a.width, grad_weight, weight_type);
     return check_launch("add_rms_norm weight gradient");
   }

@@ -78,6 +78,20 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return a != a ? a : (b != b ? b : fmaxf(a, b));
 }
 
+// `blocks` workgroups of up to 1024 threads.  One dimension holds less than 2^32
+// threads: beyond, a launch is refused or, worse, does the remainder alone.  So
+// many workgroups go over two dimensions, and block_index() counts them; up to a
+// few more than `blocks` are launched.
+inline dim3 grid_of(int64_t blocks) {
+  constexpr int64_t kMost = 1 << 21;
+  if (blocks <= kMost) return dim3(unsigned(blocks));
+  const int64_t y = (blocks + kMost - 1) / kMost;
+  return dim3(unsigned((blocks + y - 1) / y), unsigned(y));
+}
+__device__ __forceinline__ int64_t block_index() {
+  return int64_t(blockIdx.y) * gridDim.x + blockIdx.x;
+}
+
 inline bool aligned_to(const void* p, size_t bytes) {
   return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0;
 }

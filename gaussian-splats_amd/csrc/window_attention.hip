@@ -316,7 +316,6 @@ int launch_forward(const ForwardArgs& a, hipStream_t s) {
   const auto items = [&](int queries) {
     return (int64_t(a.p.queries) + queries - 1) / queries * a.p.heads * a.p.batch;
   };
-  GS_REQUIRE(items(32) < (int64_t(1) << 30), GS_ERR_OVERFLOW, "attention problem too large");
   if (items(32 * kWaves) < split_below(a.p.dim))
     attention_fwd_split_kernel<T, kDim><<<unsigned(xcd_grid(items(32))), kThreads, 0, s>>>(a);
   else
@@ -343,6 +342,11 @@ int check_attention(const gs_attention& d) {
              "type must be GS_F32, GS_F16 or GS_BF16");
   GS_REQUIRE(d.keys < (int64_t(1) << 30) && d.queries < (int64_t(1) << 30) && d.batch < 65536 &&
                  d.heads < 65536,
+             GS_ERR_OVERFLOW, "attention problem too large");
+  // Workgroups of 256 threads: a launch holds less than 2^32.
+  const int64_t most = (int64_t(1) << 24) - 8;
+  GS_REQUIRE((d.queries + 127) / 128 * d.heads * d.batch < most &&
+                 (d.keys + 127) / 128 * d.kv_heads * d.batch < most,
              GS_ERR_OVERFLOW, "attention problem too large");
   return GS_OK;
 }

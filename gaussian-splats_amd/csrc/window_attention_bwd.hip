@@ -142,9 +142,11 @@ template <typename T>
 __global__ __launch_bounds__(256) void attention_delta_kernel(BackwardArgs a, unsigned row_blocks) {
   const Problem& p = a.p;
   const int d = (threadIdx.x & 15) * 8, row = threadIdx.x >> 4;
+  const unsigned index = unsigned(block_index());
   if constexpr (std::is_same_v<T, f16>) {
-    if (blockIdx.x >= row_blocks) {
-      const unsigned at = blockIdx.x - row_blocks, blocks = unsigned(p.keys + 15) / 16;
+    if (index >= row_blocks) {
+      const unsigned at = index - row_blocks, blocks = unsigned(p.keys + 15) / 16;
+      if (at >= unsigned(p.batch) * p.kv_heads * blocks) return;
       const int kv = int(at % p.kv_heads), b = int(at / p.kv_heads / blocks);
       const int j = int(at / p.kv_heads % blocks) * 16 + row;
       const bool counts = j < p.length(b);
@@ -155,9 +157,10 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(BackwardArgs a, un
       return;
     }
   }
+  if (index >= row_blocks) return;
   const unsigned blocks = unsigned(p.queries + 15) / 16;
-  const int head = int(blockIdx.x % p.heads), b = int(blockIdx.x / p.heads / blocks);
-  const int i = int(blockIdx.x / p.heads % blocks) * 16 + row;
+  const int head = int(index % p.heads), b = int(index / p.heads / blocks);
+  const int i = int(index / p.heads % blocks) * 16 + row;
   const int64_t at = (int64_t(b) * p.heads + head) * p.queries + i;
   float sum = 0.0f, size = 0.0f;
   if (i < p.queries && d < p.dim) {
@@ -762,9 +765,6 @@ extern "C" GS_API int gs_window_attention_bwd(const gs_attention* desc, const vo
   const int join_first = a.sink_segments > 1 ? 0 : a.sink_blocks;
   const int join_blocks = int((a.sink_segments > 1 ? a.sink_blocks : 0) + (a.segments > 1 ? others : 0));
   const int64_t joined = int64_t(p.batch) * p.kv_heads * join_blocks * kBlockKeys * p.dim / 4;
-  GS_REQUIRE(row_blocks + value_blocks < (int64_t(1) << 30) && key_items < (int64_t(1) << 30) &&
-                 joined / 256 < (int64_t(1) << 30),
-             GS_ERR_OVERFLOW, "attention problem too large");
   const hipStream_t s = as_stream(stream);
   return seq::with_type(desc->type, [&](auto t) {
     using T = decltype(t);
@@ -775,7 +775,7 @@ extern "C" GS_API int gs_window_attention_bwd(const gs_attention* desc, const vo
     }
     if (rows) {
       attention_delta_kernel<T>
-          <<<unsigned(row_blocks + value_blocks), 256, 0, s>>>(a, unsigned(row_blocks));
+          <<<grid_of(row_blocks + value_blocks), 256, 0, s>>>(a, unsigned(row_blocks));
       GS_TRY(check_launch("window_attention backward"));
     }
     if (key_items) {

@@ -720,7 +720,9 @@ GS_API int gs_gated_scan_step(
  * all keys).  A query that sees no key gets zeros; values at places that a query
  * does not see, infinities and NaN among them, do not reach it.  head_dim is a
  * multiple of 8 up to 128; window > 0 (at or above keys: none), sinks >= 0,
- * scale > 0.  type is that of all tensors. */
+ * scale > 0.  type is that of all tensors.  batch * heads * ceil(queries / 128)
+ * and batch * kv_heads * ceil(keys / 128) are below 2^24 - 8 (GS_ERR_OVERFLOW
+ * otherwise). */
 typedef struct gs_attention {
   int64_t batch;
   int64_t queries;

@@ -25,7 +25,12 @@ import torch
 
 from gaussian_splats_hip.sequence import (
     add_rms_norm,
+    add_rms_norm_backward,
+    add_rms_norm_quant,
     gated_scan,
+    gated_scan_backward,
+    gated_scan_forward,
+    gated_scan_step,
     window_attention,
     window_attention_backward,
     window_attention_forward,
@@ -303,3 +308,67 @@ def test_norm_backward_over_several_rows_a_workgroup(rows, width, dtype):
         assert_within(z, ds, own + ds.abs() * u + tiny, name)
     bound = (dy.double().abs() * unit).sum(0) * (2 * u + (rows + chain + 15) * U32) + dw.abs() * u
     assert_within(got[2], dw, bound + tiny, "grad weight")
+
+
+def test_norm_of_more_threads_than_one_dimension_holds():
+    """2^26 rows and more, a wave each: 2^32 threads."""
+    rows = (1 << 26) + 5
+    x = normal((4096, 8), torch.bfloat16, 1).to(DEV).repeat(rows // 4096 + 1, 1)[:rows]
+    w = normal((8,), torch.bfloat16, 2, 0.2, 1.0).to(DEV)
+    y, _ = add_rms_norm(x, None, w)
+    codes, scales, _ = add_rms_norm_quant(x, None, w)
+    want = add_rms_norm(x[:4096], None, w)[0]
+    few, few_scales, _ = add_rms_norm_quant(x[:4096], None, w)
+    assert torch.equal(y[:rows - 5].view(-1, 4096, 8), want.expand(rows // 4096, -1, -1))
+    assert torch.equal(codes[:rows - 5].view(-1, 4096, 8), few.expand(rows // 4096, -1, -1))
+    assert torch.equal(y[rows - 5:], want[:5]) and torch.equal(codes[rows - 5:], few[:5])
+    assert torch.equal(scales[:rows - 5].view(-1, 4096), few_scales.expand(rows // 4096, -1))
+
+
+def test_weight_gradient_of_a_very_long_row():
+    """2^28 elements: 2^32 threads add the weight's gradient up."""
+    width = (1 << 28) + 70
+    x = normal((1, 4096), torch.bfloat16, 1).to(DEV).repeat(1, width // 4096 + 1)[:, :width].contiguous()
+    w, inverse = torch.ones(width, dtype=torch.bfloat16, device=DEV), torch.ones(1, device=DEV)
+    _, _, dw = add_rms_norm_backward(x, w, inverse, x, None, torch.bfloat16, False, False)
+    assert torch.equal(dw, (x[0].float() * x[0].float()).to(torch.bfloat16))
+
+
+def test_scan_of_more_threads_than_one_dimension_holds():
+    """One token of 65535 sequences of 16400 channels: 8.4 million workgroups.  One
+    step of a running stream of 2^32 channels in all."""
+    b, c = 65535, 16400
+    x = normal((1, 1, c), torch.bfloat16, 1).to(DEV).expand(b, 1, c)
+    gate = normal((1, 1, c), torch.bfloat16, 2).to(DEV).expand(b, 1, c)
+    y, last, starts = gated_scan_forward(x, gate)
+    few = gated_scan_forward(x[:2], gate[:2])
+    assert torch.equal(y, few[0][:1].expand(b, -1, -1)) and torch.equal(last, few[1][:1].expand(b, -1))
+    del y, last
+    dx, dg, _ = gated_scan_backward(x, gate, starts, x, None, need_state=False)
+    one = gated_scan_backward(x[:2], gate[:2], few[2], x[:2], None)
+    assert torch.equal(dx, one[0][:1].expand(b, -1, -1)) and torch.equal(dg, one[1][:1].expand(b, -1, -1))
+    del dx, dg, starts
+    b, c = 1 << 15, (1 << 17) + 8
+    x = normal((1, c), torch.float32, 1).to(DEV).repeat(b, 1)
+    state = x.clone()
+    y, _ = gated_scan_step(x, x, state, state_out=state)
+    few, _ = gated_scan_step(x[:1], x[:1], x[:1])
+    assert torch.equal(y, few.expand(b, -1)) and torch.equal(state, few.expand(b, -1))
+
+
+def test_attention_backward_of_many_rows():
+    """2^28 rows: delta takes 2^32 threads."""
+    b, t, h = (1 << 10) + 1, 1 << 14, 16
+    q, k, v, grad = (x.expand(b, -1, -1, -1) for x in _inputs(1, t, t, h, 1, 8, torch.float16))
+    few = [x[:2] for x in (q, k, v, grad)]
+    out, lse = window_attention_forward(q, k, v, 3, 1)
+    got = window_attention_backward(q, k, v, out, lse, grad, 3, 1)
+    out2, lse2 = window_attention_forward(*few[:3], 3, 1)
+    want = window_attention_backward(*few[:3], out2, lse2, few[3], 3, 1)
+    assert torch.equal(out, out2[:1].expand(b, -1, -1, -1)) and torch.equal(lse, lse2[:1].expand(b, -1, -1))
+    assert torch.equal(got[0], want[0][:1].expand(b, -1, -1, -1))
+    # Keys' walks are cut otherwise in the small call: sums in another order.
+    for x, y in zip(got[1:], want[1:]):
+        assert torch.equal(x, x[:1].expand(b, -1, -1, -1))
+        u = UNIT[torch.float16]
+        assert bool(((x[0] - y[0]).float().abs() <= 2 * u * y[0].float().abs() + 64 * u * y.float().abs().mean()).all())

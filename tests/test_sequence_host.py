@@ -276,3 +276,14 @@ def test_step_refuses_caches_beyond_its_counters():
         # Without positions: a call that the sizes do not turn away ends there.
         assert lib.gs_window_attention_step(ctypes.byref(d), FAKE, FAKE, FAKE, FAKE, FAKE, strides, NULL, FAKE,
                                             FAKE, 1 << 40, NULL) == nat.GS_ERR_OVERFLOW, (window, sinks)
+
+
+def test_attention_refuses_more_workgroups_than_a_launch_holds():
+    """2^24 workgroups of 256 threads; without buffers, so that a call that the
+    sizes do not turn away ends at its pointers."""
+    lib = nat.library()
+    strides = (ctypes.c_int64 * 12)(*[64] * 12)
+    d = ctypes.byref(_attention(batch=65535, queries=1024, keys=1024, heads=64, kv_heads=1, window=2, sinks=0))
+    assert lib.gs_window_attention_fwd(d, NULL, NULL, NULL, strides, NULL, NULL, NULL, NULL) == nat.GS_ERR_OVERFLOW
+    assert lib.gs_window_attention_bwd(d, NULL, NULL, NULL, NULL, NULL, NULL, strides, NULL, NULL, NULL, NULL, NULL,
+                                       1 << 50, NULL) == nat.GS_ERR_OVERFLOW
