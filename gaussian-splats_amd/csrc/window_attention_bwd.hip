@@ -149,7 +149,8 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(BackwardArgs a, un
       if (at >= unsigned(p.batch) * p.kv_heads * blocks) return;
       const int kv = int(at % p.kv_heads), b = int(at / p.kv_heads / blocks);
       const int j = int(at / p.kv_heads % blocks) * 16 + row;
-      const bool counts = j < p.length(b);
+      // Keys that some query sees.
+      const bool counts = j < p.length(b) && (j > p.offset() - p.window || j < p.sinks);
       const Frag<T> v = load_global<T>(static_cast<const T*>(a.v) + b * a.sv.batch +
                                            j * a.sv.token + kv * a.sv.head + d,
                                        counts && d < p.dim);

@@ -594,3 +594,32 @@ def test_weights_add_up_to_one(dtype):
     at = torch.full((b,), n - 1, dtype=torch.int32, device=DEV)
     out = window_attention_step(q[:, -1], k[:, -1], v[:, -1], k.clone(), v.clone(), at, n, 0, scale)
     assert bool((out == value).all())
+
+
+def test_float16_unseen_values_take_no_bits():
+    """Large values that no query sees (before every window, behind the length),
+    and gradients of queries that see nothing, leave the gradients' bits."""
+    q, k, v = _inputs(2, 300, 600, 4, 2, 64, torch.float16)
+    grad = normal(q.shape, torch.float16, 9)
+    lengths = torch.tensor([600, 320], dtype=torch.int32)
+
+    def run(v, grad):
+        args = [t.to(DEV) for t in (q, k, v)]
+        out, lse = window_attention_forward(*args, 50, 3, None, lengths.to(DEV))
+        return window_attention_backward(*args, out, lse, grad.to(DEV), 50, 3, None, lengths.to(DEV))
+
+    def bare(v, grad):
+        args = [t.to(DEV) for t in (q[1:], k[1:], v[1:])]
+        n = lengths[1:].to(DEV)
+        out, lse = window_attention_forward(*args, 50, 0, None, n)
+        return window_attention_backward(*args, out, lse, grad[1:].to(DEV), 50, 0, None, n)
+
+    base, alone = run(v, grad), bare(v, grad)
+    loud, louder = v.clone(), grad.clone()
+    loud[:, 3:251] = 60000
+    loud[1, 320:] = -60000
+    louder[1, 69:] = 60000  # positions from 369 on, which see no key without first ones
+    for x, y in zip(base, run(loud, grad)):
+        assert torch.equal(x, y)
+    for x, y in zip(alone, bare(loud, louder)):
+        assert torch.equal(x, y)
