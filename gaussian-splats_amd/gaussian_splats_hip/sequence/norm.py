@@ -89,7 +89,7 @@ def add_rms_norm_backward(
         raise TypeError(f"total is {total.dtype}, expected {dtype} or torch.float32")
     if inverse.dtype != torch.float32:
         raise TypeError(f"inverse is {inverse.dtype}, expected torch.float32")
-    if inverse.dim() != 1 or inverse.shape[0] * total.shape[-1] != total.numel():
+    if inverse.numel() * total.shape[-1] != total.numel():
         raise ValueError(f"inverse {tuple(inverse.shape)} is not that of the rows of {tuple(total.shape)}")
     for g, kind in ((grad_y, dtype), (grad_sum, total.dtype)):
         if g is not None and (g.shape != total.shape or g.dtype != kind):
