@@ -215,6 +215,9 @@ def window_attention_step(
         raise TypeError(f"positions is {positions.dtype}, expected torch.int32")
     if positions.shape != (b,):
         raise ValueError(f"positions {tuple(positions.shape)} does not fit a batch of {b}")
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if 0 in t.stride() and any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+            raise ValueError(f"{name} is expanded: its streams or slots share memory that the step writes")
     device = nat.require_gpu(q, k, v, k_cache, v_cache, positions)
     sk, sv = _strides(k_cache), _strides(v_cache)
     for name, t, s in (("k_cache", k_cache, sk), ("v_cache", v_cache, sv)):

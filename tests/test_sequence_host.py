@@ -288,3 +288,17 @@ def test_attention_refuses_more_workgroups_than_a_launch_holds():
     assert lib.gs_window_attention_fwd(d, NULL, NULL, NULL, strides, NULL, NULL, NULL, NULL) == nat.GS_ERR_OVERFLOW
     assert lib.gs_window_attention_bwd(d, NULL, NULL, NULL, NULL, NULL, NULL, strides, NULL, NULL, NULL, NULL, NULL,
                                        1 << 50, NULL) == nat.GS_ERR_OVERFLOW
+
+
+def test_step_refuses_expanded_caches():
+    """Streams that share their memory would write to it at once."""
+    q, k = torch.zeros(2, 4, 16), torch.zeros(2, 2, 16)
+    cache, at = torch.zeros(2, 9, 2, 16), torch.zeros(2, dtype=torch.int32)
+    for bad in (cache[:1].expand(2, -1, -1, -1), cache[:, :1].expand(-1, 9, -1, -1), cache[:, :, :1].expand(-1, -1, 2, -1)):
+        with pytest.raises(ValueError, match="k_cache is expanded"):
+            sequence.window_attention_step(q, k, k, bad, cache, at, 8, 1)
+        with pytest.raises(ValueError, match="v_cache is expanded"):
+            sequence.window_attention_step(q, k, k, cache, bad, at, 8, 1)
+    one = cache[:1].expand(1, -1, -1, -1).as_strided((1, 9, 2, 16), (0, 32, 16, 1))
+    with pytest.raises(ValueError, match="ROCm GPU"):
+        sequence.window_attention_step(q[:1], k[:1], k[:1], one, one, at[:1], 8, 1)
