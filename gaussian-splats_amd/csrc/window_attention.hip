@@ -18,7 +18,7 @@
 // exponentials' path) for about 45 %, LDS serves for 40 %: what is left is the
 // latency from one to the other, which four waves a SIMD hide in part.  64
 // queries a wave would halve the LDS reads but leave two waves a SIMD: 0.90 ms.
-// float16, 2 x 8160 tokens, 16 heads of 128: 0.34 ms, 670 TFLOP/s at two waves.
+// float16, 2 x 8160 tokens, 16 heads of 128: 0.33 ms, 700 TFLOP/s at two waves.
 #include "attention_tile.h"
 
 namespace gs {
