@@ -2,6 +2,7 @@
 // launch: the update torch.optim.Adam applies (its multi-tensor path, the
 // default on GPUs) to the Gaussian parameters in the reference's training step
 // (training/train.py:115, eps = 1e-15; step at train.py:151):
+//   g  <- g * factor                               (gs_adam_step_scaled)
 //   g  <- g + weight_decay * p                     (if weight_decay != 0)
 //   m  <- lerp(m, g, 1 - beta1)
 //   v  <- v * beta2 + (1 - beta2) * g * g
@@ -10,7 +11,8 @@
 // computed on the host in double precision per tensor, as torch does in
 // Python.  Each element is read once (p, g, m, v) and written once (p, m, v):
 // 28 bytes per parameter instead of the eight full passes of the op-by-op
-// update.
+// update.  The factor of a clipped gradient norm is read from device memory and
+// applied here: the gradients are not written back, which would move 8 bytes more.
 #include <algorithm>
 #include <cmath>
 
@@ -40,6 +42,7 @@ struct AdamArgs {
   AdamTensorArg t[kAdamMaxTensors];
   int count;
   float one_minus_beta1, beta2, one_minus_beta2, eps, weight_decay;
+  const float* factor;  // of the gradients, or null
 };
 
 __device__ __forceinline__ float lerp_small(float a, float b, float w) {
@@ -58,7 +61,9 @@ __device__ __forceinline__ void adam_element(const AdamArgs& a, const AdamTensor
   p = p + t.step_size * (m / denom);
 }
 
+template <bool kScaled>
 __global__ __launch_bounds__(kAdamThreads) void adam_kernel(AdamArgs a) {
+  const float factor = kScaled ? *a.factor : 1.0f;
   int k = 0;
   while (k + 1 < a.count && int64_t(blockIdx.x) >= a.t[k + 1].first_block) ++k;
   const AdamTensorArg& t = a.t[k];
@@ -73,7 +78,8 @@ __global__ __launch_bounds__(kAdamThreads) void adam_kernel(AdamArgs a) {
     for (int64_t i = base + int64_t(threadIdx.x) * 4; i < vend; i += kAdamThreads * 4) {
       const int64_t q = i >> 2;
       float4 p = p4[q], m = m4[q], v = v4[q];
-      const float4 g = g4[q];
+      float4 g = g4[q];
+      if (kScaled) g = make_float4(g.x * factor, g.y * factor, g.z * factor, g.w * factor);
       adam_element(a, t, p.x, g.x, m.x, v.x);
       adam_element(a, t, p.y, g.y, m.y, v.y);
       adam_element(a, t, p.z, g.z, m.z, v.z);
@@ -83,22 +89,17 @@ __global__ __launch_bounds__(kAdamThreads) void adam_kernel(AdamArgs a) {
       v4[q] = v;
     }
     for (int64_t i = vend + threadIdx.x; i < end; i += kAdamThreads)
-      adam_element(a, t, t.p[i], t.g[i], t.m[i], t.v[i]);
+      adam_element(a, t, t.p[i], kScaled ? t.g[i] * factor : t.g[i], t.m[i], t.v[i]);
   } else {
     for (int64_t i = base + threadIdx.x; i < end; i += kAdamThreads)
-      adam_element(a, t, t.p[i], t.g[i], t.m[i], t.v[i]);
+      adam_element(a, t, t.p[i], kScaled ? t.g[i] * factor : t.g[i], t.m[i], t.v[i]);
   }
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-}  // namespace
-}  // namespace gs
-
-using namespace gs;
-
-extern "C" GS_API int gs_adam_step(const gs_adam_tensor* tensors, int32_t count, double beta1,
-                                   double beta2, double eps, double weight_decay, void* stream) {
+int adam_step(const gs_adam_tensor* tensors, int32_t count, double beta1, double beta2, double eps,
+              double weight_decay, const float* factor, void* stream) {
   clear_error();
   GS_REQUIRE(count >= 0 && count <= kAdamMaxTensors, GS_ERR_INVALID_ARGUMENT,
              "between 0 and %d tensors per step (got %d)", kAdamMaxTensors, count);
@@ -106,6 +107,7 @@ extern "C" GS_API int gs_adam_step(const gs_adam_tensor* tensors, int32_t count,
   GS_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0,
              GS_ERR_INVALID_ARGUMENT, "betas must lie in [0, 1)");
   AdamArgs a{};
+  a.factor = factor;
   // Scalars reach the device as float, as torch's foreach ops convert them.
   a.one_minus_beta1 = float(1.0 - beta1);
   a.beta2 = float(beta2);
@@ -140,6 +142,28 @@ extern "C" GS_API int gs_adam_step(const gs_adam_tensor* tensors, int32_t count,
   a.count = used;
   if (used == 0) return GS_OK;
   GS_REQUIRE(blocks < (int64_t(1) << 31), GS_ERR_OVERFLOW, "too many parameters");
-  adam_kernel<<<unsigned(blocks), kAdamThreads, 0, as_stream(stream)>>>(a);
+  const hipStream_t on = as_stream(stream);
+  if (factor)
+    adam_kernel<true><<<unsigned(blocks), kAdamThreads, 0, on>>>(a);
+  else
+    adam_kernel<false><<<unsigned(blocks), kAdamThreads, 0, on>>>(a);
   return check_launch("adam_step");
+}
+
+}  // namespace
+}  // namespace gs
+
+using namespace gs;
+
+extern "C" GS_API int gs_adam_step(const gs_adam_tensor* tensors, int32_t count, double beta1,
+                                   double beta2, double eps, double weight_decay, void* stream) {
+  return adam_step(tensors, count, beta1, beta2, eps, weight_decay, nullptr, stream);
+}
+
+extern "C" GS_API int gs_adam_step_scaled(const gs_adam_tensor* tensors, int32_t count,
+                                          double beta1, double beta2, double eps,
+                                          double weight_decay, const float* factor, void* stream) {
+  clear_error();
+  GS_REQUIRE(factor, GS_ERR_INVALID_ARGUMENT, "null pointer: factor");
+  return adam_step(tensors, count, beta1, beta2, eps, weight_decay, factor, stream);
 }

@@ -7,6 +7,7 @@ tensors that do not live on a ROCm GPU.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import threading
 from ctypes import c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
@@ -15,7 +16,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parents[2] / "_lib" / "libgs_raster.so"
-ABI_VERSION = 22
+ABI_VERSION = 23
 
 GS_OK = 0
 GS_ERR_INVALID_ARGUMENT = 1
@@ -368,6 +369,14 @@ _SIGNATURES = {
         c_int, [c_void_p, c_int32, ctypes.c_double, ctypes.c_double, ctypes.c_double,
                 ctypes.c_double, c_void_p]
     ),
+    "gs_adam_step_scaled": (
+        c_int, [c_void_p, c_int32, ctypes.c_double, ctypes.c_double, ctypes.c_double,
+                ctypes.c_double, c_void_p, c_void_p]
+    ),
+    "gs_grad_norm_workspace_bytes": (c_size_t, [c_int64]),
+    "gs_grad_norm": (
+        c_int, [c_void_p, c_int64, ctypes.c_double, c_int32] + [c_void_p] * 3 + [c_size_t, c_void_p]
+    ),
     "gs_ssim_workspace_bytes": (c_size_t, [c_int32, c_int32]),
     "gs_ssim_fwd": (
         c_int, [c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_size_t, c_void_p]
@@ -502,6 +511,15 @@ def stream(device: torch.device) -> c_void_p:
     times a call)."""
     index = device.index if device.index is not None else torch.cuda.current_device()
     return c_void_p(torch._C._cuda_getCurrentRawStream(index))
+
+
+_here = contextlib.nullcontext()
+
+
+def on(device: torch.device):
+    """Makes ``device`` the current one for a launch: torch's default stream has
+    the same handle on every device, and a launch on it goes to the current one."""
+    return _here if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def require_gpu(*tensors: torch.Tensor) -> torch.device:

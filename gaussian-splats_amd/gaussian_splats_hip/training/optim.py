@@ -7,6 +7,11 @@ reference's relocation, training/utils.py:186-205 -- keeps working) whose
 with ``gs_adam_step``: each element is read and written once.  Supported:
 float32 GPU parameters, per-group ``lr``/``betas``/``eps``/``weight_decay``;
 ``amsgrad``, ``maximize`` and sparse gradients are not.
+
+With ``max_norm`` a step clips the 2-norm of all gradients together, as
+:func:`~gaussian_splats_hip.training.clip_grad_norm` before it would, but applies
+the factor inside the update: the gradients themselves stay as they are, and
+``grad_norm`` holds the norm (a float32 tensor, no host synchronisation).
 """
 
 from __future__ import annotations
@@ -16,6 +21,7 @@ import ctypes
 import torch
 
 from ..kernels.rasterize import _native as nat
+from .clip import check_max_norm, norm_of
 
 
 def check_adam_tensors(p: torch.Tensor, grad: torch.Tensor, exp_avg: torch.Tensor,
@@ -39,12 +45,20 @@ def check_adam_tensors(p: torch.Tensor, grad: torch.Tensor, exp_avg: torch.Tenso
 
 
 class FusedAdam(torch.optim.Adam):
+    max_norm: float | None = None
+    #: Norm of the gradients of the last step with ``max_norm``, before clipping.
+    grad_norm: torch.Tensor | None = None
+
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0,
-                 amsgrad=False, *, maximize=False):
+                 amsgrad=False, *, maximize=False, max_norm=None):
         if amsgrad or maximize:
             raise NotImplementedError("FusedAdam implements plain Adam (no amsgrad, no maximize)")
         super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
                          foreach=False)
+        self.max_norm = None if max_norm is None else check_max_norm(max_norm)
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "max_norm": self.max_norm}
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -93,15 +107,23 @@ class FusedAdam(torch.optim.Adam):
                     state["exp_avg_sq"].data_ptr(), p.numel(), float(group["lr"]),
                     int(state["step"].item()),
                 ))
+        factor = None
+        if self.max_norm is not None and keep_alive:
+            # A gradient that two parameters share counts once.
+            grads = {g.data_ptr(): g for g in keep_alive[1::4]}
+            self.grad_norm, factor = norm_of(list(grads.values()), self.max_norm)
         lib = nat.library()
         for (beta1, beta2, eps, weight_decay), entries in batches.items():
             for i in range(0, len(entries), nat.ADAM_MAX_TENSORS):
                 chunk = entries[i:i + nat.ADAM_MAX_TENSORS]
                 array = (nat.GsAdamTensor * len(chunk))(*chunk)
-                nat.check(
-                    lib.gs_adam_step(ctypes.cast(array, ctypes.c_void_p), len(chunk), beta1, beta2,
-                                     eps, weight_decay, nat.stream(device)),
-                    "adam_step",
-                )
-        del keep_alive  # the launches are enqueued; the stream orders any reuse
+                array = ctypes.cast(array, ctypes.c_void_p)
+                if factor is None:
+                    status = lib.gs_adam_step(array, len(chunk), beta1, beta2, eps, weight_decay,
+                                              nat.stream(device))
+                else:
+                    status = lib.gs_adam_step_scaled(array, len(chunk), beta1, beta2, eps,
+                                                     weight_decay, nat.ptr(factor), nat.stream(device))
+                nat.check(status, "adam_step")
+        del keep_alive, factor  # the launches are enqueued; the stream orders any reuse
         return loss

@@ -42,7 +42,7 @@ extern "C" {
 
 #define GS_API __attribute__((visibility("default")))
 
-#define GS_ABI_VERSION 22
+#define GS_ABI_VERSION 23
 
 typedef enum gs_status {
   GS_OK = 0,
@@ -604,6 +604,29 @@ typedef struct gs_adam_tensor {
 GS_API int gs_adam_step(
     const gs_adam_tensor* tensors, int32_t count, double beta1, double beta2,
     double eps, double weight_decay, void* stream);
+
+/* The same with every gradient multiplied by *factor (device memory, such as
+ * gs_grad_norm writes) before the weight decay joins it; the gradients stay. */
+GS_API int gs_adam_step_scaled(
+    const gs_adam_tensor* tensors, int32_t count, double beta1, double beta2,
+    double eps, double weight_decay, const float* factor, void* stream);
+
+/* The 2-norm of all elements of `count` tensors (contiguous, of a gs_type up to
+ * GS_BF16; the list is host memory) and factor = min(1, max_norm / (norm +
+ * 1e-6)), max_norm >= 0: one float32 each in device memory, factor NULL for none.
+ * With `scale` the tensors are multiplied by the factor in place (they must not
+ * overlap), unless it is one.  A NaN norm has a NaN factor.  The sum is float64 and
+ * does not depend on the schedule. */
+typedef struct gs_tensor {
+  void* data;
+  int64_t numel;
+  int64_t type;
+} gs_tensor;
+GS_API size_t gs_grad_norm_workspace_bytes(int64_t count);
+GS_API int gs_grad_norm(
+    const gs_tensor* tensors, int64_t count, double max_norm, int32_t scale,
+    float* norm, float* factor, void* workspace, size_t workspace_bytes,
+    void* stream);
 
 /* Scene files: the binary PLY "vertex" records of a Gaussian-splat scene
  * (src/gaussian_splats/splats/ply.py).  Fields per Gaussian in canonical
