@@ -422,6 +422,9 @@ _SIGNATURES = {
     "gs_window_attention_bwd": (c_int, [c_void_p] * 13 + [c_size_t, c_void_p]),
     "gs_window_attention_step_workspace_bytes": (c_size_t, [c_void_p]),
     "gs_window_attention_step": (c_int, [c_void_p] * 10 + [c_size_t, c_void_p]),
+    "gs_window_attention_step_quant_workspace_bytes": (c_size_t, [c_void_p]),
+    "gs_window_attention_step_quant": (c_int, [c_void_p] * 11 + [c_size_t, c_void_p]),
+    "gs_window_cache_fill_quant": (c_int, [c_void_p] * 10),
 }
 
 PLY_MAX_FIELDS = 89

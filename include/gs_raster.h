@@ -797,6 +797,33 @@ GS_API int gs_window_attention_step(
     const int32_t* positions, void* out, void* workspace,
     size_t workspace_bytes, void* stream);
 
+/* The same over caches held in 4 bits (the microscaling format MXFP4): each row of
+ * head_dim elements, a multiple of 32 (GS_ERR_UNSUPPORTED otherwise), in blocks of
+ * 32.  codes [batch, kv_heads, sinks + window, head_dim / 2], contiguous and on a
+ * 16-byte boundary, hold two elements a byte, the even one in the low half: a sign
+ * bit above the index into 0, 0.5, 1, 1.5, 2, 3, 4, 6.  exponents [batch, kv_heads,
+ * sinks + window, head_dim / 32], contiguous bytes, hold the block's power of two +
+ * 127; 255: the block is NaN.  A block is encoded with the power floor(log2 max|x|)
+ * - 2, not below -127, elements to the nearest code (ties to the even one, 6 beyond
+ * 6); one with an infinity or a NaN becomes NaN.  The new token's key and value are
+ * encoded, written and attended to as they are held. */
+GS_API size_t gs_window_attention_step_quant_workspace_bytes(const gs_attention* attention);
+GS_API int gs_window_attention_step_quant(
+    const gs_attention* attention, const void* q, const void* k, const void* v,
+    void* k_codes, void* k_exponents, void* v_codes, void* v_exponents,
+    const int32_t* positions, void* out, void* workspace, size_t workspace_bytes,
+    void* stream);
+
+/* Fills such caches from the k and v [batch, keys, kv_heads, head_dim] of a
+ * prefill (strides of k and v as in gs_window_attention_fwd; rows on 16-byte
+ * boundaries): each slot takes the last of its tokens that exist, those below
+ * lengths[b] (int32, device memory; NULL: all); a slot that has none is left as it
+ * was. */
+GS_API int gs_window_cache_fill_quant(
+    const gs_attention* attention, const void* k, const void* v,
+    const int64_t* strides, const int32_t* lengths, void* k_codes,
+    void* k_exponents, void* v_codes, void* v_exponents, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -113,3 +113,43 @@ def window_attention_step(q, k, v, k_cache, v_cache, positions, window, sinks, s
             w = torch.softmax(kk @ q[i, m].double() * scale, 0)
             out[i, m] = w @ v_cache[i, :n, m * hk // h].double()
     return out, k_cache, v_cache
+
+
+#: What the 4-bit codes 0 .. 7 stand for; 8 .. 15 are their negatives.
+MXFP4_VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def mxfp4_encode(x):
+    """(codes [.., n / 2], exponents [.., n / 32]) of rows, uint8: the power of two
+    of a block of 32 is floor(log2 max|x|) - 2, not below -127, held + 127; elements
+    go to the nearest value, of two as near the one of the even code.  A block that
+    is not finite has the exponent 255 and codes of zero."""
+    x = x.double().unflatten(-1, (-1, 32))
+    top = x.abs().amax(-1)
+    fine = torch.isfinite(x).all(-1)
+    power = torch.where(top > 0, torch.floor(torch.log2(torch.where(top > 0, top, 1.0))) - 2, -127.0)
+    power = torch.where(fine, power, 0.0).clamp(-127, 127)
+    y = (x.abs() / torch.exp2(power)[..., None])[..., None]
+    even = (0, 2, 4, 6, 1, 3, 5, 7)
+    levels = torch.tensor([MXFP4_VALUES[c] for c in even], dtype=torch.float64)
+    codes = torch.tensor(even)[(y - levels).abs().nan_to_num(0.0).argmin(-1)] + 8 * torch.signbit(x)
+    codes = torch.where(fine[..., None], codes, 0).flatten(-2).to(torch.uint8)
+    exponents = torch.where(fine, power + 127, 255.0).to(torch.uint8)
+    return codes[..., ::2] | codes[..., 1::2] << 4, exponents
+
+
+def mxfp4_decode(codes, exponents):
+    """What codes and exponents stand for, in float64."""
+    values = torch.tensor(MXFP4_VALUES + tuple(-v for v in MXFP4_VALUES), dtype=torch.float64)
+    x = values[torch.stack([codes & 15, codes >> 4], -1).flatten(-2).long()].unflatten(-1, (-1, 32))
+    power = torch.exp2(exponents.double() - 127)
+    return (x * torch.where(exponents == 255, float("nan"), power)[..., None]).flatten(-2)
+
+
+def window_cache_fill(x, length, window, sinks, capacity):
+    """The token that each slot of a cache takes of a sequence's first ``length``
+    tokens; -1: none."""
+    token = torch.full((capacity,), -1)
+    for t in range(min(length, x.shape[0])):
+        token[cache_slot(t, window, sinks)] = t
+    return token
