@@ -1,0 +1,307 @@
+// Shared pieces of the gated delta rule's kernels.
+//
+// A head's state is a matrix S [key_dim, dim].  With a = sigmoid(gate) and b =
+// sigmoid(beta), a token reads what its key finds, and writes the difference:
+//   u_t = b_t (v_t - a_t S_{t-1}^T k_t),  S_t = a_t S_{t-1} + k_t u_t^T,
+//   o_t = scale S_t^T q_t.
+// In chunks of 64 tokens, with S the state before one, G_i the logarithm of a_1 ..
+// a_i and D_ij = e^(G_i - G_j) for j <= i, the updates of a chunk solve a triangular
+// system:
+//   (I + A) U = b V - (b e^G) K S,   A_ij = b_i D_ij (k_i . k_j) for j < i,
+// so with T = (I + A)^-1, W = T (b e^G) K and F = T b V,
+//   U = F - W S,   O = scale (e^G Q S + (Q K^T * D) U),
+//   S' = e^(G_C) S + K^T (e^(G_C - G) U).
+// W and F need no state, O needs no later one: only the second line's U and the
+// third line go from chunk to chunk (delta_chain.hip), two products each, and the
+// rest runs over all chunks at once.  The backward has the same shape: with P =
+// scale Q K^T * D,
+//   dU = P^T dO + e^(G_C - G) K dS',   dS = e^(G_C) dS' + scale Q^T e^G dO - W^T dU.
+//
+// Products run on the matrix cores.  What the states depend on is to be as exact as
+// float32, so a factor that is not an input is a sum of two bfloat16 numbers (16 bits
+// of mantissa, the range of float32), and inputs in float16 are two as well, exactly;
+// products of two second parts are left out.  Outputs in bfloat16 take one part a
+// factor.  float32 inputs stay in float32, and become three parts in the chain.
+#pragma once
+
+#include "attention_tile.h"
+
+namespace gs {
+namespace delta {
+
+using namespace att;
+
+constexpr int kChunk = 64;
+constexpr int kThreads = 256;
+
+// Parts of an input, of another factor of what states depend on, and of an output.
+template <typename T>
+struct Form {
+  using Elem = bf16;
+  static constexpr int in = 1, mid = 2, out = 1;
+  static constexpr int chain_in = 1, chain = 2;
+};
+template <>
+struct Form<f16> {
+  using Elem = bf16;
+  static constexpr int in = 2, mid = 2, out = 2;
+  static constexpr int chain_in = 2, chain = 2;
+};
+template <>
+struct Form<float> {
+  using Elem = float;
+  static constexpr int in = 1, mid = 1, out = 1;
+  static constexpr int chain_in = 3, chain = 3;
+};
+
+// The parts of N numbers, largest first.
+template <typename E, int P, int N>
+struct Parts {
+  Vec<E, N> v[P];
+  __device__ __forceinline__ Parts() {}
+  __device__ __forceinline__ explicit Parts(FloatVec<N> x) {
+    v[0] = from_float<E, N>(x);
+#pragma unroll
+    for (int i = 1; i < P; ++i) {
+      x -= to_float<E, N>(v[i - 1]);
+      v[i] = from_float<E, N>(x);
+    }
+  }
+};
+
+template <typename E, int PA, int PB>
+__device__ __forceinline__ void mma_parts(const Parts<E, PA, 8>& a, const Parts<E, PB, 8>& b, Acc& c) {
+#pragma unroll
+  for (int i = 0; i < PA; ++i)
+#pragma unroll
+    for (int j = 0; j < PB; ++j)
+      if (i + j < (PA > PB ? PA : PB)) mma(a.v[i], b.v[j], c);
+}
+
+// Columns n0 + (lane & 31) of a tile, its rows k0 + 8 (lane >> 5) .. + 7: what
+// load_rows gives of the turned tile.
+template <typename T>
+__device__ __forceinline__ Frag<T> load_cols(const T* tile, int pitch, int k0, int n0) {
+  const int lane = threadIdx.x & 63;
+  if constexpr (sizeof(T) == 2) {
+    using Short4 = Vec<short, 4>;
+    using Lds = __attribute__((address_space(3))) Short4*;
+    const T* p = tile + (k0 + 8 * (lane >> 5) + ((lane & 15) >> 2)) * pitch + n0 +
+                 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    const Short4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(p));
+    const Short4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(p + 4 * pitch));
+    return __builtin_bit_cast(Frag<T>, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  } else {
+    const T* p = tile + (k0 + 8 * (lane >> 5)) * pitch + n0 + (lane & 31);
+    Frag<T> f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = p[i * pitch];
+    return f;
+  }
+}
+
+// A [kRows, kWide] matrix in LDS, a tile for each part.
+template <typename E, int P, int kRows, int kWide>
+struct Tile {
+  static constexpr int pitch = kWide + 16 / int(sizeof(E));
+  static constexpr int part = kRows * pitch;
+  static constexpr int bytes = P * part * int(sizeof(E));
+  E* p;
+
+  __device__ __forceinline__ explicit Tile(char* at) : p(reinterpret_cast<E*>(at)) {}
+  __device__ __forceinline__ Parts<E, P, 8> rows(int row0, int k0) const {
+    Parts<E, P, 8> f;
+#pragma unroll
+    for (int i = 0; i < P; ++i) f.v[i] = load_rows<E>(p + i * part, pitch, row0, k0);
+    return f;
+  }
+  __device__ __forceinline__ Parts<E, P, 8> cols(int k0, int n0) const {
+    Parts<E, P, 8> f;
+#pragma unroll
+    for (int i = 0; i < P; ++i) f.v[i] = load_cols<E>(p + i * part, pitch, k0, n0);
+    return f;
+  }
+  template <int N>
+  __device__ __forceinline__ void put(int row, int col, const Parts<E, P, N>& v) const {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      E* at = p + i * part + row * pitch + col;
+      if constexpr (N * sizeof(E) > 16) {
+        *reinterpret_cast<Vec<E, 4>*>(at) = __builtin_shufflevector(v.v[i], v.v[i], 0, 1, 2, 3);
+        *reinterpret_cast<Vec<E, 4>*>(at + 4) = __builtin_shufflevector(v.v[i], v.v[i], 4, 5, 6, 7);
+      } else {
+        *reinterpret_cast<Vec<E, N>*>(at) = v.v[i];
+      }
+    }
+  }
+  // Four numbers of a row.
+  __device__ __forceinline__ FloatVec<4> get4(int row, int col) const {
+    FloatVec<4> x(0.0f);
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+      x += to_float<E, 4>(*reinterpret_cast<const Vec<E, 4>*>(p + i * part + row * pitch + col));
+    return x;
+  }
+};
+
+// Four consecutive numbers of a 32 x 32 result's column, the s-th of four.
+__device__ __forceinline__ FloatVec<4> four(const Acc& c, int s) {
+  return FloatVec<4>{c[4 * s], c[4 * s + 1], c[4 * s + 2], c[4 * s + 3]};
+}
+__device__ __forceinline__ int four_row(int s) { return 8 * s + 4 * (int(threadIdx.x & 63) >> 5); }
+
+// Rows 0 .. 63 of `from` (rows `stride` elements apart, 16-byte boundaries) into a
+// tile, zeros from `rows` on and from column `wide` on.  Calls f(row, col, x) for what
+// is kept of eight numbers.
+template <typename T, typename E, int P, int kRows, int kWide, typename F>
+__device__ __forceinline__ void load_tile(const Tile<E, P, kRows, kWide>& tile, const T* from,
+                                          int64_t stride, int rows, int wide, F&& f) {
+  constexpr int kPerRow = kWide / 8, kCount = kRows * kPerRow / kThreads;
+  static_assert(kRows * kPerRow % kThreads == 0, "whole chunks");
+  Frag<T> x[kCount];
+#pragma unroll
+  for (int i = 0; i < kCount; ++i) {
+    const int chunk = i * kThreads + int(threadIdx.x);
+    const int row = chunk / kPerRow, col = chunk % kPerRow * 8;
+    x[i] = load_global<T>(from + row * stride + col, row < rows && col < wide);
+  }
+#pragma unroll
+  for (int i = 0; i < kCount; ++i) {
+    const int chunk = i * kThreads + int(threadIdx.x);
+    const int row = chunk / kPerRow, col = chunk % kPerRow * 8;
+    if constexpr (std::is_same_v<T, E> && P == 1) {
+      Parts<E, 1, 8> one;
+      one.v[0] = x[i];
+      f(row, col, one.v[0]);
+      tile.put(row, col, one);
+    } else {
+      FloatVec<8> y = to_float<T, 8>(x[i]);
+      f(row, col, y);
+      tile.put(row, col, Parts<E, P, 8>(y));
+    }
+  }
+}
+struct Keep {
+  template <typename V>
+  __device__ __forceinline__ void operator()(int, int, V&) const {}
+};
+
+// Numbers of a chunk's tokens that all products take.
+struct Gates {
+  float beta[kChunk];             // b
+  float hi[kChunk], lo[kChunk];   // G in powers of two, as a sum
+  float up[kChunk], down[kChunk]; // e^G, e^(G_C - G)
+  float whole;                    // e^(G_C)
+  int bad;  // the first token with a number that is not finite; kChunk: none
+  // D_ij
+  __device__ __forceinline__ float decay(int i, int j) const {
+    return __builtin_amdgcn_exp2f((hi[i] - hi[j]) + (lo[i] - lo[j]));
+  }
+};
+
+// log2 of sigmoid(x); below -300 it is no longer told from a state that is gone.
+__device__ __forceinline__ float log2_sigmoid(float x) {
+  return fmaxf(kLog2e * (fminf(x, 0.0f) - log1pf(expf(-fabsf(x)))), -300.0f);
+}
+__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
+
+struct Problem {
+  int batch, tokens, heads, key_heads, key_dim, dim, chunks;
+  float scale;
+  const int32_t* lengths;
+
+  __device__ __forceinline__ int length(int b) const {
+    return lengths ? min(max(lengths[b], 0), tokens) : tokens;
+  }
+};
+
+// A workgroup's chunk of one head.
+struct Place {
+  int b, h, c, key_head, t0, rows, valid;  // rows that exist, rows of the sequence
+  int64_t id;
+  __device__ __forceinline__ Place(const Problem& p, int64_t index) : id(index) {
+    c = int(index % p.chunks);
+    const int64_t head = index / p.chunks;
+    h = int(head % p.heads);
+    b = int(head / p.heads);
+    key_head = int(int64_t(h) * p.key_heads / p.heads);
+    t0 = c * kChunk;
+    rows = min(p.tokens - t0, kChunk);
+    valid = max(0, min(p.length(b) - t0, kChunk));
+  }
+};
+
+template <typename T>
+struct Rows {
+  const T* p;
+  Strides s;
+  __device__ __forceinline__ const T* at(int b, int t, int h) const {
+    return p + b * s.batch + t * s.token + h * s.head;
+  }
+};
+
+// By one wave, a lane a token.  The sums are float64: differences of far tokens'
+// logarithms keep their bits.
+template <typename T>
+__device__ __forceinline__ void load_gates(Gates& g, const Rows<T>& gate, const Rows<T>& beta,
+                                           const Place& at) {
+  const int lane = threadIdx.x & 63;
+  float x = INFINITY, y = -INFINITY;
+  if (lane < at.valid) {
+    x = float(*gate.at(at.b, at.t0 + lane, at.h));
+    y = float(*beta.at(at.b, at.t0 + lane, at.h));
+  }
+  const bool bad = x != x || y != y;
+  double total = bad ? 0.0 : double(log2_sigmoid(x));
+#pragma unroll
+  for (int d = 1; d < kChunk; d <<= 1) {
+    const double before = __shfl_up(total, d, kChunk);
+    if (lane >= d) total += before;
+  }
+  const double last = __shfl(total, kChunk - 1, kChunk);
+  g.beta[lane] = bad ? 0.0f : sigmoid(y);
+  g.hi[lane] = float(total);
+  g.lo[lane] = float(total - double(float(total)));
+  g.up[lane] = __builtin_amdgcn_exp2f(float(total));
+  g.down[lane] = __builtin_amdgcn_exp2f(float(last - total));
+  const uint64_t marks = __ballot(bad);
+  if (lane == 0) {
+    g.whole = __builtin_amdgcn_exp2f(float(last));
+    g.bad = marks ? __builtin_ctzll(marks) : kChunk;
+  }
+}
+
+// What is kept between the kernels, one after the other for each chunk of each
+// head; widths padded to kKey and kDim.
+struct Kept {
+  float* starts;   // [kKey, kDim]: the state before the chunk
+  float* updates;  // [64, kDim]: F, then U
+  float* solve;    // [64, 64]: T, or null
+};
+
+// Factors of the chain, a chunk of a head each.
+struct Chain {
+  bf16* left;      // parts of [64, kKey]
+  bf16* right;     // parts of [kKey, 64]
+  float* factors;  // 64 of e^(G_C - G), then e^(G_C) and the first token that is not finite
+};
+constexpr int kFactors = kChunk + 4;
+
+int64_t padded(int dim);
+
+// The chain over the chunks of every head (delta_chain.hip).
+struct ChainArgs {
+  int64_t heads;  // of all sequences
+  int chunks, key_dim, dim;
+  Chain chain;
+  const float* first;  // the state before the first chunk [heads, key_dim, dim], or null
+  float* rows;         // [64, kDim] a chunk: what the rows start with, then the rows
+  float* states;       // [kKey, kDim] a chunk: what the next state starts with
+                       // (backward), then the state before the chunk
+  float* last;         // the state behind the last chunk, or null
+};
+int launch_chain(const ChainArgs& a, int key_wide, int wide, int parts_in, bool backward,
+                 hipStream_t s);
+
+}  // namespace delta
+}  // namespace gs

@@ -62,6 +62,19 @@ class GsAttention(ctypes.Structure):
     ]
 
 
+class GsDelta(ctypes.Structure):
+    _fields_ = [
+        ("batch", c_int64),
+        ("tokens", c_int64),
+        ("heads", c_int32),
+        ("key_heads", c_int32),
+        ("key_dim", c_int32),
+        ("dim", c_int32),
+        ("type", c_int32),
+        ("scale", c_float),
+    ]
+
+
 class GsView(ctypes.Structure):
     _fields_ = [
         ("fx", c_float),
@@ -417,6 +430,14 @@ _SIGNATURES = {
     "gs_gated_scan_step": (
         c_int, [c_void_p] * 3 + [c_int64] * 2 + [c_int32] + [c_void_p] * 3
     ),
+    "gs_delta_scan_kept_bytes": (c_size_t, [c_void_p, c_int32]),
+    "gs_delta_scan_workspace_bytes": (c_size_t, [c_void_p]),
+    "gs_delta_scan_fwd": (
+        c_int, [c_void_p] * 9 + [c_int32] + [c_void_p] * 4 + [c_size_t, c_void_p]
+    ),
+    "gs_delta_scan_bwd_workspace_bytes": (c_size_t, [c_void_p]),
+    "gs_delta_scan_bwd": (c_int, [c_void_p] * 18 + [c_size_t, c_void_p]),
+    "gs_delta_scan_step": (c_int, [c_void_p] * 10),
     "gs_window_attention_fwd": (c_int, [c_void_p] * 9),
     "gs_window_attention_bwd_workspace_bytes": (c_size_t, [c_void_p]),
     "gs_window_attention_bwd": (c_int, [c_void_p] * 13 + [c_size_t, c_void_p]),

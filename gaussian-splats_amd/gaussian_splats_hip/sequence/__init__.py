@@ -1,6 +1,6 @@
 """Sequence operators of networks that predict splats from a stream of posed
-views, as HIP kernels: the residual norm, a gated linear recurrence and
-attention with a sliding window in which the stream's first tokens stay
+views, as HIP kernels: the residual norm, a gated linear recurrence, the gated
+delta rule and attention with a sliding window in which the stream's first tokens stay
 visible, each for training (forward and backward) and for one token of a
 running stream, the attention's cache in the inputs' type or in 4 bits."""
 
@@ -16,6 +16,7 @@ from .cache_quant import (
     window_attention_step_quant,
     window_cache_fill_quant,
 )
+from .delta import delta_scan, delta_scan_backward, delta_scan_forward, delta_scan_step
 from .norm import add_rms_norm, add_rms_norm_backward, add_rms_norm_forward, add_rms_norm_quant
 from .scan import gated_scan, gated_scan_backward, gated_scan_forward, gated_scan_step
 
@@ -26,6 +27,10 @@ __all__ = [
     "add_rms_norm_backward",
     "add_rms_norm_forward",
     "add_rms_norm_quant",
+    "delta_scan",
+    "delta_scan_backward",
+    "delta_scan_forward",
+    "delta_scan_step",
     "gated_scan",
     "gated_scan_backward",
     "gated_scan_forward",

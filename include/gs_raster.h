@@ -735,6 +735,65 @@ GS_API int gs_gated_scan_step(
     const void* x, const void* gate, const float* state, int64_t batch,
     int64_t channels, int32_t type, void* y, float* state_out, void* stream);
 
+/* The gated delta rule: a matrix S [key_dim, dim] for each head and sequence, with a
+ * = sigmoid(gate) and b = sigmoid(beta),
+ *   u_t = b_t (v_t - a_t S^T k_t),  S = a_t S + k_t u_t^T,  o_t = scale S^T q_t.
+ * q and k [batch, tokens, key_heads, key_dim], v [batch, tokens, heads, dim], gate
+ * and beta [batch, tokens, heads], all of one type; heads a multiple of key_heads
+ * (head h reads key h * key_heads / heads); key_dim and dim multiples of 8 up to 128
+ * (GS_ERR_UNSUPPORTED otherwise); scale > 0.  Keys longer than one let states grow. */
+typedef struct gs_delta {
+  int64_t batch;
+  int64_t tokens;
+  int32_t heads;
+  int32_t key_heads;
+  int32_t key_dim;
+  int32_t dim;
+  int32_t type;
+  float scale;
+} gs_delta;
+
+/* Writes out [batch, tokens, heads, dim], last (float32 [batch, heads, key_dim, dim],
+ * the state behind the last token) and kept (gs_delta_scan_kept_bytes with the same
+ * `backward`, 16-byte boundary), which the backward reads; it is needed without one
+ * too.  state is the one before the first token, NULL for zeros.  Tokens from
+ * lengths[b] on (int32, device memory; NULL: all exist) change no state, are not read
+ * as values and get zeros.  strides, host memory: batch, token and head stride in
+ * elements of q, k, v, gate and beta (the backward: grad_out's after them); rows of q,
+ * k, v and grad_out on 16-byte boundaries.  From a k, v, gate or beta that is not
+ * finite on (gate may be infinite) outputs and states of its head are NaN; tokens
+ * before it keep theirs.  States are float32 throughout.  The results do not depend on
+ * the schedule.  With no token nothing is written. */
+GS_API size_t gs_delta_scan_kept_bytes(const gs_delta* delta, int32_t backward);
+GS_API size_t gs_delta_scan_workspace_bytes(const gs_delta* delta);
+GS_API int gs_delta_scan_fwd(
+    const gs_delta* delta, const void* q, const void* k, const void* v,
+    const void* gate, const void* beta, const int64_t* strides,
+    const int32_t* lengths, const float* state, int32_t backward, void* out,
+    float* last, void* kept, void* workspace, size_t workspace_bytes,
+    void* stream);
+
+/* Gradients (contiguous, shaped like their inputs; those of shared keys summed over
+ * their heads in order) from the forward's kept (with `backward`); grad_out and
+ * grad_last (float32) NULL for zeros, grad_state NULL if it is not wanted.  Where
+ * the forward met a value that is not finite, gradients of its chunk of 64 tokens and
+ * of those before it need not be finite either. */
+GS_API size_t gs_delta_scan_bwd_workspace_bytes(const gs_delta* delta);
+GS_API int gs_delta_scan_bwd(
+    const gs_delta* delta, const void* q, const void* k, const void* v,
+    const void* gate, const void* beta, const void* grad_out,
+    const int64_t* strides, const int32_t* lengths,
+    const float* grad_last, const void* kept, void* grad_q, void* grad_k,
+    void* grad_v, void* grad_gate, void* grad_beta, float* grad_state,
+    void* workspace, size_t workspace_bytes, void* stream);
+
+/* One token of the rule (tokens is not read): all tensors contiguous, without the
+ * token's dimension; state_out may be state. */
+GS_API int gs_delta_scan_step(
+    const gs_delta* delta, const void* q, const void* k, const void* v,
+    const void* gate, const void* beta, const float* state, void* out,
+    float* state_out, void* stream);
+
 /* Attention with a sliding window and visible first tokens.  q [batch,
  * queries, heads, head_dim], k and v [batch, keys, kv_heads, head_dim], heads a
  * multiple of kv_heads (head h reads key head h * kv_heads / heads).  Query i

@@ -153,3 +153,52 @@ def window_cache_fill(x, length, window, sinks, capacity):
     for t in range(min(length, x.shape[0])):
         token[cache_slot(t, window, sinks)] = t
     return token
+
+
+def delta_scan(q, k, v, gate, beta, state=None, scale=None, lengths=None, grads=None):
+    """(out, last) of the gated delta rule, token after token; with ``grads``, those
+    of out and last, also the gradients of q, k, v, gate, beta and state."""
+    h, hk, d = v.shape[2], q.shape[2], q.shape[3]
+    tokens = q.shape[1]
+    scale = 1 / math.sqrt(d) if scale is None else scale
+    of = torch.arange(h) * hk // h
+    q, k, v, gate, beta = (t.double() for t in (q, k, v, gate, beta))
+    qq, kk = q[:, :, of], k[:, :, of]
+    a, b = torch.sigmoid(gate), torch.sigmoid(beta)
+    there = torch.ones(a.shape[:2], dtype=torch.bool)
+    if lengths is not None:
+        there = torch.arange(tokens) < lengths.cpu()[:, None]
+    hide = ~there[..., None]
+    a, b = a.masked_fill(hide, 1.0), b.masked_fill(hide, 0.0)
+    qq, kk, v = (t.masked_fill(hide[..., None], 0.0) for t in (qq, kk, v))
+    s = torch.zeros(v.shape[0], h, d, v.shape[3], dtype=torch.float64) if state is None else state.double()
+    states, out, u = [s], torch.empty_like(v), torch.empty_like(v)
+    for t in range(tokens):
+        kept = a[:, t, :, None, None] * s
+        u[:, t] = b[:, t, :, None] * (v[:, t] - (kk[:, t, :, :, None] * kept).sum(2))
+        s = kept + kk[:, t, :, :, None] * u[:, t, :, None]
+        out[:, t] = scale * (qq[:, t, :, :, None] * s).sum(2)
+        states.append(s)
+    if grads is None:
+        return out, s
+    do = grads[0].double().masked_fill(hide[..., None], 0.0)
+    ds = grads[1].double()
+    dq, dk, dv = torch.empty_like(qq), torch.empty_like(kk), torch.empty_like(v)
+    da, db = torch.empty_like(a), torch.empty_like(b)
+    for t in range(tokens - 1, -1, -1):
+        before, kt = states[t], kk[:, t, :, :, None]
+        ds = ds + scale * qq[:, t, :, :, None] * do[:, t, :, None]
+        dq[:, t] = scale * (states[t + 1] * do[:, t, :, None]).sum(-1)
+        du = (kt * ds).sum(2)
+        found = a[:, t, :, None] * (kt * before).sum(2)
+        db[:, t] = (du * (v[:, t] - found)).sum(-1)
+        dv[:, t] = b[:, t, :, None] * du
+        # found, and through it a S and k, has the gradient -dv.
+        dk[:, t] = (ds * u[:, t, :, None]).sum(-1) - a[:, t, :, None] * (before * dv[:, t, :, None]).sum(-1)
+        through = ds - kt * dv[:, t, :, None]
+        da[:, t] = (before * through).sum((-1, -2))
+        ds = a[:, t, :, None, None] * through
+    shared = [t.masked_fill(hide[..., None], 0.0).unflatten(2, (hk, h // hk)).sum(3) for t in (dq, dk)]
+    dgate = (da * a * torch.sigmoid(-gate)).masked_fill(hide, 0.0)
+    dbeta = (db * b * torch.sigmoid(-beta)).masked_fill(hide, 0.0)
+    return (out, s, *shared, dv.masked_fill(hide[..., None], 0.0), dgate, dbeta, ds)
