@@ -34,22 +34,33 @@ using namespace att;
 constexpr int kChunk = 64;
 constexpr int kThreads = 256;
 
+// All of the workgroup's writes to LDS are there; loads and stores of global memory
+// go on.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // Parts of an input, of another factor of what states depend on, and of an output.
 template <typename T>
 struct Form {
   using Elem = bf16;
+  using Store = bf16;
   static constexpr int in = 1, mid = 2, out = 1;
   static constexpr int chain_in = 1, chain = 2;
 };
 template <>
 struct Form<f16> {
   using Elem = bf16;
+  using Store = float;
   static constexpr int in = 2, mid = 2, out = 2;
   static constexpr int chain_in = 2, chain = 2;
 };
 template <>
 struct Form<float> {
   using Elem = float;
+  using Store = float;
   static constexpr int in = 1, mid = 1, out = 1;
   static constexpr int chain_in = 3, chain = 3;
 };
@@ -61,10 +72,19 @@ struct Parts {
   __device__ __forceinline__ Parts() {}
   __device__ __forceinline__ explicit Parts(FloatVec<N> x) {
     v[0] = from_float<E, N>(x);
+    if constexpr (P > 1) {
 #pragma unroll
-    for (int i = 1; i < P; ++i) {
-      x -= to_float<E, N>(v[i - 1]);
-      v[i] = from_float<E, N>(x);
+      for (int i = 1; i < P; ++i) {
+        // The number that a bfloat16 is has its bits above sixteen zeros.
+        using Words = Vec<uint32_t, N / 2>;
+        const Words w = __builtin_bit_cast(Words, v[i - 1]);
+#pragma unroll
+        for (int k = 0; k < N / 2; ++k) {
+          x[2 * k] -= __uint_as_float(w[k] << 16);
+          x[2 * k + 1] -= __uint_as_float(w[k] & 0xffff0000u);
+        }
+        v[i] = from_float<E, N>(x);
+      }
     }
   }
 };
@@ -134,6 +154,12 @@ struct Tile {
       }
     }
   }
+  __device__ __forceinline__ float get(int row, int col) const {
+    float x = 0.0f;
+#pragma unroll
+    for (int i = 0; i < P; ++i) x += float(p[i * part + row * pitch + col]);
+    return x;
+  }
   // Four numbers of a row.
   __device__ __forceinline__ FloatVec<4> get4(int row, int col) const {
     FloatVec<4> x(0.0f);
@@ -144,46 +170,81 @@ struct Tile {
   }
 };
 
+// Calls f(s) for N steps of a contraction, unrolled: all reads of LDS can be ahead of
+// the products.
+template <int N, typename F>
+__device__ __forceinline__ void steps(F&& f) {
+#pragma unroll
+  for (int s = 0; s < N; ++s) f(s);
+}
+// Rows 0 .. 31 of a lower triangle of 64 have 32 columns, rows 32 .. 63 all of them.
+template <typename F>
+__device__ __forceinline__ void steps_to(int row0, F&& f) {
+  if (row0)
+    steps<4>(f);
+  else
+    steps<2>(f);
+}
+// Columns 0 .. 31 have all rows, columns 32 .. 63 the rows from 32 on.
+template <typename F>
+__device__ __forceinline__ void steps_from(int col0, F&& f) {
+  if (col0)
+    steps<2>([&](int s) { f(s + 2); });
+  else
+    steps<4>(f);
+}
+
 // Four consecutive numbers of a 32 x 32 result's column, the s-th of four.
 __device__ __forceinline__ FloatVec<4> four(const Acc& c, int s) {
   return FloatVec<4>{c[4 * s], c[4 * s + 1], c[4 * s + 2], c[4 * s + 3]};
 }
 __device__ __forceinline__ int four_row(int s) { return 8 * s + 4 * (int(threadIdx.x & 63) >> 5); }
 
-// Rows 0 .. 63 of `from` (rows `stride` elements apart, 16-byte boundaries) into a
-// tile, zeros from `rows` on and from column `wide` on.  Calls f(row, col, x) for what
-// is kept of eight numbers.
-template <typename T, typename E, int P, int kRows, int kWide, typename F>
-__device__ __forceinline__ void load_tile(const Tile<E, P, kRows, kWide>& tile, const T* from,
-                                          int64_t stride, int rows, int wide, F&& f) {
-  constexpr int kPerRow = kWide / 8, kCount = kRows * kPerRow / kThreads;
+// Rows 0 .. kRows - 1 of a matrix on their way through the workgroup's registers into
+// a tile, zeros from row `rows` and column `wide` on.  Loading and storing are apart, so
+// that all matrices of a phase, and those of the next, are on their way at once: a
+// kernel of short phases waits for memory once instead of once a matrix (gradients of
+// 40000 tokens, 12 heads of 64: 523 us one matrix after the other, @GRADS@ so).
+template <typename T, int kRows, int kWide>
+struct Fetch {
+  static constexpr int kPerRow = kWide / 8, kCount = kRows * kPerRow / kThreads;
   static_assert(kRows * kPerRow % kThreads == 0, "whole chunks");
   Frag<T> x[kCount];
+
+  static __device__ __forceinline__ int row(int i) { return (i * kThreads + int(threadIdx.x)) / kPerRow; }
+  static __device__ __forceinline__ int col(int i) { return (i * kThreads + int(threadIdx.x)) % kPerRow * 8; }
+  // T of a chunk: its upper right quarter is zeros.
+  __device__ __forceinline__ void load_triangle(const T* from) {
 #pragma unroll
-  for (int i = 0; i < kCount; ++i) {
-    const int chunk = i * kThreads + int(threadIdx.x);
-    const int row = chunk / kPerRow, col = chunk % kPerRow * 8;
-    x[i] = load_global<T>(from + row * stride + col, row < rows && col < wide);
+    for (int i = 0; i < kCount; ++i)
+      x[i] = load_global<T>(from + row(i) * kWide + col(i), row(i) >= kRows / 2 || col(i) < kWide / 2);
   }
+  __device__ __forceinline__ void load(const T* from, int64_t stride, int rows, int wide) {
 #pragma unroll
-  for (int i = 0; i < kCount; ++i) {
-    const int chunk = i * kThreads + int(threadIdx.x);
-    const int row = chunk / kPerRow, col = chunk % kPerRow * 8;
-    if constexpr (std::is_same_v<T, E> && P == 1) {
-      Parts<E, 1, 8> one;
-      one.v[0] = x[i];
-      f(row, col, one.v[0]);
-      tile.put(row, col, one);
-    } else {
-      FloatVec<8> y = to_float<T, 8>(x[i]);
-      f(row, col, y);
-      tile.put(row, col, Parts<E, P, 8>(y));
+    for (int i = 0; i < kCount; ++i)
+      x[i] = load_global<T>(from + row(i) * stride + col(i), row(i) < rows && col(i) < wide);
+  }
+  // Calls f(row, col, numbers) for what is kept of eight.
+  template <typename E, int P, typename F>
+  __device__ __forceinline__ void put(const Tile<E, P, kRows, kWide>& tile, F&& f) const {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+      if constexpr (std::is_same_v<T, E> && P == 1) {
+        Parts<E, 1, 8> one;
+        one.v[0] = x[i];
+        f(row(i), col(i), one.v[0]);
+        tile.put(row(i), col(i), one);
+      } else {
+        FloatVec<8> y = to_float<T, 8>(x[i]);
+        f(row(i), col(i), y);
+        tile.put(row(i), col(i), Parts<E, P, 8>(y));
+      }
     }
   }
-}
-struct Keep {
-  template <typename V>
-  __device__ __forceinline__ void operator()(int, int, V&) const {}
+  template <typename E, int P>
+  __device__ __forceinline__ void put(const Tile<E, P, kRows, kWide>& tile) const {
+    put(tile, [](int, int, auto&) {});
+  }
 };
 
 // Numbers of a chunk's tokens that all products take.
@@ -191,6 +252,7 @@ struct Gates {
   float beta[kChunk];             // b
   float hi[kChunk], lo[kChunk];   // G in powers of two, as a sum
   float up[kChunk], down[kChunk]; // e^G, e^(G_C - G)
+  float fade[kChunk], rest[kChunk];  // 1 - a, 1 - b
   float whole;                    // e^(G_C)
   int bad;  // the first token with a number that is not finite; kChunk: none
   // D_ij
@@ -240,49 +302,69 @@ struct Rows {
   }
 };
 
-// By one wave, a lane a token.  The sums are float64: differences of far tokens'
-// logarithms keep their bits.
-template <typename T>
-__device__ __forceinline__ void load_gates(Gates& g, const Rows<T>& gate, const Rows<T>& beta,
-                                           const Place& at) {
-  const int lane = threadIdx.x & 63;
-  float x = INFINITY, y = -INFINITY;
-  if (lane < at.valid) {
-    x = float(*gate.at(at.b, at.t0 + lane, at.h));
-    y = float(*beta.at(at.b, at.t0 + lane, at.h));
+// The gates on their way: a kernel loads them before its tiles, which they would else
+// wait behind.
+struct GatePair {
+  float gate, beta;
+  template <typename T>
+  __device__ __forceinline__ GatePair(const Rows<T>& g, const Rows<T>& b, const Place& at)
+      : gate(INFINITY), beta(-INFINITY) {
+    const int lane = threadIdx.x & 63;
+    if (lane < at.valid) {
+      gate = float(*g.at(at.b, at.t0 + lane, at.h));
+      beta = float(*b.at(at.b, at.t0 + lane, at.h));
+    }
   }
-  const bool bad = x != x || y != y;
-  double total = bad ? 0.0 : double(log2_sigmoid(x));
+  // By one wave, a lane a token.  The sums are float64: differences of far tokens'
+  // logarithms keep their bits.
+  __device__ __forceinline__ void put(Gates& g) const {
+    const int lane = threadIdx.x & 63;
+    const bool bad = gate != gate || beta != beta;
+    double total = bad ? 0.0 : double(log2_sigmoid(gate));
 #pragma unroll
-  for (int d = 1; d < kChunk; d <<= 1) {
-    const double before = __shfl_up(total, d, kChunk);
-    if (lane >= d) total += before;
+    for (int d = 1; d < kChunk; d <<= 1) {
+      const double before = __shfl_up(total, d, kChunk);
+      if (lane >= d) total += before;
+    }
+    const double last = __shfl(total, kChunk - 1, kChunk);
+    g.beta[lane] = bad ? 0.0f : sigmoid(beta);
+    g.hi[lane] = float(total);
+    g.lo[lane] = float(total - double(float(total)));
+    g.up[lane] = __builtin_amdgcn_exp2f(float(total));
+    g.down[lane] = __builtin_amdgcn_exp2f(float(last - total));
+    g.fade[lane] = sigmoid(-gate);
+    g.rest[lane] = sigmoid(-beta);
+    const uint64_t marks = __ballot(bad);
+    if (lane == 0) {
+      g.whole = __builtin_amdgcn_exp2f(float(last));
+      g.bad = marks ? __builtin_ctzll(marks) : kChunk;
+    }
   }
-  const double last = __shfl(total, kChunk - 1, kChunk);
-  g.beta[lane] = bad ? 0.0f : sigmoid(y);
-  g.hi[lane] = float(total);
-  g.lo[lane] = float(total - double(float(total)));
-  g.up[lane] = __builtin_amdgcn_exp2f(float(total));
-  g.down[lane] = __builtin_amdgcn_exp2f(float(last - total));
-  const uint64_t marks = __ballot(bad);
-  if (lane == 0) {
-    g.whole = __builtin_amdgcn_exp2f(float(last));
-    g.bad = marks ? __builtin_ctzll(marks) : kChunk;
-  }
-}
+};
 
 // What is kept between the kernels, one after the other for each chunk of each
-// head; widths padded to kKey and kDim.
+// head; widths padded to kKey and kDim.  A column lies together: the chain's lanes
+// have one, with consecutive rows in their registers.
+// What products take in one bfloat16 part is kept so (Form's Store).
 struct Kept {
-  float* starts;   // [kKey, kDim]: the state before the chunk
-  float* updates;  // [64, kDim]: F, then U
-  float* solve;    // [64, 64]: T, or null
+  float* solve;   // [64, 64]: T, or null; its upper right quarter is not written
+  void* starts;   // [kDim, kKey]: the state before the chunk, turned
+  void* updates;  // [kDim, 64]: U, turned
 };
+
+// Where four elements of a row, from column `col` on, lie in a first operand of 16 x 16
+// results: fragments of 16 rows and 32 columns, `steps` of them beside each other,
+// each in the order of the lanes, whose group g has columns 4 g .. + 3 and 16 + 4 g ..
+// + 3 of it.
+__device__ __forceinline__ int fragment_at(int row, int col, int steps) {
+  return ((row >> 4) * steps + (col >> 5)) * 512 + ((row & 15) + 16 * ((col & 15) >> 2)) * 8 +
+         ((col & 16) >> 2);
+}
 
 // Factors of the chain, a chunk of a head each.
 struct Chain {
-  bf16* left;      // parts of [64, kKey]
-  bf16* right;     // parts of [kKey, 64]
+  bf16* left;      // parts of [64, kKey], in fragments
+  bf16* right;     // parts of [kKey, 64], in fragments
   float* factors;  // 64 of e^(G_C - G), then e^(G_C) and the first token that is not finite
 };
 constexpr int kFactors = kChunk + 4;
@@ -295,11 +377,20 @@ struct ChainArgs {
   int chunks, key_dim, dim;
   Chain chain;
   const float* first;  // the state before the first chunk [heads, key_dim, dim], or null
-  float* rows;         // [64, kDim] a chunk: what the rows start with, then the rows
-  float* states;       // [kKey, kDim] a chunk: what the next state starts with
-                       // (backward), then the state before the chunk
+  int group;                 // heads that share keys
+  const float* rows_from;    // [kDim, 64] a chunk: what the rows start with
+  void* rows;                // the rows, float32 or (forward) Form's Store; may be rows_from
+  const float* states_from;  // [kDim, kKey] a chunk: what the next state starts with (backward)
+  void* states;              // the state before the chunk, Form's Store; may be states_from
   float* last;         // the state behind the last chunk, or null
+  // Cut sequences: what each segment maps a state to, in fragments, and what it adds
+  // [kDim, kKey].
+  int segments;
+  bf16* maps;
+  float* adds;
+  int each, blocks;  // chunks of a segment, blocks of columns (the launch's)
 };
+int chain_segments(int64_t heads, int64_t chunks, int dim);
 int launch_chain(const ChainArgs& a, int key_wide, int wide, int parts_in, bool backward,
                  hipStream_t s);
 

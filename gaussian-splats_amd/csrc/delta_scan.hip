@@ -22,9 +22,13 @@ struct ForwardArgs {
   Problem p;
   Rows<T> q, k, v, gate, beta;
   Kept kept;
+  float* free;  // [kDim, 64] a chunk: F turned
   Chain chain;
   T* out;
   int64_t count;  // chunks of all heads
+  int segments;   // of the chain, with its scratch
+  bf16* maps;
+  float* adds;
 };
 
 constexpr int kPitchA = kChunk + 4;
@@ -70,10 +74,10 @@ __device__ __forceinline__ void solve_triangle(const float* a, float* t) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) t[(block + 2 * i + (c >> 4)) * kPitchA + block + 16 + (c & 15)] = 0.0f;
   }
-  __syncthreads();
+  lds_barrier();
   for (int d = 1; d < 4; ++d) {
     if (wave < 4 - d) solve_block(a, t, d + wave, wave);
-    __syncthreads();
+    lds_barrier();
   }
 }
 
@@ -106,8 +110,13 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(ForwardArgs<T> 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const KTile k(k_space);
   const VTile v(v_space);
-  if (wave == 0) load_gates(g, a.gate, a.beta, at);
-  __syncthreads();
+  const GatePair gates(a.gate, a.beta, at);
+  Fetch<T, kChunk, kKey> k_in;
+  Fetch<T, kChunk, kDim> v_in;
+  k_in.load(a.k.at(at.b, at.t0, at.key_head), a.k.s.token, at.valid, a.p.key_dim);
+  v_in.load(a.v.at(at.b, at.t0, at.h), a.v.s.token, at.valid, a.p.dim);
+  if (wave == 0) gates.put(g);
+  lds_barrier();
   const auto mark = [&](int row, int, auto& x) {
     bool bad = false;
 #pragma unroll
@@ -117,13 +126,13 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(ForwardArgs<T> 
       atomicMin(&g.bad, row);
     }
   };
-  load_tile<T>(k, a.k.at(at.b, at.t0, at.key_head), a.k.s.token, at.valid, a.p.key_dim, mark);
-  load_tile<T>(v, a.v.at(at.b, at.t0, at.h), a.v.s.token, at.valid, a.p.dim, mark);
+  k_in.put(k, mark);
+  v_in.put(v, mark);
   if (threadIdx.x < kChunk) {
     by_value[threadIdx.x] = g.beta[threadIdx.x];
     by_key[threadIdx.x] = -g.beta[threadIdx.x] * g.up[threadIdx.x];
   }
-  __syncthreads();
+  lds_barrier();
   // A: a wave each for the blocks of 32 on and below the diagonal; a lane has a row
   // i and the columns of its registers.
   if (wave < 3) {
@@ -142,58 +151,69 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(ForwardArgs<T> 
       *reinterpret_cast<FloatVec<4>*>(system + i * kPitchA + j) = x;
     }
   }
-  __syncthreads();
+  lds_barrier();
   solve_triangle(system, solve);
   if (a.kept.solve) {
     float* to = a.kept.solve + index * kChunk * kChunk;
 #pragma unroll
     for (int s = 0; s < kChunk * kChunk / 4 / kThreads; ++s) {
       const int e = (s * kThreads + int(threadIdx.x)) * 4, row = e / kChunk, col = e % kChunk;
-      FloatVec<4> x = *reinterpret_cast<const FloatVec<4>*>(solve + row * kPitchA + col);
-      if (row < 32 && col >= 32) x = FloatVec<4>(0.0f);
-      *reinterpret_cast<FloatVec<4>*>(to + e) = x;
+      if (row >= 32 || col < 32)
+        *reinterpret_cast<FloatVec<4>*>(to + e) = *reinterpret_cast<const FloatVec<4>*>(solve + row * kPitchA + col);
     }
   }
-  // -W and F, turned: a lane has a token and consecutive columns in its registers.
-  const int m0 = 32 * (wave & 1), token = m0 + (lane & 31), steps = m0 ? 4 : 2;
+  // -W: a lane has a token and consecutive columns in its registers.
+  const int m0 = 32 * (wave & 1), token = m0 + (lane & 31);
   bf16* left = a.chain.left + index * M::chain * kChunk * kKey;
 #pragma unroll
   for (int t = 0; t < kKey / 64; ++t) {
     const int n0 = 32 * ((wave >> 1) + 2 * t);
     Acc c(0.0f);
-    for (int s = 0; s < steps; ++s)
+    steps_to(m0, [&](int s) {
       mma_parts(k.cols(16 * s, n0), solve_rows<E, M::mid>(solve, m0, 16 * s, by_key), c);
+    });
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       const Parts<bf16, M::chain, 4> x(four(c, s));
 #pragma unroll
       for (int i = 0; i < M::chain; ++i)
-        *reinterpret_cast<Vec<bf16, 4>*>(left + (i * kChunk + token) * kKey + n0 + four_row(s)) = x.v[i];
+        *reinterpret_cast<Vec<bf16, 4>*>(left + i * kChunk * kKey +
+                                         fragment_at(token, n0 + four_row(s), kKey / 32)) = x.v[i];
     }
   }
-  float* rows = a.kept.updates + index * kChunk * kDim;
+  // F turned: a lane has a column and consecutive tokens.
+  float* rows = a.free + index * kChunk * kDim;
 #pragma unroll
   for (int t = 0; t < kDim / 64; ++t) {
     const int n0 = 32 * ((wave >> 1) + 2 * t);
     Acc c(0.0f);
-    for (int s = 0; s < steps; ++s)
-      mma_parts(v.cols(16 * s, n0), solve_rows<E, M::mid>(solve, m0, 16 * s, by_value), c);
+    steps_to(m0, [&](int s) {
+      mma_parts(solve_rows<E, M::mid>(solve, m0, 16 * s, by_value), v.cols(16 * s, n0), c);
+    });
 #pragma unroll
     for (int s = 0; s < 4; ++s)
-      *reinterpret_cast<FloatVec<4>*>(rows + token * kDim + n0 + four_row(s)) = four(c, s);
+      *reinterpret_cast<FloatVec<4>*>(rows + (n0 + (lane & 31)) * kChunk + m0 + four_row(s)) = four(c, s);
   }
-  // K turned.
-  bf16* right = a.chain.right + index * M::chain_in * kKey * kChunk;
-  for (int e = wave; e < kKey / 32 * 4; e += 4) {
+  // K turned, once for the heads that share it.
+  const int group = a.p.heads / a.p.key_heads;
+  bf16* right = a.chain.right + ((int64_t(at.b) * a.p.key_heads + at.key_head) * a.p.chunks + at.c) *
+                                    M::chain_in * kKey * kChunk;
+  for (int e = at.h % group ? kKey : wave; e < kKey / 32 * 4; e += 4) {
     const int n0 = 32 * (e / 4), t0 = 16 * (e % 4);
     FloatVec<8> x(0.0f);
     const Parts<E, M::in, 8> f = k.cols(t0, n0);
 #pragma unroll
     for (int i = 0; i < M::in; ++i) x += to_float<E, 8>(f.v[i]);
     const Parts<bf16, M::chain_in, 8> y(x);
+    const int row = n0 + (lane & 31), col = t0 + 8 * (lane >> 5);
 #pragma unroll
-    for (int i = 0; i < M::chain_in; ++i)
-      *reinterpret_cast<Frag<bf16>*>(right + (i * kKey + n0 + (lane & 31)) * kChunk + t0 + 8 * (lane >> 5)) = y.v[i];
+    for (int i = 0; i < M::chain_in; ++i) {
+      bf16* to = right + i * kKey * kChunk;
+      *reinterpret_cast<Vec<bf16, 4>*>(to + fragment_at(row, col, 2)) =
+          __builtin_shufflevector(y.v[i], y.v[i], 0, 1, 2, 3);
+      *reinterpret_cast<Vec<bf16, 4>*>(to + fragment_at(row, col + 4, 2)) =
+          __builtin_shufflevector(y.v[i], y.v[i], 4, 5, 6, 7);
+    }
   }
   float* factors = a.chain.factors + index * kFactors;
   if (threadIdx.x < kChunk) factors[threadIdx.x] = g.down[threadIdx.x];
@@ -209,8 +229,8 @@ __global__ __launch_bounds__(kThreads) void delta_output_kernel(ForwardArgs<T> a
   using M = Form<T>;
   using E = typename M::Elem;
   using KTile = Tile<E, M::in, kChunk, kKey>;
-  using STile = Tile<E, M::out, kKey, 64>;
-  using UTile = Tile<E, M::out, kChunk, 64>;
+  using STile = Tile<E, M::out, 64, kKey>;  // 64 columns of the state, turned
+  using UTile = Tile<E, M::out, 64, kChunk>;
   using PTile = Tile<E, M::out, kChunk, kChunk>;
   constexpr int kShared = KTile::bytes > STile::bytes ? KTile::bytes : STile::bytes;
   __shared__ __align__(16) char q_space[KTile::bytes], k_space[kShared];
@@ -224,14 +244,28 @@ __global__ __launch_bounds__(kThreads) void delta_output_kernel(ForwardArgs<T> a
   const STile state(k_space);
   const UTile u(u_space);
   const PTile p(p_space);
-  if (wave == 0) load_gates(g, a.gate, a.beta, at);
-  load_tile<T>(q, a.q.at(at.b, at.t0, at.key_head), a.q.s.token, at.valid, a.p.key_dim, Keep{});
-  load_tile<T>(k, a.k.at(at.b, at.t0, at.key_head), a.k.s.token, at.valid, a.p.key_dim,
-               [](int, int, auto& x) {
+  const GatePair gates(a.gate, a.beta, at);
+  using Store = typename M::Store;
+  const Store* starts = static_cast<const Store*>(a.kept.starts) + index * kKey * kDim;
+  const Store* updates = static_cast<const Store*>(a.kept.updates) + index * kChunk * kDim;
+  Fetch<T, kChunk, kKey> q_in, k_in;
+  Fetch<Store, 64, kKey> state_in;
+  Fetch<Store, 64, kChunk> u_in;
+  const auto fetch = [&](int d0) {
+    state_in.load(starts + d0 * kKey, kKey, a.p.dim - d0, a.p.key_dim);
+    u_in.load(updates + d0 * kChunk, kChunk, a.p.dim - d0, kChunk);
+  };
+  q_in.load(a.q.at(at.b, at.t0, at.key_head), a.q.s.token, at.valid, a.p.key_dim);
+  k_in.load(a.k.at(at.b, at.t0, at.key_head), a.k.s.token, at.valid, a.p.key_dim);
+  fetch(0);
+  if (wave == 0) gates.put(g);
+  q_in.put(q);
+  k_in.put(k, [](int, int, auto& x) {
 #pragma unroll
-                 for (int i = 0; i < 8; ++i) x[i] = finite(float(x[i])) ? x[i] : decltype(x[i] + x[i])(0.0f);
-               });
-  __syncthreads();
+    for (int i = 0; i < 8; ++i) x[i] = finite(float(x[i])) ? x[i] : decltype(x[i] + x[i])(0.0f);
+  });
+  u_in.put(u);
+  lds_barrier();
   // P = scale Q K^T * D.
   {
     const int i0 = wave ? 32 : 0, j0 = wave == 2 ? 32 : 0;
@@ -250,24 +284,23 @@ __global__ __launch_bounds__(kThreads) void delta_output_kernel(ForwardArgs<T> a
       if (wave < 3) p.put(i, j, Parts<E, M::out, 4>(x));
     }
   }
-  const int m0 = 32 * (wave & 1), token = m0 + (lane & 31), n0 = 32 * (wave >> 1), steps = m0 ? 4 : 2;
+  const int m0 = 32 * (wave & 1), token = m0 + (lane & 31), n0 = 32 * (wave >> 1);
   const float up = a.p.scale * g.up[token];
   const bool bad = token >= int(a.chain.factors[index * kFactors + kChunk + 1]);
-  const float* starts = a.kept.starts + index * kKey * kDim;
-  const float* updates = a.kept.updates + index * kChunk * kDim;
   T* out = a.out + ((int64_t(at.b) * a.p.tokens + at.t0 + token) * a.p.heads + at.h) * a.p.dim;
 #pragma unroll
   for (int d0 = 0; d0 < kDim; d0 += 64) {
     if (d0 >= a.p.dim) break;
-    __syncthreads();
-    load_tile<float>(state, starts + d0, kDim, a.p.key_dim, a.p.dim - d0, Keep{});
-    load_tile<float>(u, updates + d0, kDim, kChunk, a.p.dim - d0, Keep{});
-    __syncthreads();
+    lds_barrier();
+    state_in.put(state);
+    if (d0) u_in.put(u);
+    if (d0 + 64 < a.p.dim) fetch(d0 + 64);
+    lds_barrier();
     Acc c(0.0f);
 #pragma unroll
-    for (int s = 0; s < kKey / 16; ++s) mma_parts(state.cols(16 * s, n0), q.rows(m0, 16 * s), c);
+    for (int s = 0; s < kKey / 16; ++s) mma_parts(state.rows(n0, 16 * s), q.rows(m0, 16 * s), c);
     c *= up;
-    for (int s = 0; s < steps; ++s) mma_parts(u.cols(16 * s, n0), p.rows(m0, 16 * s), c);
+    steps_to(m0, [&](int s) { mma_parts(u.rows(n0, 16 * s), p.rows(m0, 16 * s), c); });
     if (token < at.rows) {
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
@@ -287,7 +320,8 @@ int forward(const ForwardArgs<T>& a, const float* state, float* last, hipStream_
   delta_prepare_kernel<T, kKey, kDim><<<grid, kThreads, 0, s>>>(a);
   GS_TRY(check_launch("delta_scan prepare"));
   ChainArgs chain{int64_t(a.p.batch) * a.p.heads, a.p.chunks, a.p.key_dim, a.p.dim, a.chain, state,
-                  a.kept.updates, a.kept.starts, last};
+                  a.p.heads / a.p.key_heads, a.free, a.kept.updates, nullptr, a.kept.starts, last,
+                  a.segments, a.maps, a.adds, 0, 0};
   GS_TRY(launch_chain(chain, kKey, kDim, Form<T>::chain_in, false, s));
   delta_output_kernel<T, kKey, kDim><<<grid, kThreads, 0, s>>>(a);
   return check_launch("delta_scan output");
@@ -334,13 +368,28 @@ delta::Problem delta_problem(const gs_delta& d, const int32_t* lengths) {
           int((d.tokens + delta::kChunk - 1) / delta::kChunk), d.scale, lengths};
 }
 
-delta::Kept delta_kept(const gs_delta& d, float* kept, bool solve) {
+// Bytes of an element of what is kept for one product (Form's Store).
+size_t delta_store_bytes(const gs_delta& d) { return d.type == GS_BF16 ? 2 : 4; }
+
+delta::Kept delta_kept(const gs_delta& d, void* kept, bool solve) {
   const int64_t n = delta_chunks(d), wide = delta::padded(d.dim);
+  char* at = static_cast<char*>(kept);
   delta::Kept k;
-  k.starts = kept;
-  k.updates = k.starts + n * delta::padded(d.key_dim) * wide;
-  k.solve = solve ? k.updates + n * delta::kChunk * wide : nullptr;
+  k.solve = solve ? reinterpret_cast<float*>(at) : nullptr;
+  if (solve) at += n * delta::kChunk * delta::kChunk * sizeof(float);
+  k.starts = at;
+  k.updates = at + n * delta::padded(d.key_dim) * wide * delta_store_bytes(d);
   return k;
+}
+
+// Scratch of a chain in segments.
+size_t delta_segment_bytes(const gs_delta& d) {
+  const int64_t chunks = (d.tokens + delta::kChunk - 1) / delta::kChunk;
+  const int n = delta::chain_segments(d.batch * d.heads, chunks, d.dim);
+  const size_t key = delta::padded(d.key_dim), parts = d.type == GS_F32 ? 3 : 2;
+  return n == 1 ? 0
+                : size_t(n) * d.batch * d.heads *
+                      (key * delta::padded(d.dim) * sizeof(float) + parts * key * key * sizeof(uint16_t));
 }
 
 // Parts in the chain of an input and of another factor.
@@ -364,15 +413,17 @@ using namespace gs;
 extern "C" GS_API size_t gs_delta_scan_kept_bytes(const gs_delta* desc, int32_t backward) {
   if (!desc || check_delta(*desc) != GS_OK) return 0;
   const size_t wide = delta::padded(desc->dim);
-  const size_t a_chunk = delta::padded(desc->key_dim) * wide + delta::kChunk * wide +
-                         (backward ? delta::kChunk * delta::kChunk : 0);
-  return size_t(delta_chunks(*desc)) * a_chunk * sizeof(float);
+  const size_t a_chunk = (delta::padded(desc->key_dim) + delta::kChunk) * wide * delta_store_bytes(*desc) +
+                         (backward ? delta::kChunk * delta::kChunk * sizeof(float) : 0);
+  return size_t(delta_chunks(*desc)) * a_chunk;
 }
 
 extern "C" GS_API size_t gs_delta_scan_workspace_bytes(const gs_delta* desc) {
   if (!desc || check_delta(*desc) != GS_OK) return 0;
-  return size_t(delta_chunks(*desc)) *
-         (delta_left_bytes(*desc, delta_parts_in(*desc) + delta_parts_mid(*desc)) + delta::kFactors * sizeof(float));
+  return delta_segment_bytes(*desc) +
+         size_t(delta_chunks(*desc)) *
+             (delta_left_bytes(*desc, delta_parts_in(*desc) + delta_parts_mid(*desc)) +
+              (delta::kFactors + delta::kChunk * delta::padded(desc->dim)) * sizeof(float));
 }
 
 extern "C" GS_API int gs_delta_scan_fwd(const gs_delta* desc, const void* q, const void* k,
@@ -406,12 +457,17 @@ extern "C" GS_API int gs_delta_scan_fwd(const gs_delta* desc, const void* q, con
     a.v = rows(v, 2);
     a.gate = rows(gate, 3);
     a.beta = rows(beta, 4);
-    a.kept = delta_kept(*desc, static_cast<float*>(kept), backward);
+    a.kept = delta_kept(*desc, kept, backward);
     a.chain.factors = static_cast<float*>(workspace);
-    a.chain.left = reinterpret_cast<delta::bf16*>(a.chain.factors + n * delta::kFactors);
+    a.free = a.chain.factors + n * delta::kFactors;
+    a.chain.left = reinterpret_cast<delta::bf16*>(a.free + n * delta::kChunk * delta::padded(desc->dim));
     a.chain.right = a.chain.left + n * delta_left_bytes(*desc, delta_parts_mid(*desc)) / 2;
     a.out = static_cast<T*>(out);
     a.count = n;
+    a.segments = delta::chain_segments(desc->batch * desc->heads, a.p.chunks, desc->dim);
+    a.adds = reinterpret_cast<float*>(a.chain.right + n * delta_left_bytes(*desc, delta_parts_in(*desc)) / 2);
+    a.maps = reinterpret_cast<delta::bf16*>(a.adds + int64_t(a.segments) * desc->batch * desc->heads *
+                                                         delta::padded(desc->key_dim) * delta::padded(desc->dim));
     const hipStream_t s = as_stream(stream);
     // Heads of up to 64 have tiles of their own.
     if (desc->key_dim <= 64)

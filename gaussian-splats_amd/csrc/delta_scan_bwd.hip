@@ -35,9 +35,11 @@ int check_delta_rows(const void* p, const int64_t* strides, int32_t type, const 
 int64_t delta_chunks(const gs_delta& d);
 size_t delta_left_bytes(const gs_delta& d, int parts);
 delta::Problem delta_problem(const gs_delta& d, const int32_t* lengths);
-delta::Kept delta_kept(const gs_delta& d, float* kept, bool solve);
+size_t delta_store_bytes(const gs_delta& d);
+delta::Kept delta_kept(const gs_delta& d, void* kept, bool solve);
 int delta_parts_in(const gs_delta& d);
 int delta_parts_mid(const gs_delta& d);
+size_t delta_segment_bytes(const gs_delta& d);
 
 namespace delta {
 namespace {
@@ -48,14 +50,18 @@ struct BackwardArgs {
   Rows<T> q, k, v, gate, beta, grad;  // grad.p may be null
   Kept kept;
   Chain chain;
-  float* du;    // [64, kDim] a chunk
-  float* ends;  // [kKey, kDim] a chunk: dS behind it
+  float* du;      // [kDim, 64] a chunk
+  float* begins;  // [kDim, kKey] a chunk: scale Q^T e^G dO
+  void* ends;     // [kDim, kKey] a chunk, Form's Store: dS behind it; may be begins
   T* dq;
   T* dk;
   T* dv;
   T* dgate;
   T* dbeta;
   int64_t count;
+  int segments;
+  bf16* maps;
+  float* adds;
 };
 
 constexpr int kPitchA = kChunk + 4;
@@ -82,20 +88,20 @@ __global__ __launch_bounds__(kThreads) void delta_back_prepare_kernel(BackwardAr
   const OTile grad(o_space);
   const PTile p(p_space);
   const T* q_rows = a.q.at(at.b, at.t0, at.key_head);
-  if (wave == 0) load_gates(g, a.gate, a.beta, at);
-  load_tile<T>(k, a.k.at(at.b, at.t0, at.key_head), a.k.s.token, at.valid, a.p.key_dim, Keep{});
-  load_tile<T>(q, q_rows, a.q.s.token, at.valid, a.p.key_dim, Keep{});
-  load_tile<T>(grad, a.grad.at(at.b, at.t0, at.h), a.grad.s.token, a.grad.p ? at.valid : 0, a.p.dim, Keep{});
-  {
-    const float* from = a.kept.solve + index * kChunk * kChunk;
-#pragma unroll
-    for (int s = 0; s < kChunk * kChunk / 4 / kThreads; ++s) {
-      const int e = (s * kThreads + int(threadIdx.x)) * 4;
-      *reinterpret_cast<FloatVec<4>*>(solve + e / kChunk * kPitchA + e % kChunk) =
-          *reinterpret_cast<const FloatVec<4>*>(from + e);
-    }
-  }
-  __syncthreads();
+  const GatePair gates(a.gate, a.beta, at);
+  Fetch<T, kChunk, kKey> k_in, q_in;
+  Fetch<T, kChunk, kDim> grad_in;
+  Fetch<float, kChunk, kChunk> solve_in;
+  k_in.load(a.k.at(at.b, at.t0, at.key_head), a.k.s.token, at.valid, a.p.key_dim);
+  q_in.load(q_rows, a.q.s.token, at.valid, a.p.key_dim);
+  grad_in.load(a.grad.at(at.b, at.t0, at.h), a.grad.s.token, a.grad.p ? at.valid : 0, a.p.dim);
+  solve_in.load_triangle(a.kept.solve + index * kChunk * kChunk);
+  if (wave == 0) gates.put(g);
+  k_in.put(k);
+  q_in.put(q);
+  grad_in.put(grad);
+  solve_in.put(Tile<float, 1, kChunk, kChunk>(reinterpret_cast<char*>(solve)));
+  lds_barrier();
   if (threadIdx.x < kChunk) by_key[threadIdx.x] = -g.beta[threadIdx.x] * g.up[threadIdx.x];
   if (wave < 3) {
     const int i0 = wave ? 32 : 0, j0 = wave == 2 ? 32 : 0, i = i0 + (lane & 31);
@@ -111,7 +117,7 @@ __global__ __launch_bounds__(kThreads) void delta_back_prepare_kernel(BackwardAr
       p.put(i, j, Parts<E, F::mid, 4>(x));
     }
   }
-  __syncthreads();
+  lds_barrier();
   const int m0 = 32 * (wave & 1), token = m0 + (lane & 31);
   // -W turned: a lane has a dimension and consecutive tokens.
   bf16* right = a.chain.right + index * F::chain * kKey * kChunk;
@@ -119,33 +125,43 @@ __global__ __launch_bounds__(kThreads) void delta_back_prepare_kernel(BackwardAr
   for (int t = 0; t < kKey / 64; ++t) {
     const int n0 = 32 * ((wave >> 1) + 2 * t);
     Acc c(0.0f);
-    for (int s = 0; s < (m0 ? 4 : 2); ++s) {
+    steps_to(m0, [&](int s) {
       const int kk = 16 * s + 8 * (lane >> 5);
       const float* row = solve + token * kPitchA + kk;
       FloatVec<8> x;
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = row[i] * by_key[kk + i];
       mma_parts(Parts<E, F::mid, 8>(x), k.cols(16 * s, n0), c);
-    }
+    });
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       const Parts<bf16, F::chain, 4> x(four(c, s));
 #pragma unroll
       for (int i = 0; i < F::chain; ++i)
-        *reinterpret_cast<Vec<bf16, 4>*>(right + (i * kKey + n0 + (lane & 31)) * kChunk + m0 + four_row(s)) = x.v[i];
+        *reinterpret_cast<Vec<bf16, 4>*>(right + i * kKey * kChunk +
+                                         fragment_at(n0 + (lane & 31), m0 + four_row(s), 2)) = x.v[i];
     }
   }
-  bf16* left = a.chain.left + index * F::chain_in * kChunk * kKey;
-  for (int e = wave; e < 2 * (kKey / 16); e += 4) {
+  // K, once for the heads that share it.
+  const int group = a.p.heads / a.p.key_heads;
+  bf16* left = a.chain.left + ((int64_t(at.b) * a.p.key_heads + at.key_head) * a.p.chunks + at.c) *
+                                  F::chain_in * kChunk * kKey;
+  for (int e = at.h % group ? kKey : wave; e < 2 * (kKey / 16); e += 4) {
     const int row0 = 32 * (e & 1), k0 = 16 * (e >> 1);
     FloatVec<8> x(0.0f);
     const Parts<E, F::in, 8> f = k.rows(row0, k0);
 #pragma unroll
     for (int i = 0; i < F::in; ++i) x += to_float<E, 8>(f.v[i]);
     const Parts<bf16, F::chain_in, 8> y(x);
+    const int row = row0 + (lane & 31), col = k0 + 8 * (lane >> 5);
 #pragma unroll
-    for (int i = 0; i < F::chain_in; ++i)
-      *reinterpret_cast<Frag<bf16>*>(left + (i * kChunk + row0 + (lane & 31)) * kKey + k0 + 8 * (lane >> 5)) = y.v[i];
+    for (int i = 0; i < F::chain_in; ++i) {
+      bf16* to = left + i * kChunk * kKey;
+      *reinterpret_cast<Vec<bf16, 4>*>(to + fragment_at(row, col, kKey / 32)) =
+          __builtin_shufflevector(y.v[i], y.v[i], 0, 1, 2, 3);
+      *reinterpret_cast<Vec<bf16, 4>*>(to + fragment_at(row, col + 4, kKey / 32)) =
+          __builtin_shufflevector(y.v[i], y.v[i], 4, 5, 6, 7);
+    }
   }
   // P^T dO.
   float* du = a.du + index * kChunk * kDim;
@@ -153,25 +169,24 @@ __global__ __launch_bounds__(kThreads) void delta_back_prepare_kernel(BackwardAr
   for (int t = 0; t < kDim / 64; ++t) {
     const int n0 = 32 * ((wave >> 1) + 2 * t);
     Acc c(0.0f);
-    for (int s = m0 / 16; s < 4; ++s) mma_parts(grad.cols(16 * s, n0), p.cols(16 * s, m0), c);
+    steps_from(m0, [&](int s) { mma_parts(p.cols(16 * s, m0), grad.cols(16 * s, n0), c); });
 #pragma unroll
     for (int s = 0; s < 4; ++s)
-      *reinterpret_cast<FloatVec<4>*>(du + token * kDim + n0 + four_row(s)) = four(c, s);
+      *reinterpret_cast<FloatVec<4>*>(du + (n0 + (lane & 31)) * kChunk + m0 + four_row(s)) = four(c, s);
   }
-  __syncthreads();
-  load_tile<T>(q_up, q_rows, a.q.s.token, at.valid, a.p.key_dim,
-               [&](int row, int, auto& x) { x = x * (a.p.scale * g.up[row]); });
-  __syncthreads();
+  lds_barrier();
+  q_in.put(q_up, [&](int row, int, auto& x) { x = x * (a.p.scale * g.up[row]); });
+  lds_barrier();
   // scale Q^T e^G dO.
-  float* ends = a.ends + index * kKey * kDim;
+  float* begins = a.begins + index * kKey * kDim;
   for (int e = wave; e < kKey / 32 * (kDim / 32); e += 4) {
     const int k0 = 32 * (e / (kDim / 32)), n0 = 32 * (e % (kDim / 32));
     Acc c(0.0f);
 #pragma unroll
-    for (int s = 0; s < 4; ++s) mma_parts(grad.cols(16 * s, n0), q_up.cols(16 * s, k0), c);
+    for (int s = 0; s < 4; ++s) mma_parts(q_up.cols(16 * s, k0), grad.cols(16 * s, n0), c);
 #pragma unroll
     for (int s = 0; s < 4; ++s)
-      *reinterpret_cast<FloatVec<4>*>(ends + (k0 + (lane & 31)) * kDim + n0 + four_row(s)) = four(c, s);
+      *reinterpret_cast<FloatVec<4>*>(begins + (n0 + (lane & 31)) * kKey + k0 + four_row(s)) = four(c, s);
   }
   float* factors = a.chain.factors + index * kFactors;
   if (threadIdx.x < kChunk) factors[threadIdx.x] = g.down[threadIdx.x];
@@ -179,22 +194,23 @@ __global__ __launch_bounds__(kThreads) void delta_back_prepare_kernel(BackwardAr
 }
 
 // Sums of a result's columns, over the 32 lanes of a half: each lane with bit 4 clear
-// gets that of one register, sums_register().
-__device__ __forceinline__ float column_sums(const Acc& c) {
-  const int lane = threadIdx.x & 63;
-  float e[16];
+// gets that of one register, sums_register().  A step adds what the lane's neighbour
+// gives of its half of the registers, and halves them.
+template <int N>
+__device__ __forceinline__ float column_sums(const FloatVec<2 * N>& c) {
+  constexpr int kFar = 8 / N;
+  const bool high = (threadIdx.x & 63) & kFar;
+  FloatVec<N> sums;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) e[i] = c[i];
-#pragma unroll
-  for (int d = 1, n = 8; n; d <<= 1, n >>= 1) {
-    const bool high = lane & d;
-#pragma unroll
-    for (int i = 0; i < n; ++i) {
-      const float send = high ? e[i] : e[i + n], keep = high ? e[i + n] : e[i];
-      e[i] = keep + __shfl_xor(send, d, kWave);
-    }
+  for (int i = 0; i < N; ++i) {
+    float low = c[i], up = c[i + N];
+    asm volatile("" : "+v"(low), "+v"(up));  // or the choice becomes a search by index
+    sums[i] = (high ? up : low) + __shfl_xor(high ? low : up, kFar, kWave);
   }
-  return e[0] + __shfl_xor(e[0], 16, kWave);
+  if constexpr (N == 1)
+    return sums[0] + __shfl_xor(sums[0], 16, kWave);
+  else
+    return column_sums<N / 2>(sums);
 }
 __device__ __forceinline__ int sums_register() {
   const int lane = threadIdx.x;
@@ -209,19 +225,19 @@ __global__ __launch_bounds__(kThreads, (kKey == 64 && std::is_same_v<T, bf16> ? 
   constexpr int P = F::out;
   static_assert(P == F::in, "inputs and results have the same parts here");
   using Half = Tile<E, P, kChunk, 64>;   // half of a value's dimensions
-  using STile = Tile<E, P, kKey, 64>;
+  using STile = Tile<E, P, 64, kKey>;  // 64 columns of a state, turned
   using KTile = Tile<E, P, kChunk, kKey>;
   using Fine = Tile<E, F::mid, kChunk, 64>;
   constexpr int kFirst = 2 * Half::bytes + 2 * Fine::bytes + STile::bytes;
-  constexpr int kSecond = 3 * Half::bytes + 2 * KTile::bytes;
+  constexpr int kSecond = 2 * Half::bytes + 2 * KTile::bytes;
   __shared__ __align__(16) char space[kFirst > kSecond ? kFirst : kSecond];
   __shared__ Gates g;
   __shared__ float dots[3][2][kChunk], crossing[2][3][32], inner[4];
   const Half grad(space), u(space + Half::bytes), x(space + 2 * Half::bytes);
   const Fine du(space + 2 * Half::bytes), solve(space + 2 * Half::bytes + Fine::bytes);
   const STile state(space + 2 * Half::bytes + 2 * Fine::bytes);
-  const Half n_tile(space), m_tile(space + Half::bytes), mb_tile(space + 2 * Half::bytes);
-  const KTile q(space + 3 * Half::bytes), k(space + 3 * Half::bytes + KTile::bytes);
+  const Half n_tile(space), m_tile(space + Half::bytes);
+  const KTile q(space + 2 * Half::bytes), k(space + 2 * Half::bytes + KTile::bytes);
   constexpr int kTiles = kKey / 64;
   const int64_t work = seq::block_index();
   const int group = a.p.heads / a.p.key_heads;
@@ -231,36 +247,59 @@ __global__ __launch_bounds__(kThreads, (kKey == 64 && std::is_same_v<T, bf16> ? 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int m0 = 32 * (wave & 1), side = wave >> 1, token = m0 + (lane & 31);
   const int i0 = wave ? 32 : 0, j0 = wave == 2 ? 32 : 0;  // of the triangles, waves 0 .. 2
+  Fetch<T, kChunk, 64> grad_in;
+  using Store = typename F::Store;
+  Fetch<Store, 64, kChunk> u_in;
+  Fetch<float, 64, kChunk> du_in;
+  Fetch<float, kChunk, kChunk> solve_in;
+  Fetch<Store, 64, kKey> state_in, end_in;
+  Fetch<T, kChunk, kKey> q_in, k_in;
+  const auto fetch_half = [&](const Place& at, int d0) {
+    const int64_t base = at.id * kDim + d0;
+    const int wide = a.p.dim - d0;
+    grad_in.load(a.grad.at(at.b, at.t0, at.h) + d0, a.grad.s.token, a.grad.p ? at.valid : 0, wide);
+    u_in.load(static_cast<const Store*>(a.kept.updates) + base * kChunk, kChunk, wide, kChunk);
+    du_in.load(a.du + base * kChunk, kChunk, wide, kChunk);
+    state_in.load(static_cast<const Store*>(a.kept.starts) + base * kKey, kKey, wide, a.p.key_dim);
+    end_in.load(static_cast<const Store*>(a.ends) + base * kKey, kKey, wide, a.p.key_dim);
+  };
   Acc dq_all[kTiles], dk_all[kTiles];
 #pragma unroll
   for (int t = 0; t < kTiles; ++t) dq_all[t] = dk_all[t] = Acc(0.0f);
   for (int member = 0; member < group; ++member) {
     const int64_t index = first + int64_t(member) * a.p.chunks;
     const Place at(a.p, index);
-    __syncthreads();
-    if (wave == 0) load_gates(g, a.gate, a.beta, at);
+    const GatePair gates(a.gate, a.beta, at);
+    solve_in.load_triangle(a.kept.solve + index * kChunk * kChunk);
+    fetch_half(at, 0);
+    q_in.load(a.q.at(at.b, at.t0, at.key_head), a.q.s.token, at.valid, a.p.key_dim);
+    k_in.load(a.k.at(at.b, at.t0, at.key_head), a.k.s.token, at.valid, a.p.key_dim);
+    lds_barrier();
+    if (wave == 0) gates.put(g);
     Acc dq[kTiles], z[kTiles], y[kTiles], n(0.0f), m(0.0f);
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) dq[t] = z[t] = y[t] = Acc(0.0f);
     float found = 0.0f, both = 0.0f;
-    const float* from = a.kept.solve + index * kChunk * kChunk;
-    load_tile<float>(solve, from, kChunk, kChunk, kChunk, Keep{});
-    const float* u_row = a.kept.updates + (index * kChunk + token) * kDim;
+    solve_in.put(solve);
     const int64_t row = ((int64_t(at.b) * a.p.tokens + at.t0 + token) * a.p.heads + at.h) * a.p.dim;
 #pragma unroll
     for (int d0 = 0; d0 < kDim; d0 += 64) {
       if (d0 >= a.p.dim) break;
       const int wide = a.p.dim - d0;
-      if (d0) __syncthreads();
-      load_tile<T>(grad, a.grad.at(at.b, at.t0, at.h) + d0, a.grad.s.token, a.grad.p ? at.valid : 0, wide, Keep{});
-      load_tile<float>(u, a.kept.updates + index * kChunk * kDim + d0, kDim, kChunk, wide, Keep{});
-      load_tile<float>(du, a.du + index * kChunk * kDim + d0, kDim, kChunk, wide, Keep{});
-      load_tile<float>(state, a.kept.starts + index * kKey * kDim + d0, kDim, a.p.key_dim, wide, Keep{});
-      __syncthreads();
+      if (d0) lds_barrier();
+      grad_in.put(grad);
+      u_in.put(u);
+      du_in.put(du);
+      state_in.put(state);
+#pragma unroll
+      for (int i = 0; i < end_in.kCount; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) both += float(end_in.x[i][e]) * float(state_in.x[i][e]);
+      lds_barrier();
       // dR of the wave's tokens and 32 dimensions.
       Acc r(0.0f);
-      for (int s = m0 / 16; s < 4; ++s) mma_parts(du.cols(16 * s, 32 * side), solve.cols(16 * s, m0), r);
-      __syncthreads();
+      steps_from(m0, [&](int s) { mma_parts(du.rows(32 * side, 16 * s), solve.cols(16 * s, m0), r); });
+      lds_barrier();
       const float b = g.beta[token];
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
@@ -270,48 +309,39 @@ __global__ __launch_bounds__(kThreads, (kKey == 64 && std::is_same_v<T, bf16> ? 
         if (token < at.rows && col < wide) {
           FloatVec<4> out = b * dr;
           if (token < at.valid) {
-            const FloatVec<4> uu = *reinterpret_cast<const FloatVec<4>*>(u_row + d0 + col);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) found += uu[i] * dr[i];
+            for (int i = 0; i < 4; ++i) found += u.get(col + i, token) * dr[i];
           } else {
             out = FloatVec<4>(0.0f);
           }
           *reinterpret_cast<Vec<T, 4>*>(a.dv + row + d0 + col) = from_float<T, 4>(out);
         }
       }
-      __syncthreads();
+      lds_barrier();
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
         if (wave < 3) {
-          const auto left = u.rows(j0, 16 * s);
+          const auto left = u.cols(16 * s, j0);
           mma_parts(left, grad.rows(i0, 16 * s), n);
           mma_parts(left, x.rows(i0, 16 * s), m);
         }
         const auto go = grad.rows(m0, 16 * s), dr = x.rows(m0, 16 * s);
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
-          const auto left = state.rows(32 * (side + 2 * t), 16 * s);
+          const auto left = state.cols(16 * s, 32 * (side + 2 * t));
           mma_parts(left, go, dq[t]);
           mma_parts(left, dr, z[t]);
         }
       }
-      __syncthreads();
-      // dS', and its product with S.
-      const float* start = a.kept.starts + index * kKey * kDim + d0;
-      load_tile<float>(state, a.ends + index * kKey * kDim + d0, kDim, a.p.key_dim, wide,
-                       [&](int row, int col, auto& ds) {
-                         if (row < a.p.key_dim && col < wide) {
-                           const FloatVec<8> s = to_float<float, 8>(load_global<float>(start + row * kDim + col, true));
-#pragma unroll
-                           for (int i = 0; i < 8; ++i) both += ds[i] * s[i];
-                         }
-                       });
-      __syncthreads();
+      lds_barrier();
+      end_in.put(state);
+      if (d0 + 64 < a.p.dim) fetch_half(at, d0 + 64);
+      lds_barrier();
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        const auto right = u.rows(m0, 16 * s);
+        const auto right = u.cols(16 * s, m0);
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) mma_parts(state.rows(32 * (side + 2 * t), 16 * s), right, y[t]);
+        for (int t = 0; t < kTiles; ++t) mma_parts(state.cols(16 * s, 32 * (side + 2 * t)), right, y[t]);
       }
     }
     const float up = g.up[token], down = g.down[token], beta = g.beta[token];
@@ -321,7 +351,7 @@ __global__ __launch_bounds__(kThreads, (kKey == 64 && std::is_same_v<T, bf16> ? 
       z[t] *= -up;
       y[t] *= down;
     }
-    __syncthreads();
+    lds_barrier();
     if (wave < 3) {
       const int i = i0 + (lane & 31);
       const float b = g.beta[i];
@@ -336,8 +366,7 @@ __global__ __launch_bounds__(kThreads, (kKey == 64 && std::is_same_v<T, bf16> ? 
           mm[e] = j + e < i ? -d * mm[e] : 0.0f;
         }
         n_tile.put(i, j, Parts<E, P, 4>(nn));
-        m_tile.put(i, j, Parts<E, P, 4>(mm));
-        mb_tile.put(i, j, Parts<E, P, 4>(b * mm));
+        m_tile.put(i, j, Parts<E, P, 4>(b * mm));
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           n[4 * s + e] = nn[e];
@@ -345,9 +374,9 @@ __global__ __launch_bounds__(kThreads, (kKey == 64 && std::is_same_v<T, bf16> ? 
         }
       }
     }
-    load_tile<T>(q, a.q.at(at.b, at.t0, at.key_head), a.q.s.token, at.valid, a.p.key_dim, Keep{});
-    load_tile<T>(k, a.k.at(at.b, at.t0, at.key_head), a.k.s.token, at.valid, a.p.key_dim, Keep{});
-    __syncthreads();
+    q_in.put(q);
+    k_in.put(k);
+    lds_barrier();
     if (wave < 3) {
       Acc qk(0.0f), kk(0.0f);
 #pragma unroll
@@ -362,7 +391,7 @@ __global__ __launch_bounds__(kThreads, (kKey == 64 && std::is_same_v<T, bf16> ? 
       for (int r = 0; r < 16; ++r) sum += n[r];
       sum += __shfl_xor(sum, 32, kWave);
       if (lane < 32) crossing[0][wave][lane] = sum;
-      const float column = column_sums(n);
+      const float column = column_sums<8>(n);
       if ((lane & 16) == 0) crossing[1][wave][acc_row_of_half(sums_register()) + 4 * (lane >> 5)] = column;
     }
     float reads = 0.0f, writes = 0.0f;
@@ -378,28 +407,30 @@ __global__ __launch_bounds__(kThreads, (kKey == 64 && std::is_same_v<T, bf16> ? 
           writes += kk[i] * y[t][4 * s + i];
         }
       }
-    for (int s = 0; s < (m0 ? 4 : 2); ++s) {
-      const auto nn = n_tile.rows(m0, 16 * s), mm = m_tile.rows(m0, 16 * s);
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-        const auto left = k.cols(16 * s, 32 * (side + 2 * t));
-        mma_parts(left, nn, dq[t]);
-        mma_parts(left, mm, z[t]);
-      }
-    }
-    for (int s = m0 / 16; s < 4; ++s) {
-      const auto nn = n_tile.cols(16 * s, m0), mm = mb_tile.cols(16 * s, m0);
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-        mma_parts(q.cols(16 * s, 32 * (side + 2 * t)), nn, y[t]);
-        mma_parts(k.cols(16 * s, 32 * (side + 2 * t)), mm, y[t]);
-      }
-    }
+    // The rest goes to the sums over the heads: b M has b of the key that reads in its
+    // rows.
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) {
       dq_all[t] += dq[t];
       dk_all[t] += beta * z[t] + y[t];
     }
+    steps_to(m0, [&](int s) {
+      const auto nn = n_tile.rows(m0, 16 * s), mm = m_tile.rows(m0, 16 * s);
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) {
+        const auto left = k.cols(16 * s, 32 * (side + 2 * t));
+        mma_parts(left, nn, dq_all[t]);
+        mma_parts(left, mm, dk_all[t]);
+      }
+    });
+    steps_from(m0, [&](int s) {
+      const auto nn = n_tile.cols(16 * s, m0), mm = m_tile.cols(16 * s, m0);
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) {
+        mma_parts(q.cols(16 * s, 32 * (side + 2 * t)), nn, dk_all[t]);
+        mma_parts(k.cols(16 * s, 32 * (side + 2 * t)), mm, dk_all[t]);
+      }
+    });
     const float all[3] = {reads, writes, found};
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
@@ -409,7 +440,7 @@ __global__ __launch_bounds__(kThreads, (kKey == 64 && std::is_same_v<T, bf16> ? 
 #pragma unroll
     for (int d = 1; d < kWave; d <<= 1) both += __shfl_xor(both, d, kWave);
     if (lane == 0) inner[wave] = both;
-    __syncthreads();
+    lds_barrier();
     if (wave == 0) {
       const int row = lane & 31;
       const float wrote = dots[1][0][lane] + dots[1][1][lane];
@@ -430,10 +461,8 @@ __global__ __launch_bounds__(kThreads, (kKey == 64 && std::is_same_v<T, bf16> ? 
       if (lane < at.rows) {
         float dgate = 0.0f, dbeta = 0.0f;
         if (lane < at.valid) {
-          const float gate = float(*a.gate.at(at.b, at.t0 + lane, at.h));
-          const float raw = float(*a.beta.at(at.b, at.t0 + lane, at.h));
-          dgate = (total + rest) * sigmoid(-gate);
-          dbeta = (dots[2][0][lane] + dots[2][1][lane]) * sigmoid(-raw);
+          dgate = (total + rest) * g.fade[lane];
+          dbeta = (dots[2][0][lane] + dots[2][1][lane]) * g.rest[lane];
         }
         const int64_t to = (int64_t(at.b) * a.p.tokens + at.t0 + lane) * a.p.heads + at.h;
         a.dgate[to] = T(dgate);
@@ -465,7 +494,8 @@ int backward(const BackwardArgs<T>& a, const float* grad_last, float* grad_state
   delta_back_prepare_kernel<T, kKey, kDim><<<seq::grid_of(a.count), kThreads, 0, s>>>(a);
   GS_TRY(check_launch("delta_scan backward prepare"));
   ChainArgs chain{int64_t(a.p.batch) * a.p.heads, a.p.chunks, a.p.key_dim, a.p.dim, a.chain, grad_last,
-                  a.du, a.ends, grad_state};
+                  a.p.heads / a.p.key_heads, a.du, a.du, a.begins, a.ends, grad_state, a.segments, a.maps,
+                  a.adds, 0, 0};
   GS_TRY(launch_chain(chain, kKey, kDim, Form<T>::chain_in, true, s));
   const int64_t groups = a.count / (a.p.heads / a.p.key_heads);
   delta_grads_kernel<T, kKey, kDim><<<seq::grid_of(groups), kThreads, 0, s>>>(a);
@@ -481,9 +511,11 @@ using namespace gs;
 extern "C" GS_API size_t gs_delta_scan_bwd_workspace_bytes(const gs_delta* desc) {
   if (!desc || check_delta(*desc) != GS_OK) return 0;
   const size_t wide = delta::padded(desc->dim);
-  return size_t(delta_chunks(*desc)) *
+  return delta_segment_bytes(*desc) +
+         size_t(delta_chunks(*desc)) *
          (delta_left_bytes(*desc, delta_parts_in(*desc) + delta_parts_mid(*desc)) +
-          (delta::kFactors + (delta::kChunk + delta::padded(desc->key_dim)) * wide) * sizeof(float));
+          (delta::kFactors + (delta::kChunk + delta::padded(desc->key_dim)) * wide) * sizeof(float) +
+          (delta_store_bytes(*desc) == 2 ? delta::padded(desc->key_dim) * wide * 2 : 0));
 }
 
 extern "C" GS_API int gs_delta_scan_bwd(
@@ -523,12 +555,17 @@ extern "C" GS_API int gs_delta_scan_bwd(
     a.gate = rows(gate, 3);
     a.beta = rows(beta, 4);
     a.grad = grad_out ? rows(grad_out, 5) : delta::Rows<T>{nullptr, {0, 0, 0}};
-    a.kept = delta_kept(*desc, static_cast<float*>(const_cast<void*>(kept)), true);
+    a.kept = delta_kept(*desc, const_cast<void*>(kept), true);
     const int64_t wide = delta::padded(desc->dim);
     a.chain.factors = static_cast<float*>(workspace);
     a.du = a.chain.factors + n * delta::kFactors;
-    a.ends = a.du + n * delta::kChunk * wide;
-    a.chain.left = reinterpret_cast<delta::bf16*>(a.ends + n * delta::padded(desc->key_dim) * wide);
+    a.begins = a.du + n * delta::kChunk * wide;
+    a.ends = a.begins;
+    a.chain.left = reinterpret_cast<delta::bf16*>(a.begins + n * delta::padded(desc->key_dim) * wide);
+    if (delta_store_bytes(*desc) == 2) {
+      a.ends = a.chain.left;
+      a.chain.left += n * delta::padded(desc->key_dim) * wide;
+    }
     a.chain.right = a.chain.left + n * delta_left_bytes(*desc, delta_parts_in(*desc)) / 2;
     a.dq = static_cast<T*>(grad_q);
     a.dk = static_cast<T*>(grad_k);
@@ -536,6 +573,10 @@ extern "C" GS_API int gs_delta_scan_bwd(
     a.dgate = static_cast<T*>(grad_gate);
     a.dbeta = static_cast<T*>(grad_beta);
     a.count = n;
+    a.segments = delta::chain_segments(desc->batch * desc->heads, a.p.chunks, desc->dim);
+    a.adds = reinterpret_cast<float*>(a.chain.right + n * delta_left_bytes(*desc, delta_parts_mid(*desc)) / 2);
+    a.maps = reinterpret_cast<delta::bf16*>(a.adds + int64_t(a.segments) * desc->batch * desc->heads *
+                                                         delta::padded(desc->key_dim) * wide);
     const hipStream_t s = as_stream(stream);
     if (desc->key_dim <= 64)
       return desc->dim <= 64 ? delta::backward<T, 64, 64>(a, grad_last, grad_state, s)

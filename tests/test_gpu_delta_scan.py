@@ -122,7 +122,7 @@ def _head(q, k, v, a, b, state, scale, do, dlast, dtype):
         rows["k"].append(b[:, None] * z + y)
         rows["v"].append((b * row_r)[:, None].expand_as(du))
         # b db = u . dR, which the formula's other side equals.
-        rows["beta"].append(row_r * u.norm(dim=1) + dr.norm(dim=1) * x["row_u"] + few * (dr * u).abs().sum(1))
+        rows["beta"].append(row_r * u.norm(dim=1) + dr.norm(dim=1) * x["row_u"] + e_out * (dr * u).abs().sum(1))
         # What crosses a token: pairs, reads of the state before, writes into dS', and the
         # state itself; the sums in float32 of all of it.
         pair = n_mat.abs() * (aq @ ak.T) + bm * (ak @ ak.T)
@@ -257,6 +257,40 @@ def test_errors_as_a_whole(dtype):
             most = (4 if name == "gate" else 2) * UNIT[dtype]
         print(f"[delta] {dtype} {name} {off:.2e} of {most:.2e}", flush=True)
         assert off <= most, (name, off, most)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(1, 8300, 2, 1, 64, 64), (1, 8192, 1, 1, 40, 72), (1, 8501, 1, 1, 128, 104)])
+def test_long_sequences(shape, dtype):
+    """Sequences of so many chunks that the chain is cut into segments: as exact as a
+    whole as shorter ones, with a few units more for the segments' maps, and the same
+    values as in two calls that hand the state on, whose chains are not cut."""
+    b, t, h, hk, d, dv = shape
+    print(f"[delta] long {shape} {dtype}", flush=True)
+    inputs = _inputs(*shape, dtype, shift=5.0)
+    state = normal((b, h, d, dv), torch.float32, 9)
+    do, dlast = normal(inputs[2].shape, dtype, 50, 0.1), normal(state.shape, torch.float32, 51, 0.1)
+    values = orc.delta_scan(*inputs, state, grads=(do, dlast))
+    on = [x.to(DEV).requires_grad_(True) for x in (*inputs, state)]
+    got = delta_scan(*on)
+    grads = torch.autograd.grad(got, on, (do.to(DEV), dlast.to(DEV)))
+    for name, x, value in zip(NAMES, (*got, *grads), values):
+        off = float((x.detach().cpu().double() - value).norm() / value.norm())
+        if dtype == torch.float32:
+            most = 2.0**-17
+        elif name in ("last", "state"):
+            most = 2.0**-15
+        else:
+            most = (4 if name == "gate" else 2) * UNIT[dtype]
+        print(f"[delta] long {dtype} {name} {off:.2e} of {most:.2e}", flush=True)
+        assert off <= most, (name, off, most)
+    with torch.no_grad():
+        first, middle = delta_scan(*(x[:, :4096] for x in on[:5]), on[5])
+        rest, last = delta_scan(*(x[:, 4096:] for x in on[:5]), middle)
+    for a, c in ((torch.cat([first, rest], 1), got[0]), (last, got[1])):
+        unit = UNIT[a.dtype] if a.dtype == dtype else U32
+        chain = 2.0**-20 if dtype == torch.float32 else 2.0**-15
+        assert float((a.double() - c.double()).norm() / c.double().norm()) <= 2 * unit + chain
 
 
 @pytest.mark.parametrize("dtype", TYPES)
