@@ -17,9 +17,11 @@
 // is cut into segments, which all run at once, from a state of zeros and, without F and
 // Y, from the unit matrix: that is what a segment adds and what it maps a state to.
 // Each workgroup of the second pass starts from the product of the maps before it and
-// walks its segment once more.  Twice the work and more, in a tenth of the time.
+// walks its segment once more.
 //
-// Measured, 12 heads of 64 x 64, 625 chunks, bfloat16: @CHAIN@
+// Measured, 12 heads of 64 x 64, 625 chunks, bfloat16: 823 us forwards and 827 backwards
+// in one pass, 164 (65 and 99) and 244 (117 and 127) in 21 segments.  What bounds it now
+// is a chunk's own two products and the barrier between them, some 1.5 us.
 #include "delta_scan.h"
 
 namespace gs {
@@ -52,10 +54,11 @@ struct Walk {
   static constexpr int kLeft = PL * 4 * kSteps, kRight = PR * kTiles * 2, kPieces = kLeft + kRight;
   static constexpr int kLoads = (kPieces + kWaves - 1) / kWaves;  // of a thread
   // Two chunks in LDS where they fit, and one or two more on their way, where the
-  // registers hold them.
+  // registers hold them: two ahead, the maps of 625 chunks forwards take 71 us, one
+  // ahead 98; at keys of 128 two spill (32 chunks, 8 heads, again: 137 us, 52 with one).
   static constexpr int kRing = kPieces <= 64 ? 2 : 1;
-  static constexpr int kAhead = kWaves == 8 || (kPieces > 24 && kPieces <= 48) ? 2 : 1;
-  static constexpr int kPerSimd = kWaves == 8 || (kPieces <= 24 && kWaves == 4) ? 2 : 1;
+  static constexpr int kAhead = (kWaves == 8 && kPieces <= 24) || (kPieces > 24 && kPieces <= 48 && kKey == 64 && kWaves == 4) ? 2 : 1;
+  static constexpr int kPerSimd = kWaves == 8 || (kPass == kWhole && kPieces <= 24 && kWaves == 4) ? 2 : 1;
   static constexpr int kFactorsAt = kRing * kPieces * kPiece * 2;  // bytes
   static constexpr int kShared = kFactorsAt + kRing * kFactors * 4;
   // What later kernels take in one bfloat16 part is stored so.
@@ -68,6 +71,7 @@ struct Walk {
     Acc4 factors, rows[4], next[kBack ? kTiles : 1];
 
     // id: the chunk of the head; key: that of the keys that its group shares.
+    // col < 0: the unit matrix's, all lanes of which load one place that they do not take.
     __device__ __forceinline__ void load(const ChainArgs& a, int64_t id, int64_t key, int col) {
       const int thread = threadIdx.x, wave = thread >> 6, lane = thread & 63;
       const bf16* l = a.chain.left + (kBack ? key : id) * kLeft * kPiece + lane * 8;
@@ -79,11 +83,11 @@ struct Walk {
       }
       factors = *reinterpret_cast<const Acc4*>(a.chain.factors + id * kFactors + 4 * min(thread, kFactors / 4 - 1));
       const int group = lane >> 4;
-      const float* x = a.rows_from + (id * kDim + col) * kChunk + 4 * group;
+      const float* x = a.rows_from + id * kDim * kChunk + (col < 0 ? 0 : col * kChunk + 4 * group);
 #pragma unroll
       for (int m = 0; m < 4; ++m) rows[m] = *reinterpret_cast<const Acc4*>(x + 16 * m);
       if constexpr (kBack) {
-        const float* y = a.states_from + (id * kDim + col) * kKey + 4 * group;
+        const float* y = a.states_from + id * kDim * kKey + (col < 0 ? 0 : col * kKey + 4 * group);
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) next[t] = *reinterpret_cast<const Acc4*>(y + 16 * t);
       }
@@ -190,7 +194,7 @@ void chain_kernel(ChainArgs a) {
   const int segment = blockIdx.z / a.blocks, place = min(int(blockIdx.z % a.blocks) * kWaves + wave, all - 1);
   const bool unit = place >= own;
   const int col = (unit ? place - own : place) * kCols + n;
-  const int from = unit ? col % kDim : col;  // of rows that the unit matrix's do not take
+  const int from = unit ? -1 : col;
   const int first = segment * a.each, count = min(a.each, a.chunks - first);
   const auto chunk_of = [&](int i) {
     const int c = first + min(i, count - 1);
@@ -218,14 +222,31 @@ void chain_kernel(ChainArgs a) {
 #pragma unroll
   for (int i = 0; i < W::kAhead; ++i) load(stage[i], i);
   if constexpr (kPass == kAgain) {
-    // What the segments before this one make of the state.
+    // What the segments before this one make of the state, of maps that the workgroup
+    // reads once and puts in LDS, each while the one before is taken.
+    constexpr int kMap = PS * W::kTiles * W::kSteps, kEach = kMap / kWaves;
+    static_assert(kMap % kWaves == 0 && kMap <= W::kRing * W::kPieces, "a map has its place");
+    Frag<bf16> piece[kEach];
+    Acc4 y[W::kTiles];
+    const auto fetch = [&](int g) {
+      const int64_t at = head * a.segments + min(g, segment - 1);
+      const bf16* map = a.maps + at * kMap * kPiece + lane * 8;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        piece[i] = *reinterpret_cast<const Frag<bf16>*>(map + (i * kWaves + wave) * kPiece);
+    };
+    if (segment) fetch(0);
+    bf16* held = reinterpret_cast<bf16*>(space) + lane * 8;
     for (int g = 0; g < segment; ++g) {
-      const int64_t at = head * a.segments + g;
-      const bf16* map = a.maps + at * PS * W::kTiles * W::kSteps * kPiece + lane * 8;
-      const float* add = a.adds + (at * kDim + col) * kKey + 4 * group;
-      Acc4 y[W::kTiles];
+      const float* add = a.adds + ((head * a.segments + g) * kDim + col) * kKey + 4 * group;
 #pragma unroll
       for (int t = 0; t < W::kTiles; ++t) y[t] = *reinterpret_cast<const Acc4*>(add + 16 * t);
+      lds_barrier();
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        *reinterpret_cast<Frag<bf16>*>(held + (i * kWaves + wave) * kPiece) = piece[i];
+      fetch(g + 1);
+      lds_barrier();
 #pragma unroll
       for (int st = 0; st < W::kSteps; ++st) {
         Frag<bf16> b[PS];
@@ -234,8 +255,8 @@ void chain_kernel(ChainArgs a) {
         for (int p = 0; p < PS; ++p)
 #pragma unroll
           for (int t = 0; t < W::kTiles; ++t) {
-            const Frag<bf16> f = *reinterpret_cast<const Frag<bf16>*>(
-                map + ((p * W::kTiles + t) * W::kSteps + st) * kPiece);
+            const Frag<bf16> f =
+                *reinterpret_cast<const Frag<bf16>*>(held + ((p * W::kTiles + t) * W::kSteps + st) * kPiece);
 #pragma unroll
             for (int j = 0; j < PS; ++j)
               if (p + j < PS) y[t] = mma16(f, b[j], y[t]);
@@ -244,6 +265,7 @@ void chain_kernel(ChainArgs a) {
 #pragma unroll
       for (int t = 0; t < W::kTiles; ++t) s[t] = y[t];
     }
+    if (segment) lds_barrier();
   }
   // No branch in the loop: at one the loads that are on their way would have to be
   // waited for.  Behind the last chunk it is loaded again.
@@ -346,19 +368,27 @@ int launch_pass(ChainArgs a, hipStream_t s) {
 
 template <int kKey, int kDim, int PI, int PM, bool kBack>
 int launch(ChainArgs a, hipStream_t s) {
-  // Eight waves share L and R where there are as many and 256 registers hold a wave's part.
-  constexpr bool kSmall = (PI + PM) * kKey <= 384;
-  constexpr int kMapWaves = kSmall ? 8 : 4, kColWaves = kSmall && kDim == 128 ? 8 : 4;
+  // A map's waves are its columns' and the unit matrix's: eight of them share L and R
+  // where 256 registers hold a wave's part (float16 of 128, 16 heads, 8 segments of 16:
+  // 63 us, 102 with four).  Again they do not: there they spill (113 us, 156 with eight).
+  constexpr int kMapWaves = PI <= 2 ? 8 : 4, kColWaves = 4;
   a.each = (a.chunks + a.segments - 1) / a.segments;
   a.segments = (a.chunks + a.each - 1) / a.each;
   if (a.segments > 1) {
     GS_TRY((launch_pass<kKey, kDim, PI, PM, kBack, kMaps, kMapWaves>(a, s)));
     return launch_pass<kKey, kDim, PI, PM, kBack, kAgain, kColWaves>(a, s);
   }
-  // A CU alone gets some 40 GB/s from behind its L2, which few workgroups' chunks wait
-  // for: then each wave has a CU of its own.  @ALONE@
+  // A CU alone gets some 40 GB/s from behind its L2, and a barrier waits for the slowest
+  // of its waves: with CUs to spare, workgroups are smaller.  A wave alone, where 512
+  // registers hold its part and a chunk on its way (12 heads of 64, 32 chunks, bfloat16:
+  // 29 us, 37 with four waves), else two (8 heads of 64 x 128, float32: 31 us, 40 with
+  // four, and one spills; of 128: 136, 156 with four).
   const int64_t waves = a.heads * ((a.dim + kCols - 1) / kCols);
-  if (waves <= 256) return launch_pass<kKey, kDim, PI, PM, kBack, kWhole, 1>(a, s);
+  if constexpr ((PI + PM) * kKey <= 192) {
+    if (waves <= 256) return launch_pass<kKey, kDim, PI, PM, kBack, kWhole, 1>(a, s);
+  } else if (waves <= 256) {
+    return launch_pass<kKey, kDim, PI, PM, kBack, kWhole, 2>(a, s);
+  }
   return launch_pass<kKey, kDim, PI, PM, kBack, kWhole, kColWaves>(a, s);
 }
 
@@ -380,12 +410,14 @@ int launch_sizes(const ChainArgs& a, int key_wide, int wide, int parts_in, hipSt
 
 }  // namespace
 
-// Segments of a sequence: as many as give every CU a workgroup, of sixteen chunks and
-// more; below eight of them the two passes gain nothing.
+// Segments of a sequence: as many as give every CU a workgroup of the second pass, of
+// eight chunks and more.  Four of them are as quick as one pass or quicker (12 heads of
+// 64, 32 chunks: 37 us for 45 in bfloat16, 53 for 68 in float32; 32 heads of 128: 78 for
+// 70, 8 heads: 61 for 69), three are not (35 for 36), twenty-one are five times as quick.
 int chain_segments(int64_t heads, int64_t chunks, int dim) {
   const int64_t blocks = (dim + 63) / 64;
-  const int64_t most = std::min<int64_t>({chunks / 16, 256 / std::max<int64_t>(heads * blocks, 1), 32});
-  return most < 8 ? 1 : int(most);
+  const int64_t most = std::min<int64_t>({chunks / 8, 256 / std::max<int64_t>(heads * blocks, 1), 32});
+  return most < 4 ? 1 : int(most);
 }
 
 int launch_chain(const ChainArgs& a, int key_wide, int wide, int parts_in, bool backward,

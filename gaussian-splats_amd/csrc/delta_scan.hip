@@ -9,8 +9,9 @@
 // in all later chunks, outputs and states are NaN; products with zeros of a triangle
 // would carry it to tokens before it.
 //
-// Measured, 40000 tokens, 12 heads of 64 on 4, bfloat16: 186 us to
-// prepare, 90 the outputs, and the chain.
+// Measured, 40000 tokens, 12 heads of 64 on 4, bfloat16: 132 us to prepare (with three
+// workgroups a CU, LDS used twice; 186 with two), 79 the outputs, and the chain.  The
+// inverse's short dependent steps bound the first, the reads of states the second.
 #include "delta_scan.h"
 
 namespace gs {
@@ -100,8 +101,11 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(ForwardArgs<T> 
   using E = typename M::Elem;
   using KTile = Tile<E, M::in, kChunk, kKey>;
   using VTile = Tile<E, M::in, kChunk, kDim>;
-  __shared__ __align__(16) char k_space[KTile::bytes], v_space[VTile::bytes];
-  __shared__ __align__(16) float system[kChunk * kPitchA], solve[kChunk * kPitchA];
+  // The values take the place of A, once T is there: three workgroups share a CU.
+  constexpr int kSystem = kChunk * kPitchA * int(sizeof(float));
+  __shared__ __align__(16) char k_space[KTile::bytes];
+  __shared__ __align__(16) char v_space[kSystem > VTile::bytes ? kSystem : VTile::bytes];
+  __shared__ __align__(16) float solve[kChunk * kPitchA];
   __shared__ float by_key[kChunk], by_value[kChunk];
   __shared__ Gates g;
   const int64_t index = seq::block_index();
@@ -110,6 +114,7 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(ForwardArgs<T> 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const KTile k(k_space);
   const VTile v(v_space);
+  float* system = reinterpret_cast<float*>(v_space);
   const GatePair gates(a.gate, a.beta, at);
   Fetch<T, kChunk, kKey> k_in;
   Fetch<T, kChunk, kDim> v_in;
@@ -127,7 +132,8 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(ForwardArgs<T> 
     }
   };
   k_in.put(k, mark);
-  v_in.put(v, mark);
+#pragma unroll
+  for (int i = 0; i < v_in.kCount; ++i) mark(v_in.row(i), 0, v_in.x[i]);
   if (threadIdx.x < kChunk) {
     by_value[threadIdx.x] = g.beta[threadIdx.x];
     by_key[threadIdx.x] = -g.beta[threadIdx.x] * g.up[threadIdx.x];
@@ -145,14 +151,16 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(ForwardArgs<T> 
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       const int j = j0 + four_row(s);
-      FloatVec<4> x = four(c, s);
+      FloatVec<4> x = four(c, s) * g.decay(i, j);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) x[r] = j + r < i ? b * g.decay(i, j + r) * x[r] : 0.0f;
+      for (int r = 0; r < 4; ++r) x[r] = j + r < i ? b * x[r] : 0.0f;
       *reinterpret_cast<FloatVec<4>*>(system + i * kPitchA + j) = x;
     }
   }
   lds_barrier();
   solve_triangle(system, solve);
+  v_in.put(v);
+  lds_barrier();
   if (a.kept.solve) {
     float* to = a.kept.solve + index * kChunk * kChunk;
 #pragma unroll
@@ -278,9 +286,9 @@ __global__ __launch_bounds__(kThreads) void delta_output_kernel(ForwardArgs<T> a
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       const int j = j0 + four_row(s);
-      FloatVec<4> x = four(c, s);
+      FloatVec<4> x = four(c, s) * g.decay(i, j);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) x[r] = j + r <= i ? a.p.scale * g.decay(i, j + r) * x[r] : 0.0f;
+      for (int r = 0; r < 4; ++r) x[r] = j + r <= i ? a.p.scale * x[r] : 0.0f;
       if (wave < 3) p.put(i, j, Parts<E, M::out, 4>(x));
     }
   }

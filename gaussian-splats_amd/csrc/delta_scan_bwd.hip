@@ -24,8 +24,9 @@
 // registers, so that the factors of a token are one number, its scalar products need
 // no exchange but of four lanes, and stores are of consecutive elements.
 //
-// Measured, 40000 tokens, 12 heads of 64 on 4, bfloat16: 227 us to
-// prepare, 421 the gradients, and the chain.
+// Measured, 40000 tokens, 12 heads of 64 on 4, bfloat16: 134 us to prepare (227 with two
+// workgroups a CU), 213 the gradients (421 before sums stayed in registers and gates
+// were read as vectors), and the chain.  LDS traffic and latency bound both.
 #include "delta_scan.h"
 
 namespace gs {
@@ -75,8 +76,10 @@ __global__ __launch_bounds__(kThreads) void delta_back_prepare_kernel(BackwardAr
   using OTile = Tile<E, F::in, kChunk, kDim>;
   using PTile = Tile<E, F::mid, kChunk, kChunk>;
   static_assert(QTile::bytes <= 2 * KTile::bytes, "the scaled q takes the place of k and q");
-  __shared__ __align__(16) char kq_space[2 * KTile::bytes], o_space[OTile::bytes], p_space[PTile::bytes];
-  __shared__ __align__(16) float solve[kChunk * kPitchA];
+  // P takes T's place, once W is there: three workgroups share a CU.
+  constexpr int kSolve = kChunk * kPitchA * int(sizeof(float));
+  __shared__ __align__(16) char kq_space[2 * KTile::bytes], o_space[OTile::bytes];
+  __shared__ __align__(16) char p_space[kSolve > PTile::bytes ? kSolve : PTile::bytes];
   __shared__ float by_key[kChunk];
   __shared__ Gates g;
   const int64_t index = seq::block_index();
@@ -87,6 +90,7 @@ __global__ __launch_bounds__(kThreads) void delta_back_prepare_kernel(BackwardAr
   const QTile q_up(kq_space);
   const OTile grad(o_space);
   const PTile p(p_space);
+  float* solve = reinterpret_cast<float*>(p_space);
   const T* q_rows = a.q.at(at.b, at.t0, at.key_head);
   const GatePair gates(a.gate, a.beta, at);
   Fetch<T, kChunk, kKey> k_in, q_in;
@@ -103,20 +107,6 @@ __global__ __launch_bounds__(kThreads) void delta_back_prepare_kernel(BackwardAr
   solve_in.put(Tile<float, 1, kChunk, kChunk>(reinterpret_cast<char*>(solve)));
   lds_barrier();
   if (threadIdx.x < kChunk) by_key[threadIdx.x] = -g.beta[threadIdx.x] * g.up[threadIdx.x];
-  if (wave < 3) {
-    const int i0 = wave ? 32 : 0, j0 = wave == 2 ? 32 : 0, i = i0 + (lane & 31);
-    Acc c(0.0f);
-#pragma unroll
-    for (int s = 0; s < kKey / 16; ++s) mma_parts(k.rows(j0, 16 * s), q.rows(i0, 16 * s), c);
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const int j = j0 + four_row(s);
-      FloatVec<4> x = four(c, s);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) x[r] = j + r <= i ? a.p.scale * g.decay(i, j + r) * x[r] : 0.0f;
-      p.put(i, j, Parts<E, F::mid, 4>(x));
-    }
-  }
   lds_barrier();
   const int m0 = 32 * (wave & 1), token = m0 + (lane & 31);
   // -W turned: a lane has a dimension and consecutive tokens.
@@ -163,6 +153,22 @@ __global__ __launch_bounds__(kThreads) void delta_back_prepare_kernel(BackwardAr
           __builtin_shufflevector(y.v[i], y.v[i], 4, 5, 6, 7);
     }
   }
+  lds_barrier();
+  if (wave < 3) {
+    const int i0 = wave ? 32 : 0, j0 = wave == 2 ? 32 : 0, i = i0 + (lane & 31);
+    Acc c(0.0f);
+#pragma unroll
+    for (int s = 0; s < kKey / 16; ++s) mma_parts(k.rows(j0, 16 * s), q.rows(i0, 16 * s), c);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int j = j0 + four_row(s);
+      FloatVec<4> x = four(c, s) * g.decay(i, j);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = j + r <= i ? a.p.scale * x[r] : 0.0f;
+      p.put(i, j, Parts<E, F::mid, 4>(x));
+    }
+  }
+  lds_barrier();
   // P^T dO.
   float* du = a.du + index * kChunk * kDim;
 #pragma unroll
@@ -358,12 +364,12 @@ __global__ __launch_bounds__(kThreads, (kKey == 64 && std::is_same_v<T, bf16> ? 
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
         const int j = j0 + four_row(s);
-        FloatVec<4> nn = four(n, s), mm = four(m, s);
+        const FloatVec<4> d = g.decay(i, j);
+        FloatVec<4> nn = four(n, s) * d, mm = four(m, s) * d;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float d = g.decay(i, j + e);
-          nn[e] = j + e <= i ? a.p.scale * d * nn[e] : 0.0f;
-          mm[e] = j + e < i ? -d * mm[e] : 0.0f;
+          nn[e] = j + e <= i ? a.p.scale * nn[e] : 0.0f;
+          mm[e] = j + e < i ? -mm[e] : 0.0f;
         }
         n_tile.put(i, j, Parts<E, P, 4>(nn));
         m_tile.put(i, j, Parts<E, P, 4>(b * mm));
