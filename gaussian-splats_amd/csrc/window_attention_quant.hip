@@ -19,8 +19,8 @@
 // flight that it has with 16-bit elements, so more waves share a CU: LDS is used
 // twice, for the values' tiles and for the join of the waves.
 //
-// Measured, bfloat16, 32 streams of up to 8176 slots, 32 heads of 128 on 8: 77 us
-// for 259 MB, 3.4 TB/s; the cache in 16 bits takes 189.
+// Measured, bfloat16, 32 streams of up to 8176 slots, 32 heads of 128 on 8: 59 us
+// for 259 MB, 4.4 TB/s; the cache in 16 bits takes 189.
 #include "attention_tile.h"
 
 namespace gs {
@@ -388,13 +388,17 @@ __global__ __launch_bounds__(kThreads) void step_quant_join_kernel(StepArgs a) {
   static_cast<T*>(a.out)[row * a.dim + d] = T(none ? 0.0f : (o + other[d]) / whole);
 }
 
-// Workgroups of one stream and key head: as many as fill the GPU, with a tile for
-// each of their waves.
+// Workgroups of one stream and key head: as many as the GPU holds at once (three a CU,
+// in float32 one), with a tile for each of their waves.  More wait for a place and
+// spend more on starts and ends (32 streams of 32 heads of 128 on 8 over 8176 slots:
+// bfloat16 55 us with 768, 64 with 2048; 6 streams: 23 and 36; float32 346 with 256, 405
+// with 2048).
 int plan_splits(const gs_attention& d) {
   const int64_t capacity = d.sinks + d.window;
   const int64_t rows = d.batch * d.kv_heads * ((d.heads / d.kv_heads + 31) / 32);
   const int64_t most = (capacity + kWaves * kKeys - 1) / (kWaves * kKeys);
-  return int(std::max<int64_t>(1, std::min<int64_t>({most, 2048 / std::max<int64_t>(rows, 1), kMostSplits})));
+  const int64_t held = d.type == GS_F32 ? 256 : 768;
+  return int(std::max<int64_t>(1, std::min<int64_t>({most, held / std::max<int64_t>(rows, 1), kMostSplits})));
 }
 
 // Filling: a slot takes the last of its tokens.  Four lanes a block, eight elements
