@@ -91,27 +91,28 @@ def clip_grad_norm(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm: 
     stretches of memory overlap, are refused.  A norm of NaN makes every gradient NaN, an infinite
     one makes them zero where they are finite."""
     max_norm = check_max_norm(max_norm)
-    grads, seen = [], set()
+    grads, flat, spans, seen = [], [], [], set()
     for p in _list(parameters):
         g = p.grad
         if g is None:
             continue
         _check(g)
-        mark = (g.data_ptr(), g.shape, g.stride(), g.dtype)
-        if g.numel() and mark not in seen:
-            seen.add(mark)
-            grads.append(g)
+        start, count = g.data_ptr(), g.numel()
+        mark = (start, g.shape, g.stride(), g.dtype)
+        if not count or mark in seen:
+            continue
+        seen.add(mark)
+        f = _flat(g)
+        if f is not g:
+            if any(n > 1 and s == 0 for n, s in zip(g.shape, g.stride())):
+                raise ValueError("a gradient is expanded: its elements share memory that clipping writes")
+            count = 1 + sum((n - 1) * s for n, s in zip(g.shape, g.stride()))
+        grads.append(g)
+        flat.append(f)
+        spans.append((start, start + count * g.element_size()))
     if not grads:
         return torch.zeros(())
-    flat = [_flat(g) for g in grads]
-    nat.require_gpu(*grads)
     end = 0
-    spans = []
-    for g, f in zip(grads, flat):
-        if f is not g and any(n > 1 and s == 0 for n, s in zip(g.shape, g.stride())):
-            raise ValueError("a gradient is expanded: its elements share memory that clipping writes")
-        last = sum((n - 1) * s for n, s in zip(g.shape, g.stride()))
-        spans.append((g.data_ptr(), g.data_ptr() + (last + 1) * g.element_size()))
     for lo, hi in sorted(spans):
         if lo < end:
             raise ValueError("two gradients' stretches of memory overlap")
