@@ -223,7 +223,9 @@ void chain_kernel(ChainArgs a) {
   for (int i = 0; i < W::kAhead; ++i) load(stage[i], i);
   if constexpr (kPass == kAgain) {
     // What the segments before this one make of the state, of maps that the workgroup
-    // reads once and puts in LDS, each while the one before is taken.
+    // reads once and puts in LDS, each while the one before is taken.  The state goes
+    // in with all its bits, in three parts: a segment behind a sequence's end, whose map
+    // is the unit matrix, leaves it as it is.
     constexpr int kMap = PS * W::kTiles * W::kSteps, kEach = kMap / kWaves;
     static_assert(kMap % kWaves == 0 && kMap <= W::kRing * W::kPieces, "a map has its place");
     Frag<bf16> piece[kEach];
@@ -249,8 +251,8 @@ void chain_kernel(ChainArgs a) {
       lds_barrier();
 #pragma unroll
       for (int st = 0; st < W::kSteps; ++st) {
-        Frag<bf16> b[PS];
-        operand<PS>(s[2 * st], s[2 * st + 1], b);
+        Frag<bf16> b[3];
+        operand<3>(s[2 * st], s[2 * st + 1], b);
 #pragma unroll
         for (int p = 0; p < PS; ++p)
 #pragma unroll
@@ -258,8 +260,8 @@ void chain_kernel(ChainArgs a) {
             const Frag<bf16> f =
                 *reinterpret_cast<const Frag<bf16>*>(held + ((p * W::kTiles + t) * W::kSteps + st) * kPiece);
 #pragma unroll
-            for (int j = 0; j < PS; ++j)
-              if (p + j < PS) y[t] = mma16(f, b[j], y[t]);
+            for (int j = 0; j < 3; ++j)
+              if (p == 0 || p + j < PS) y[t] = mma16(f, b[j], y[t]);
           }
       }
 #pragma unroll

@@ -118,12 +118,13 @@ class FusedAdam(torch.optim.Adam):
                 chunk = entries[i:i + nat.ADAM_MAX_TENSORS]
                 array = (nat.GsAdamTensor * len(chunk))(*chunk)
                 array = ctypes.cast(array, ctypes.c_void_p)
-                if factor is None:
-                    status = lib.gs_adam_step(array, len(chunk), beta1, beta2, eps, weight_decay,
-                                              nat.stream(device))
-                else:
-                    status = lib.gs_adam_step_scaled(array, len(chunk), beta1, beta2, eps,
-                                                     weight_decay, nat.ptr(factor), nat.stream(device))
+                with nat.on(device):
+                    if factor is None:
+                        status = lib.gs_adam_step(array, len(chunk), beta1, beta2, eps, weight_decay,
+                                                  nat.stream(device))
+                    else:
+                        status = lib.gs_adam_step_scaled(array, len(chunk), beta1, beta2, eps,
+                                                         weight_decay, nat.ptr(factor), nat.stream(device))
                 nat.check(status, "adam_step")
         del keep_alive, factor  # the launches are enqueued; the stream orders any reuse
         return loss

@@ -273,3 +273,28 @@ def test_offsets_beyond_32_bits():
     window_cache_fill_quant(k[:, None].to(DEV), k[:, None].to(DEV), *cache, window)
     assert torch.equal(cache[0][0, 0, 0].cpu(), orc.mxfp4_encode(k[0])[0][0])
     assert torch.equal(cache[0][:, :, -near:].cpu(), kept[0])
+
+
+def test_fill_in_a_graph():
+    """A captured filling follows its buffers' tokens and lengths."""
+    k, v = (normal((3, 90, 2, 64), torch.bfloat16, i).to(DEV) for i in (1, 2))
+    lengths = torch.tensor([90, 5, 0], dtype=torch.int32, device=DEV)
+    cache, twin = (QuantWindowCache(3, 2, 64, 30, 4, DEV) for _ in range(2))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        cache.fill(k, v, lengths)
+    torch.cuda.current_stream().wait_stream(side)
+    twin.fill(k, v, lengths)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.fill(k, v, lengths)
+    for turn in range(3):
+        for i, x in enumerate((k, v)):
+            x.copy_(normal(x.shape, torch.bfloat16, 10 * turn + i))
+        lengths.copy_(torch.tensor([turn, 90 - turn, 40]))
+        graph.replay()
+        torch.cuda.synchronize()
+        twin.fill(k, v, lengths)
+        for a, c in zip((*cache._tensors(), cache.positions), (*twin._tensors(), twin.positions)):
+            assert torch.equal(a, c)
