@@ -10,7 +10,7 @@
 // would carry it to tokens before it.
 //
 // Measured, 40000 tokens, 12 heads of 64 on 4, bfloat16: 132 us to prepare (with three
-// workgroups a CU, LDS used twice; 186 with two), 79 the outputs, and the chain.  The
+// workgroups a CU, LDS used twice; 186 with two), 73 the outputs, and the chain.  The
 // inverse's short dependent steps bound the first, the reads of states the second.
 #include "delta_scan.h"
 
@@ -232,26 +232,28 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(ForwardArgs<T> 
   }
 }
 
+// Q and K are in LDS for P = Q K^T alone; then Q's rows are in registers, and the
+// state's columns, U and P take the place, so that two workgroups share a CU in every
+// type and size (float16 heads of 128: 171 us for 2048 chunks, 268 with one).
 template <typename T, int kKey, int kDim>
-__global__ __launch_bounds__(kThreads) void delta_output_kernel(ForwardArgs<T> a) {
+__global__ __launch_bounds__(kThreads, 2) void delta_output_kernel(ForwardArgs<T> a) {
   using M = Form<T>;
   using E = typename M::Elem;
   using KTile = Tile<E, M::in, kChunk, kKey>;
   using STile = Tile<E, M::out, 64, kKey>;  // 64 columns of the state, turned
   using UTile = Tile<E, M::out, 64, kChunk>;
   using PTile = Tile<E, M::out, kChunk, kChunk>;
-  constexpr int kShared = KTile::bytes > STile::bytes ? KTile::bytes : STile::bytes;
-  __shared__ __align__(16) char q_space[KTile::bytes], k_space[kShared];
-  __shared__ __align__(16) char u_space[UTile::bytes], p_space[PTile::bytes];
+  constexpr int kFirst = 2 * KTile::bytes, kThen = STile::bytes + UTile::bytes + PTile::bytes;
+  __shared__ __align__(16) char space[kFirst > kThen ? kFirst : kThen];
   __shared__ Gates g;
   const int64_t index = seq::block_index();
   if (index >= a.count) return;
   const Place at(a.p, index);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const KTile q(q_space), k(k_space);
-  const STile state(k_space);
-  const UTile u(u_space);
-  const PTile p(p_space);
+  const KTile q(space), k(space + KTile::bytes);
+  const STile state(space);
+  const UTile u(space + STile::bytes);
+  const PTile p(space + STile::bytes + UTile::bytes);
   const GatePair gates(a.gate, a.beta, at);
   using Store = typename M::Store;
   const Store* starts = static_cast<const Store*>(a.kept.starts) + index * kKey * kDim;
@@ -272,8 +274,11 @@ __global__ __launch_bounds__(kThreads) void delta_output_kernel(ForwardArgs<T> a
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = finite(float(x[i])) ? x[i] : decltype(x[i] + x[i])(0.0f);
   });
-  u_in.put(u);
   lds_barrier();
+  const int m0 = 32 * (wave & 1), token = m0 + (lane & 31), n0 = 32 * (wave >> 1);
+  Parts<E, M::in, 8> own[kKey / 16];
+#pragma unroll
+  for (int s = 0; s < kKey / 16; ++s) own[s] = q.rows(m0, 16 * s);
   // P = scale Q K^T * D.
   {
     const int i0 = wave ? 32 : 0, j0 = wave == 2 ? 32 : 0;
@@ -282,6 +287,7 @@ __global__ __launch_bounds__(kThreads) void delta_output_kernel(ForwardArgs<T> a
 #pragma unroll
       for (int s = 0; s < kKey / 16; ++s) mma_parts(k.rows(j0, 16 * s), q.rows(i0, 16 * s), c);
     }
+    lds_barrier();
     const int i = i0 + (lane & 31);
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
@@ -292,21 +298,20 @@ __global__ __launch_bounds__(kThreads) void delta_output_kernel(ForwardArgs<T> a
       if (wave < 3) p.put(i, j, Parts<E, M::out, 4>(x));
     }
   }
-  const int m0 = 32 * (wave & 1), token = m0 + (lane & 31), n0 = 32 * (wave >> 1);
   const float up = a.p.scale * g.up[token];
   const bool bad = token >= int(a.chain.factors[index * kFactors + kChunk + 1]);
   T* out = a.out + ((int64_t(at.b) * a.p.tokens + at.t0 + token) * a.p.heads + at.h) * a.p.dim;
 #pragma unroll
   for (int d0 = 0; d0 < kDim; d0 += 64) {
     if (d0 >= a.p.dim) break;
-    lds_barrier();
+    if (d0) lds_barrier();
     state_in.put(state);
-    if (d0) u_in.put(u);
+    u_in.put(u);
     if (d0 + 64 < a.p.dim) fetch(d0 + 64);
     lds_barrier();
     Acc c(0.0f);
 #pragma unroll
-    for (int s = 0; s < kKey / 16; ++s) mma_parts(state.rows(n0, 16 * s), q.rows(m0, 16 * s), c);
+    for (int s = 0; s < kKey / 16; ++s) mma_parts(state.rows(n0, 16 * s), own[s], c);
     c *= up;
     steps_to(m0, [&](int s) { mma_parts(u.rows(n0, 16 * s), p.rows(m0, 16 * s), c); });
     if (token < at.rows) {
