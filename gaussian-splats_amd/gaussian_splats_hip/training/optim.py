@@ -73,6 +73,8 @@ class FusedAdam(torch.optim.Adam):
         # all launches are enqueued (a contiguous copy of a gradient would
         # otherwise return to the caching allocator before the kernel runs).
         keep_alive: list[torch.Tensor] = []
+        # For the norm: a gradient that two parameters share counts once.
+        counted: dict[tuple, torch.Tensor] = {}
         device = None
         for group in self.param_groups:
             beta1, beta2 = group["betas"]
@@ -102,6 +104,8 @@ class FusedAdam(torch.optim.Adam):
                 check_adam_tensors(p, grad, state["exp_avg"], state["exp_avg_sq"])
                 state["step"] += 1
                 keep_alive += (p, grad, state["exp_avg"], state["exp_avg_sq"])
+                if self.max_norm is not None:
+                    counted.setdefault((p.grad.data_ptr(), p.grad.shape, p.grad.stride()), grad)
                 batches.setdefault(key, []).append(nat.GsAdamTensor(
                     p.data_ptr(), grad.data_ptr(), state["exp_avg"].data_ptr(),
                     state["exp_avg_sq"].data_ptr(), p.numel(), float(group["lr"]),
@@ -109,9 +113,7 @@ class FusedAdam(torch.optim.Adam):
                 ))
         factor = None
         if self.max_norm is not None and keep_alive:
-            # A gradient that two parameters share counts once.
-            grads = {g.data_ptr(): g for g in keep_alive[1::4]}
-            self.grad_norm, factor = norm_of(list(grads.values()), self.max_norm)
+            self.grad_norm, factor = norm_of(list(counted.values()), self.max_norm)
         lib = nat.library()
         for (beta1, beta2, eps, weight_decay), entries in batches.items():
             for i in range(0, len(entries), nat.ADAM_MAX_TENSORS):
@@ -126,5 +128,5 @@ class FusedAdam(torch.optim.Adam):
                         status = lib.gs_adam_step_scaled(array, len(chunk), beta1, beta2, eps,
                                                          weight_decay, nat.ptr(factor), nat.stream(device))
                 nat.check(status, "adam_step")
-        del keep_alive, factor  # the launches are enqueued; the stream orders any reuse
+        del keep_alive, counted, factor  # the launches are enqueued; the stream orders any reuse
         return loss

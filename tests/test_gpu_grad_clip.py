@@ -226,3 +226,17 @@ def test_adam_within_the_limit_keeps_its_bits():
             opt.step()
         out.append(p.detach())
     assert torch.equal(*out)
+
+
+def test_adam_counts_a_shared_gradient_once():
+    """One gradient of two parameters counts once, in any layout; two gradients that
+    begin at one place and have different shapes are two."""
+    held = normal((6, 20), torch.float32, 1).to(DEV)
+    for first, second, count in ((held, held, 1), (held.t(), held.t(), 1), (held[:3], held, None)):
+        params = [torch.nn.Parameter(torch.zeros(g.shape, device=DEV)) for g in (first, second)]
+        for p, g in zip(params, (first, second)):
+            p.grad = g
+        opt = FusedAdam(params, max_norm=1.0)
+        opt.step()
+        want = _norm64([first.cpu()] if count else [first.cpu(), second.cpu()])
+        assert_within(opt.grad_norm, torch.tensor(want), want * NORM, "norm")
