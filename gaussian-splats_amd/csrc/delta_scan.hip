@@ -100,8 +100,10 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(ForwardArgs<T> 
   using M = Form<T>;
   using E = typename M::Elem;
   using KTile = Tile<E, M::in, kChunk, kKey>;
-  using VTile = Tile<E, M::in, kChunk, kDim>;
-  // The values take the place of A, once T is there: three workgroups share a CU.
+  // The values take the place of A, once T is there, 64 columns at a time: three
+  // workgroups of 64 x 64 share a CU in bfloat16, two of 128 x 128 in every type
+  // (@PREP@).
+  using VTile = Tile<E, M::in, kChunk, 64>;
   constexpr int kSystem = kChunk * kPitchA * int(sizeof(float));
   __shared__ __align__(16) char k_space[KTile::bytes];
   __shared__ __align__(16) char v_space[kSystem > VTile::bytes ? kSystem : VTile::bytes];
@@ -117,9 +119,11 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(ForwardArgs<T> 
   float* system = reinterpret_cast<float*>(v_space);
   const GatePair gates(a.gate, a.beta, at);
   Fetch<T, kChunk, kKey> k_in;
-  Fetch<T, kChunk, kDim> v_in;
+  Fetch<T, kChunk, 64> v_in[kDim / 64];
   k_in.load(a.k.at(at.b, at.t0, at.key_head), a.k.s.token, at.valid, a.p.key_dim);
-  v_in.load(a.v.at(at.b, at.t0, at.h), a.v.s.token, at.valid, a.p.dim);
+#pragma unroll
+  for (int t = 0; t < kDim / 64; ++t)
+    v_in[t].load(a.v.at(at.b, at.t0, at.h) + 64 * t, a.v.s.token, at.valid, a.p.dim - 64 * t);
   if (wave == 0) gates.put(g);
   lds_barrier();
   const auto mark = [&](int row, int, auto& x) {
@@ -133,7 +137,9 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(ForwardArgs<T> 
   };
   k_in.put(k, mark);
 #pragma unroll
-  for (int i = 0; i < v_in.kCount; ++i) mark(v_in.row(i), 0, v_in.x[i]);
+  for (int t = 0; t < kDim / 64; ++t)
+#pragma unroll
+    for (int i = 0; i < v_in[t].kCount; ++i) mark(v_in[t].row(i), 0, v_in[t].x[i]);
   if (threadIdx.x < kChunk) {
     by_value[threadIdx.x] = g.beta[threadIdx.x];
     by_key[threadIdx.x] = -g.beta[threadIdx.x] * g.up[threadIdx.x];
@@ -159,7 +165,7 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(ForwardArgs<T> 
   }
   lds_barrier();
   solve_triangle(system, solve);
-  v_in.put(v);
+  v_in[0].put(v);
   lds_barrier();
   if (a.kept.solve) {
     float* to = a.kept.solve + index * kChunk * kChunk;
@@ -193,14 +199,19 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(ForwardArgs<T> 
   float* rows = a.free + index * kChunk * kDim;
 #pragma unroll
   for (int t = 0; t < kDim / 64; ++t) {
-    const int n0 = 32 * ((wave >> 1) + 2 * t);
+    const int n0 = 32 * (wave >> 1);
+    if (t) {
+      lds_barrier();
+      v_in[t].put(v);
+      lds_barrier();
+    }
     Acc c(0.0f);
     steps_to(m0, [&](int s) {
       mma_parts(solve_rows<E, M::mid>(solve, m0, 16 * s, by_value), v.cols(16 * s, n0), c);
     });
 #pragma unroll
     for (int s = 0; s < 4; ++s)
-      *reinterpret_cast<FloatVec<4>*>(rows + (n0 + (lane & 31)) * kChunk + m0 + four_row(s)) = four(c, s);
+      *reinterpret_cast<FloatVec<4>*>(rows + (64 * t + n0 + (lane & 31)) * kChunk + m0 + four_row(s)) = four(c, s);
   }
   // K turned, once for the heads that share it.
   const int group = a.p.heads / a.p.key_heads;
@@ -234,7 +245,7 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(ForwardArgs<T> 
 
 // Q and K are in LDS for P = Q K^T alone; then Q's rows are in registers, and the
 // state's columns, U and P take the place, so that two workgroups share a CU in every
-// type and size (float16 heads of 128: 171 us for 2048 chunks, 268 with one).
+// type and size (float16 heads of 128: 171 us for 4096 chunks, 268 with one).
 template <typename T, int kKey, int kDim>
 __global__ __launch_bounds__(kThreads, 2) void delta_output_kernel(ForwardArgs<T> a) {
   using M = Form<T>;
