@@ -58,7 +58,7 @@ struct Walk {
   // ahead 98; at keys of 128 two spill (32 chunks, 8 heads, again: 137 us, 52 with one).
   static constexpr int kRing = kPieces <= 64 ? 2 : 1;
   static constexpr int kAhead = (kWaves == 8 && kPieces <= 24) || (kPieces > 24 && kPieces <= 48 && kKey == 64 && kWaves == 4) ? 2 : 1;
-  static constexpr int kPerSimd = kWaves == 8 || (kPass == kWhole && kPieces <= 24 && kWaves == 4) ? 2 : 1;
+  static constexpr int kPerSimd = kWaves == 8 ? 2 : 1;
   static constexpr int kFactorsAt = kRing * kPieces * kPiece * 2;  // bytes
   static constexpr int kShared = kFactorsAt + kRing * kFactors * 4;
   // What later kernels take in one bfloat16 part is stored so.
@@ -384,11 +384,15 @@ int launch(ChainArgs a, hipStream_t s) {
   // of its waves: with CUs to spare, workgroups are smaller.  A wave alone, where 512
   // registers hold its part and a chunk on its way (12 heads of 64, 32 chunks, bfloat16:
   // 29 us, 37 with four waves), else two (8 heads of 64 x 128, float32: 31 us, 40 with
-  // four, and one spills; of 128: 136, 156 with four).
+  // four, and one spills; of 128: 136, 156 with four).  With keys of 64 that holds up to
+  // two such waves a CU (128 heads of 64, 19 chunks, backwards: bfloat16 61 us, 72 with
+  // four; float32 72 and 99; 192 heads: 77 and 75), with wider ones for one (64 heads of
+  // 128, float32, backwards: 186 us with two waves, 144 with four).
   const int64_t waves = a.heads * ((a.dim + kCols - 1) / kCols);
+  constexpr int64_t kSpare = kKey == 64 ? 512 : 256;
   if constexpr ((PI + PM) * kKey <= 192) {
-    if (waves <= 256) return launch_pass<kKey, kDim, PI, PM, kBack, kWhole, 1>(a, s);
-  } else if (waves <= 256) {
+    if (waves <= kSpare) return launch_pass<kKey, kDim, PI, PM, kBack, kWhole, 1>(a, s);
+  } else if (waves <= kSpare) {
     return launch_pass<kKey, kDim, PI, PM, kBack, kWhole, 2>(a, s);
   }
   return launch_pass<kKey, kDim, PI, PM, kBack, kWhole, kColWaves>(a, s);
