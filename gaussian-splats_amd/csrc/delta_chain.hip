@@ -382,12 +382,13 @@ int launch(ChainArgs a, hipStream_t s) {
   }
   // A CU alone gets some 40 GB/s from behind its L2, and a barrier waits for the slowest
   // of its waves: with CUs to spare, workgroups are smaller.  A wave alone, where 512
-  // registers hold its part and a chunk on its way (12 heads of 64, 32 chunks, bfloat16:
-  // 29 us, 37 with four waves), else two (8 heads of 64 x 128, float32: 31 us, 40 with
-  // four, and one spills; of 128: 136, 156 with four).  With keys of 64 that holds up to
-  // two such waves a CU (128 heads of 64, 19 chunks, backwards: bfloat16 61 us, 72 with
-  // four; float32 72 and 99; 192 heads: 77 and 75), with wider ones for one (64 heads of
-  // 128, float32, backwards: 186 us with two waves, 144 with four).
+  // registers hold its part and a chunk on its way (8 heads of 64, 19 chunks, bfloat16:
+  // 29 us, 37 with four waves), else two (12 heads of 40 x 72, 13 chunks, float32: 31 us,
+  // 40 with four, and one spills; 8 heads of 128, 32 chunks: 136, 156 with four).  With
+  // keys of 64 that holds up to two such waves a CU (128 heads of 64, 19 chunks,
+  // backwards: bfloat16 61 us, 72 with four; float32 72 and 99; 192 heads: 77 and 75),
+  // with wider ones for one (64 heads of 128, float32, backwards: 186 us with two waves,
+  // 144 with four).
   const int64_t waves = a.heads * ((a.dim + kCols - 1) / kCols);
   constexpr int64_t kSpare = kKey == 64 ? 512 : 256;
   if constexpr ((PI + PM) * kKey <= 192) {

@@ -264,7 +264,7 @@ def test_errors_as_a_whole(dtype):
 def test_long_sequences(shape, dtype):
     """Sequences of so many chunks that the chain is cut into segments: as exact as a
     whole as shorter ones, with a few units more for the segments' maps, and the same
-    values as in two calls that hand the state on, whose chains are not cut."""
+    values as in two calls that hand the state on."""
     b, t, h, hk, d, dv = shape
     print(f"[delta] long {shape} {dtype}", flush=True)
     inputs = _inputs(*shape, dtype, shift=5.0)

@@ -13,6 +13,7 @@ import pytest
 import torch
 
 from gaussian_splats_hip.sequence import delta_scan, delta_scan_backward, delta_scan_forward
+from oracle import sequence as oracle
 from sequence_helpers import TYPES, UNIT, normal
 from test_gpu_delta_scan import DEV, _inputs
 
@@ -127,3 +128,34 @@ def test_in_a_graph():
         for x, do, (_, captured) in zip(inputs, dos, graphs):
             for a, c in zip(captured, run(x, do)):
                 assert torch.equal(a, c)
+
+
+def test_two_calls_at_once():
+    """Calls on two streams, cut and uncut, do not disturb one another."""
+    calls = [[x.to(DEV) for x in _inputs(*s, torch.bfloat16)]
+             for s in ((1, 5000, 4, 2, 64, 64), (1, 3000, 2, 2, 128, 128), (2, 700, 3, 1, 40, 72))]
+    alone = [delta_scan(*x) for x in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    for _ in range(3):
+        got = []
+        for x, stream in zip(calls, streams):
+            with torch.cuda.stream(stream):
+                got.append(delta_scan(*x))
+        torch.cuda.synchronize()
+        for a, c in zip(got, alone):
+            assert torch.equal(a[0], c[0]) and torch.equal(a[1], c[1])
+
+
+def test_one_tensor_as_query_and_key():
+    """The same tensor twice, and gradients that are expanded: both sides' errors add up."""
+    q, _, v, gate, beta = _inputs(1, 150, 2, 2, 16, 24, torch.float32)
+    ones = torch.ones(v.shape), torch.ones(1, 2, 16, 24)
+    want = oracle.delta_scan(q, q, v, gate, beta, grads=ones)
+    on = [x.to(DEV).requires_grad_(True) for x in (q, v, gate, beta)]
+    out, last = delta_scan(on[0], on[0], *on[1:])
+    (out.sum() + last.sum()).backward()
+    exact = [want[2] + want[3], *want[4:7]]
+    sizes = [want[2].norm() + want[3].norm(), *(x.norm() for x in want[4:7])]
+    for x, value, size in zip(on, exact, sizes):
+        assert float((x.grad.cpu().double() - value).norm()) <= 2.0**-18 * float(size)
