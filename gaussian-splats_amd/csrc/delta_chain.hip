@@ -188,11 +188,17 @@ void chain_kernel(ChainArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, group = lane >> 4;
   const int64_t head = block_index();
   if (head >= a.heads) return;
-  // Waves of columns; behind them the unit matrix's.  The last workgroup's last ones
-  // do another's work again.
-  const int own = (a.dim + kCols - 1) / kCols, all = own + (kPass == kMaps ? W::kTiles : 0);
-  const int segment = blockIdx.z / a.blocks, place = min(int(blockIdx.z % a.blocks) * kWaves + wave, all - 1);
-  const bool unit = place >= own;
+  // Waves of columns; behind them, in the maps' pass, the unit matrix's.  The last
+  // workgroup's spare waves take their share of L and R to LDS too, and no two waves store
+  // to one place: rows and states may be walked in place (backwards), with nothing between
+  // one wave's loads of them and another's stores.  In the passes that store, spare waves
+  // have the padding's columns, which are zeros and exist up to kDim; in the maps' pass
+  // they repeat the last wave's walk and store nothing.
+  static_assert(kPass == kMaps || kDim / kCols % kWaves == 0, "spare waves' columns exist");
+  const int own = (a.dim + kCols - 1) / kCols, all = own + W::kTiles;
+  const int segment = blockIdx.z / a.blocks, ticket = int(blockIdx.z % a.blocks) * kWaves + wave;
+  const int place = kPass == kMaps ? min(ticket, all - 1) : ticket;
+  const bool unit = kPass == kMaps && place >= own;
   const int col = (unit ? place - own : place) * kCols + n;
   const int from = unit ? -1 : col;
   const int first = segment * a.each, count = min(a.each, a.chunks - first);
@@ -230,6 +236,7 @@ void chain_kernel(ChainArgs a) {
     static_assert(kMap % kWaves == 0 && kMap <= W::kRing * W::kPieces, "a map has its place");
     Frag<bf16> piece[kEach];
     Acc4 y[W::kTiles];
+    const int known = min(place, own - 1) * kCols + n;  // the maps' pass adds to no padding
     const auto fetch = [&](int g) {
       const int64_t at = head * a.segments + min(g, segment - 1);
       const bf16* map = a.maps + at * kMap * kPiece + lane * 8;
@@ -240,7 +247,7 @@ void chain_kernel(ChainArgs a) {
     if (segment) fetch(0);
     bf16* held = reinterpret_cast<bf16*>(space) + lane * 8;
     for (int g = 0; g < segment; ++g) {
-      const float* add = a.adds + ((head * a.segments + g) * kDim + col) * kKey + 4 * group;
+      const float* add = a.adds + ((head * a.segments + g) * kDim + known) * kKey + 4 * group;
 #pragma unroll
       for (int t = 0; t < W::kTiles; ++t) y[t] = *reinterpret_cast<const Acc4*>(add + 16 * t);
       lds_barrier();
@@ -327,6 +334,7 @@ void chain_kernel(ChainArgs a) {
   for (int k = 0; k < W::kAhead - 1; ++k)
     if (i0 + k < count) run(i0 + k, stage[(k + kLead) % W::kAhead]);
   if constexpr (kPass == kMaps) {
+    if (ticket >= all) return;
     const int64_t at = head * a.segments + segment;
     if (unit) {
       // As a first operand: row 16 t + 4 g + i of column col, in the order of fragments.
