@@ -11,7 +11,10 @@ float32 GPU parameters, per-group ``lr``/``betas``/``eps``/``weight_decay``;
 With ``max_norm`` a step clips the 2-norm of all gradients together, as
 :func:`~gaussian_splats_hip.training.clip_grad_norm` before it would, but applies
 the factor inside the update: the gradients themselves stay as they are, and
-``grad_norm`` holds the norm (a float32 tensor, no host synchronisation).
+``grad_norm`` holds the norm (a float32 tensor, no host synchronisation; None behind
+a step in which no parameter had a gradient).  As no gradient is written, expanded
+ones and ones that share a part of their memory are not refused: all elements of each
+count, but one gradient of several parameters once.
 """
 
 from __future__ import annotations
@@ -46,7 +49,8 @@ def check_adam_tensors(p: torch.Tensor, grad: torch.Tensor, exp_avg: torch.Tenso
 
 class FusedAdam(torch.optim.Adam):
     max_norm: float | None = None
-    #: Norm of the gradients of the last step with ``max_norm``, before clipping.
+    #: Norm of the last step's gradients before clipping; None without ``max_norm`` or
+    #: without a gradient.
     grad_norm: torch.Tensor | None = None
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0,
@@ -66,6 +70,7 @@ class FusedAdam(torch.optim.Adam):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        self.grad_norm = None  # not that of an earlier step, whatever becomes of this one
         # Tensors of every group that share betas, eps and weight decay go into
         # one launch (the learning rate is per tensor).
         batches: dict[tuple, list] = {}

@@ -240,3 +240,18 @@ def test_adam_counts_a_shared_gradient_once():
         opt.step()
         want = _norm64([first.cpu()] if count else [first.cpu(), second.cpu()])
         assert_within(opt.grad_norm, torch.tensor(want), want * NORM, "norm")
+
+
+def test_adam_norm_is_the_last_steps():
+    """Steps with a gradient, without one and with one again."""
+    p = torch.nn.Parameter(torch.zeros(50, device=DEV))
+    opt = FusedAdam([p], max_norm=1.0)
+    for seed in (1, None, 2):
+        p.grad = None if seed is None else normal((50,), torch.float32, seed).to(DEV)
+        before = p.detach().clone()
+        opt.step()
+        if seed is None:
+            assert opt.grad_norm is None and torch.equal(p.detach(), before)
+        else:
+            want = _norm64([p.grad])
+            assert_within(opt.grad_norm, torch.tensor(want), want * NORM, "norm")

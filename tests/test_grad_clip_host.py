@@ -73,3 +73,17 @@ def test_c_abi_checks():
     assert call([(256, 5, 0)], ws=None) == nat.GS_ERR_WORKSPACE
     assert lib.gs_grad_norm_workspace_bytes(129) == 2 * need
     assert lib.gs_adam_step_scaled(None, 0, 0.9, 0.999, 1e-8, 0.0, None, None) == nat.GS_ERR_INVALID_ARGUMENT
+
+
+def test_no_norm_of_an_earlier_step():
+    """A step without gradients, or one that is refused, leaves no older step's norm."""
+    p = torch.nn.Parameter(torch.zeros(3))
+    opt = FusedAdam([p], max_norm=1.0)
+    opt.grad_norm = torch.tensor(5.0)
+    opt.step()
+    assert opt.grad_norm is None
+    opt.grad_norm = torch.tensor(5.0)
+    p.grad = torch.ones(3)
+    with pytest.raises(TypeError, match="ROCm GPU"):
+        opt.step()
+    assert opt.grad_norm is None
