@@ -119,8 +119,12 @@ class Block(nn.Module):
         y, stream = add_rms_norm(self.scan_out(mixed), stream, self.norms[1])
         q, k, v = self._qkv(y)
         if cache is not None:
-            state.copy_(last)
+            # Both fit before either is written: copy_ alone would spread one sequence's
+            # state over those of several streams.
+            if state.shape != last.shape:
+                raise ValueError(f"state {tuple(state.shape)} is not {list(last.shape)}, that of the tokens")
             cache.fill(k, v)
+            state.copy_(last)
         out = window_attention(q, k, v, self.window, self.sinks)
         y, stream = add_rms_norm(self.attention_out(out.flatten(-2)), stream, self.norms[2])
         return self.down(F.gelu(self.up(y))), stream
