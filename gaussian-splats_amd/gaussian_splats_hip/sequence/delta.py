@@ -145,9 +145,8 @@ def delta_scan_backward(
 
 class _DeltaScan(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, gate, beta, state, scale, lengths):
+    def forward(ctx, q, k, v, gate, beta, state, scale, lengths, backward):
         ctx.set_materialize_grads(False)
-        backward = any(ctx.needs_input_grad)
         out, last, kept = delta_scan_forward(q, k, v, gate, beta, state, scale, lengths, backward)
         if backward:
             ctx.save_for_backward(q, k, v, gate, beta, kept, lengths)
@@ -159,7 +158,7 @@ class _DeltaScan(torch.autograd.Function):
     def backward(ctx, grad_out, grad_last):
         q, k, v, gate, beta, kept, lengths = ctx.saved_tensors
         return (*delta_scan_backward(q, k, v, gate, beta, kept, grad_out, grad_last, ctx.scale, lengths,
-                                     ctx.needs_input_grad[5]), None, None)
+                                     ctx.needs_input_grad[5]), None, None, None)
 
 
 def delta_scan(
@@ -179,7 +178,10 @@ def delta_scan(
     A gate of -inf forgets what came before, one of +inf keeps it whole.  From a k, v,
     beta or gate that is not finite otherwise on, its head gives NaN.  Differentiable
     in q, k, v, gate, beta and state."""
-    return _DeltaScan.apply(q, k, v, gate, beta, state, scale, lengths)
+    # needs_input_grad does not know of no_grad, under which nothing is kept for a backward.
+    backward = torch.is_grad_enabled() and any(
+        t is not None and t.requires_grad for t in (q, k, v, gate, beta, state))
+    return _DeltaScan.apply(q, k, v, gate, beta, state, scale, lengths, backward)
 
 
 def delta_scan_step(

@@ -163,3 +163,30 @@ def test_c_abi_checks():
     assert lib.gs_delta_scan_step(problem(), FAKE, FAKE, FAKE, FAKE, FAKE, ctypes.c_void_p(264), FAKE, FAKE,
                                   None) == nat.GS_ERR_INVALID_ARGUMENT
     assert lib.gs_delta_scan_step(problem(b=0), None, None, None, None, None, None, None, None, None) == nat.GS_OK
+
+
+def test_only_a_backward_keeps_triangles(monkeypatch):
+    """What the forward keeps goes by whether a gradient can come: not under no_grad or
+    inference_mode, even of inputs that require one."""
+    from gaussian_splats_hip.sequence import delta
+
+    asked = []
+
+    def forward(q, k, v, gate, beta, state, scale, lengths, backward):
+        asked.append(backward)
+        return torch.zeros_like(v), torch.zeros(1, 2, 8, 8), torch.zeros(0)
+
+    monkeypatch.setattr(delta, "delta_scan_forward", forward)
+    inputs = [torch.zeros(1, 3, 1, 8), torch.zeros(1, 3, 1, 8), torch.zeros(1, 3, 2, 8), torch.zeros(1, 3, 2),
+              torch.zeros(1, 3, 2), torch.zeros(1, 2, 8, 8)]
+    sequence.delta_scan(*inputs)
+    for i in range(6):
+        leaves = [t.clone().requires_grad_(j == i) for j, t in enumerate(inputs)]
+        out, last = sequence.delta_scan(*leaves)
+        assert out.requires_grad and last.requires_grad
+        with torch.no_grad():
+            out, last = sequence.delta_scan(*leaves)
+        assert not out.requires_grad and not last.requires_grad
+        with torch.inference_mode():
+            sequence.delta_scan(*leaves)
+    assert asked == [False] + [True, False, False] * 6
