@@ -157,3 +157,47 @@ def test_captured_steps_of_all_together():
         torch.cuda.synchronize()
         for name in want:
             torch.testing.assert_close(out[name], want[name], rtol=0, atol=0)
+
+
+def test_training_clips_what_is_above_the_limit(monkeypatch):
+    """A limit of half the first step's norm, as a run without one has it: training
+    passes every step's gradients to the clipping, which brings the first ones down."""
+    seen = []
+    clip = predictor.clip_grad_norm
+
+    def recorded(parameters, limit):
+        parameters = list(parameters)
+        norm = clip(parameters, limit)
+        seen.append((float(norm), float(grad_norm([p.grad for p in parameters]))))
+        return norm
+
+    monkeypatch.setattr(predictor, "clip_grad_norm", recorded)
+    sizes = {"views": 2, "size": 64, "log": lambda *_: None, "mixer": "delta"}
+    predictor.train(steps=1, max_norm=float("inf"), **sizes)
+    (first, kept), = seen
+    assert first > 0.0 and kept == first
+    limit = first / 2
+    seen.clear()
+    predictor.train(steps=3, max_norm=limit, **sizes)
+    assert len(seen) == 3 and seen[0][0] > limit
+    for before, after in seen:
+        # The clipped ones are rounded to bfloat16 once more.
+        want = min(before, limit)
+        assert abs(after - want) <= want * (2.0**-8 + 1e-5)
+
+
+def test_a_prefill_of_a_single_stream_only():
+    """States of several streams refuse one's tokens and go on as if nothing had been asked."""
+    tokens, rays = _tokens(12)
+    for mixer, bits in (("gated", 16), ("delta", 16), ("delta", 4)):
+        torch.manual_seed(3)
+        model = predictor.SplatPredictor(width=128, heads=4, kv_heads=2, window=20, sinks=2, dtype=torch.float32,
+                                         mixer=mixer).to("cuda")
+        asked, other = model.start(4, cache_bits=bits), model.start(4, cache_bits=bits)
+        for states in (asked, other):
+            model.step(tokens[:4], rays[:4], states)
+        with pytest.raises(ValueError):
+            model.prefill(tokens, rays, asked)
+        a, c = (model.step(tokens[4:8], rays[4:8], states) for states in (asked, other))
+        for name in a:
+            assert torch.equal(a[name], c[name])
