@@ -19,8 +19,19 @@
 // flight that it has with 16-bit elements, so more waves share a CU: LDS is used
 // twice, for the values' tiles and for the join of the waves.
 //
-// Measured, bfloat16, 32 streams of up to 8176 slots, 32 heads of 128 on 8: 59 us
-// for 259 MB, 4.4 TB/s; the cache in 16 bits takes 189.
+// Codes are exact in 16 bits, so all that an output loses before its own rounding is
+// what its probabilities lose on their way into the second product.  They go in as two
+// numbers of the type: the result's 32 columns are 16 heads twice, and the upper ones take
+// the second part, in products that would else multiply columns without a head.  Once
+// rounded probabilities left 0.0021 (2-norm, bfloat16) where one rounding leaves 0.0017,
+// in 65 us a call instead of 66; from 17 heads a key on there are two tiles for one
+// (32 heads a key: 118 us for 81, and 158 with both parts in 32 columns).
+//
+// Measured, bfloat16, 32 streams of up to 8176 slots, 32 heads of 128 on 8: 66 us a call
+// for 259 MB; the step's kernel 58 us, 4.5 TB/s, the join 5; the cache in 16 bits takes
+// 189.  Three workgroups a CU leave 168 registers, and rows of 128 spill 17 that every
+// tile reads again.  In float32 (328 us) one workgroup a CU, for its registers and LDS,
+// and float32's products at a seventh of the rate bound it.
 #include "attention_tile.h"
 
 namespace gs {
@@ -108,9 +119,38 @@ __device__ __forceinline__ void store_frag(T* p, const Frag<T>& f) {
 
 using Word4 = Vec<uint32_t, 4>;
 
+// Of a float32, those that a 16-bit type has (float16 from its smallest normal number on).
+template <typename T>
+constexpr uint32_t kTakenBits = std::is_same_v<T, bf16> ? 0xffff0000u : 0xffffe000u;
+
+// acc_frag, cut off to these bits.
+template <typename T>
+__device__ __forceinline__ Frag<T> cut_frag(const Acc& c, int s) {
+  if constexpr (sizeof(T) == 4) {
+    return acc_frag<T>(c, s);
+  } else {
+    Word4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float a = c[8 * s + 2 * i], b = c[8 * s + 2 * i + 1];
+      if constexpr (std::is_same_v<T, bf16>)
+        w[i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
+      else
+        w[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+    }
+    return __builtin_bit_cast(Frag<T>, w);
+  }
+}
+
+// Heads of a tile, the columns of its products.  With 16-bit types its upper 16 columns
+// are the lower ones' heads once more, for the second part of their probabilities.
+template <typename T>
+constexpr int kHeads = sizeof(T) == 2 ? 16 : 32;
+
 template <typename T, int kDim>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 1) void step_quant_kernel(StepArgs a) {
   constexpr int kPitchT = kPitch<T, kDim>;
+  constexpr bool kBeside = sizeof(T) == 2;
   constexpr int kSteps = kDim / 16, kBlocks = kDim / 32;
   constexpr int kHalf = kDim / 64;                     // blocks of half a row
   constexpr int kCount = kKeys * kBlocks / kWave;      // blocks of values a lane converts
@@ -125,10 +165,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 1) void step_quant_k
   __shared__ float tops[kWaves][32], sums[kWaves][32];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5, col = lane & 31;
-  const int group = a.heads / a.kv_heads, group_tiles = (group + 31) / 32;
+  const int group = a.heads / a.kv_heads, group_tiles = (group + kHeads<T> - 1) / kHeads<T>;
   const int kv = blockIdx.y / group_tiles, group_tile = blockIdx.y % group_tiles;
   const int b = blockIdx.z, split = blockIdx.x;
-  const int member = group_tile * 32 + col;
+  const int member = group_tile * kHeads<T> + col % kHeads<T>;
   const bool live = member < group;
   const int pos = a.positions[b];
   const int capacity = a.sinks + a.window;
@@ -175,6 +215,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 1) void step_quant_k
     }
   }
   const float c = a.scale * kLog2e;
+  // The bits of a probability that the lower columns take.
+  const uint32_t upper = col < 16 ? 0u : kTakenBits<T>;
   float top = -INFINITY, sum = 0.0f;
   Acc o[kBlocks];
 #pragma unroll
@@ -285,11 +327,16 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 1) void step_quant_k
     const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] * c - base);
-    // Probabilities go into the second product in the inputs' type, and so into the
-    // sum, so that weights add up to one.
+    // Probabilities go into the second product, and so into the sum, as two numbers of a
+    // 16-bit type that add up to them but for 2^-16: the values are exact in it, which
+    // leaves the output its own rounding.  Beside each other the parts cost no product.
+    if constexpr (kBeside) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] -= __uint_as_float(__float_as_uint(s[r]) & upper);
+    }
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
-      const Frag<T> pf = acc_frag<T>(s, st);
+      const Frag<T> pf = cut_frag<T>(s, st);
       sum = add_all(pf, sum);
 #pragma unroll
       for (int n = 0; n < kBlocks; ++n) mma(load_turned<T>(tile, kPitchT, 16 * st, 32 * n), pf, o[n]);
@@ -298,6 +345,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 1) void step_quant_k
   }
   // The waves join: the largest maximum, then the sums one wave after the other.
   sum += __shfl_xor(sum, 32, 64);
+  if constexpr (kBeside) sum += __shfl_xor(sum, 16, 64);
   if (half == 0) {
     tops[wave][col] = top;
     sums[wave][col] = sum;
@@ -328,16 +376,18 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 1) void step_quant_k
     sums[0][col] = whole;
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < 32 * kDim; e += kThreads) {
+  for (int e = threadIdx.x; e < kHeads<T> * kDim; e += kThreads) {
     const int m = e / kDim, d = e % kDim;
-    if (group_tile * 32 + m >= group || d >= a.dim) continue;
-    const int64_t row = int64_t(b) * a.heads + kv * group + group_tile * 32 + m;
+    if (group_tile * kHeads<T> + m >= group || d >= a.dim) continue;
+    const int64_t row = int64_t(b) * a.heads + kv * group + group_tile * kHeads<T> + m;
+    float value = shared.joined[m][d];
+    if constexpr (kBeside) value += shared.joined[m + 16][d];
     if (a.splits == 1) {
       const float l = sums[0][m];
       const bool none = tops[0][m] == -INFINITY && l == 0.0f;
-      static_cast<T*>(a.out)[row * a.dim + d] = T(none ? 0.0f : shared.joined[m][d] / l);
+      static_cast<T*>(a.out)[row * a.dim + d] = T(none ? 0.0f : value / l);
     } else {
-      a.parts[(row * a.splits + split) * a.dim + d] = shared.joined[m][d];
+      a.parts[(row * a.splits + split) * a.dim + d] = value;
       if (d == 0) {
         a.stats[(row * a.splits + split) * 2] = tops[0][m];
         a.stats[(row * a.splits + split) * 2 + 1] = sums[0][m];
@@ -388,21 +438,29 @@ __global__ __launch_bounds__(kThreads) void step_quant_join_kernel(StepArgs a) {
   static_cast<T*>(a.out)[row * a.dim + d] = T(none ? 0.0f : (o + other[d]) / whole);
 }
 
+// Tiles of heads of a stream.
+int64_t key_tiles(const gs_attention& d) {
+  const int heads = d.type == GS_F32 ? kHeads<float> : kHeads<f16>;
+  return int64_t(d.kv_heads) * ((d.heads / d.kv_heads + heads - 1) / heads);
+}
+
 // Workgroups of one stream and key head: as many as the GPU holds at once (three a CU,
 // in float32 one), with a tile for each of their waves.  More wait for a place and
-// spend more on starts and ends (32 streams of 32 heads of 128 on 8 over 8176 slots:
-// bfloat16 55 us with 768, 64 with 2048; 6 streams: 23 and 36; float32 346 with 256, 405
-// with 2048).
+// spend more on starts and ends (calls, 32 streams of 32 heads of 128 on 8 over 8176
+// slots: bfloat16 74-76 us with 768, 81-83 with 2048; 6 streams: 22 and 34; float32 326 with
+// 256, 368 with 2048; 6 streams: 79 and 127).
 int plan_splits(const gs_attention& d) {
   const int64_t capacity = d.sinks + d.window;
-  const int64_t rows = d.batch * d.kv_heads * ((d.heads / d.kv_heads + 31) / 32);
+  const int64_t rows = d.batch * key_tiles(d);
   const int64_t most = (capacity + kWaves * kKeys - 1) / (kWaves * kKeys);
   const int64_t held = d.type == GS_F32 ? 256 : 768;
   return int(std::max<int64_t>(1, std::min<int64_t>({most, held / std::max<int64_t>(rows, 1), kMostSplits})));
 }
 
 // Filling: a slot takes the last of its tokens.  Four lanes a block, eight elements
-// each; keys and values in one launch.
+// each; keys and values in one launch.  Bound by the issue of instructions: 367 vector
+// ones a wave (counted), 16 waves a SIMD for 2 x 8160 tokens of 4 heads of 128 into 4096
+// slots, 10 of its 12 us; its 21 MB are 4 us.
 struct FillArgs {
   int batch, kv_heads, dim, window, sinks, tokens;
   const void* from[2];
@@ -514,8 +572,7 @@ extern "C" GS_API int gs_window_attention_step_quant(
   a.out = out;
   a.stats = static_cast<float*>(workspace);
   a.parts = a.stats + int64_t(a.batch) * a.heads * a.splits * 2;
-  const int64_t rows = int64_t(a.kv_heads) * ((a.heads / a.kv_heads + 31) / 32);
-  const dim3 grid(unsigned(a.splits), unsigned(rows), unsigned(a.batch));
+  const dim3 grid(unsigned(a.splits), unsigned(key_tiles(*desc)), unsigned(a.batch));
   const hipStream_t s = as_stream(stream);
   return seq::with_type(desc->type, [&](auto t) {
     using T = decltype(t);

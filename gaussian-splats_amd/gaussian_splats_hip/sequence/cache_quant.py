@@ -6,8 +6,9 @@ and each element a 4-bit code: a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 time
 power, the nearest (ties to the even code, 6 beyond 6).  That is the microscaling
 format MXFP4, 4.25 bits an element: a cache of a given size serves 3.8 times as
 many streams as in 16 bits, and a step reads 3.8 times less.  Codes stand for
-values of any of the inputs' types exactly, so the attention itself rounds as
-:func:`window_attention_step` does.  A block with an infinity or a NaN is NaN.
+values of the type that they were made from exactly (float16 does not hold all that
+blocks made from bfloat16 or float32 can), and the attention over them is rounded to
+the type once, at its end.  A block with an infinity or a NaN is NaN.
 
 Caches are four contiguous uint8 tensors: codes [batch, kv_heads, sinks + window,
 dim / 2], the even element in a byte's low half, and exponents [batch, kv_heads,

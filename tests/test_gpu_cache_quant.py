@@ -298,3 +298,26 @@ def test_fill_in_a_graph():
         twin.fill(k, v, lengths)
         for a, c in zip((*cache._tensors(), cache.positions), (*twin._tensors(), twin.positions)):
             assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(64, 8, 2, 64, 6, 1), (16, 34, 1, 128, 9, 0), (40, 16, 1, 96, 7, 0)])
+def test_outputs_have_one_rounding(shape, dtype):
+    """With values of one sign an output is as large as what is added up for it.
+    Probabilities are two numbers of the type, each cut off: within 2^-15 relative in
+    bfloat16 (2^-20 in float16, beside float32's scores at 2^-18), which moves a value
+    over the border between two of the type, 2^-8 (2^-11) of it apart, in at most 2^-6
+    (2^-6) of all places.  Probabilities rounded to the type once, 2^-9 (2^-12) off,
+    moved a twelfth of them."""
+    b, h, hk, d, window, sinks = shape
+    n = window + sinks
+    q, k, v = normal((b, h, d), dtype, 1), normal((b, hk, d), dtype, 2), normal((b, hk, d), dtype, 3).abs()
+    cache = _cache(b, hk, n, d, 4)
+    cache[2] &= 0x77
+    positions = torch.full((b,), n - 1, dtype=torch.int32)
+    want, _, _ = _step(q, k, v, cache, positions, window, sinks)
+    out = window_attention_step_quant(q.to(DEV), k.to(DEV), v.to(DEV), *(t.to(DEV) for t in cache),
+                                      positions.to(DEV), window, sinks).cpu()
+    moved = float((out != want.to(dtype)).double().mean())
+    print(f"[step quant] {shape} {dtype}: {moved:.4f} of the values moved", flush=True)
+    assert moved <= 2.0**-6
