@@ -56,8 +56,12 @@ struct Walk {
   // Two chunks in LDS where they fit, and one or two more on their way, where the
   // registers hold them: two ahead, the maps of 625 chunks forwards take 71 us, one
   // ahead 98; at keys of 128 two spill (32 chunks, 8 heads, again: 137 us, 52 with one).
+  // Backwards, with states on their way too, two spill earlier (the same maps in bfloat16:
+  // 20 registers, 129 us, 111 with one; the passes of float32 as well).
   static constexpr int kRing = kPieces <= 64 ? 2 : 1;
-  static constexpr int kAhead = (kWaves == 8 && kPieces <= 24) || (kPieces > 24 && kPieces <= 48 && kKey == 64 && kWaves == 4) ? 2 : 1;
+  static constexpr int kAhead = kKey == 64 && (kWaves == 8 ? kPieces <= 24 && !kBack
+                                                           : kWaves == 4 && kPieces > 24 && kPieces <= (kBack ? 32 : 48))
+                                    ? 2 : 1;
   static constexpr int kPerSimd = kWaves == 8 ? 2 : 1;
   static constexpr int kFactorsAt = kRing * kPieces * kPiece * 2;  // bytes
   static constexpr int kShared = kFactorsAt + kRing * kFactors * 4;
