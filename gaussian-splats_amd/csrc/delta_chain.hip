@@ -20,8 +20,10 @@
 // walks its segment once more.
 //
 // Measured, 12 heads of 64 x 64, 625 chunks, bfloat16: 823 us forwards and 827 backwards
-// in one pass, 164 (65 and 99) and 244 (117 and 127) in 21 segments.  What bounds it now
-// is a chunk's own two products and the barrier between them, some 1.5 us.
+// in one pass, 169 (68 and 101) and 240 (111 and 129) in 21 segments.  Many segments are
+// bound by what they move, counted: forwards 163 and 286 MB, backwards 241 and 410, which is
+// 2.2 to 3.2 TB/s of a copy's 5.1; a walk of few by a chunk's two products behind each
+// other and their barrier, some 1.5 us.
 #include "delta_scan.h"
 
 namespace gs {
@@ -430,9 +432,12 @@ int launch_sizes(const ChainArgs& a, int key_wide, int wide, int parts_in, hipSt
 }  // namespace
 
 // Segments of a sequence: as many as give every CU a workgroup of the second pass, of
-// eight chunks and more.  Four of them are as quick as one pass or quicker (12 heads of
-// 64, 32 chunks: 37 us for 45 in bfloat16, 53 for 68 in float32; 32 heads of 128: 78 for
-// 70, 8 heads: 61 for 69), three are not (35 for 36), twenty-one are five times as quick.
+// eight chunks and more, from four on.  Four take between a fifth less and a tenth more
+// than one pass (12 heads of 64, 32 chunks: 37 us for 45 in bfloat16, 53 for 68 in
+// float32; 8 heads of 128: 61 for 69, 32 heads: 78 for 70), three gain nothing at 32
+// chunks (35 for 36), twenty-one are five times as quick.  So 65 heads of 64 and more
+// (33 above 64) walk in one pass, however long: a forward call of 625 chunks in bfloat16 takes
+// 1.90 ms for 64 heads in four segments and 2.18 for 65 in none.
 int chain_segments(int64_t heads, int64_t chunks, int dim) {
   const int64_t blocks = (dim + 63) / 64;
   const int64_t most = std::min<int64_t>({chunks / 8, 256 / std::max<int64_t>(heads * blocks, 1), 32});

@@ -17,11 +17,19 @@
 // scale Q K^T * D,
 //   dU = P^T dO + e^(G_C - G) K dS',   dS = e^(G_C) dS' + scale Q^T e^G dO - W^T dU.
 //
-// Products run on the matrix cores.  What the states depend on is to be as exact as
-// float32, so a factor that is not an input is a sum of two bfloat16 numbers (16 bits
-// of mantissa, the range of float32), and inputs in float16 are two as well, exactly;
-// products of two second parts are left out.  Outputs in bfloat16 take one part a
-// factor.  float32 inputs stay in float32, and become three parts in the chain.
+// Products run on the matrix cores, whose sums are float32, as are the states that go
+// from chunk to chunk.  bfloat16 inputs go in as they are, float16 as a sum of two
+// bfloat16 numbers, exactly; any other factor of what states depend on is two as well,
+// 16 bits of mantissa and float32's range, with products of two second parts left out:
+// the last state is within some 5e-6 (2-norm) where sums in float32 alone leave 1e-7.
+// float32 inputs stay in float32, and become three parts in the chain.
+//
+// bfloat16's outputs and gradients take such factors (states, U, P, dR, ..) in one part,
+// and what is kept for their products is kept so, which gives the bits that rounding it
+// there would.  They are 0.0026-0.0033 off (2-norm), a rounding of their own alone is
+// 0.0017.  With two parts there too they had that: the view stream of 40000 tokens, 12 heads
+// of 64 on 4, took 1033 us for 893; 16 sequences of 1024 tokens, 16 heads on 4, forwards and
+// backwards, 494 for 414 at 64 x 64 and 1457 for 1101 at 128 x 128.
 #pragma once
 
 #include "attention_tile.h"

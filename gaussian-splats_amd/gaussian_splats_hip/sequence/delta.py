@@ -11,9 +11,11 @@ and into which it writes the difference to the token's value,
 Time is linear in the number of tokens and a running stream's memory constant.
 ``delta_scan`` is the training and prefill form, in chunks of 64 tokens whose
 products run on the matrix cores; ``delta_scan_step`` takes one token of each of
-several streams.  States are float32 throughout.  Keys should not be longer than
-one (``torch.nn.functional.normalize``): what a longer one writes can grow from
-token to token.
+several streams.  The recurrence, and the states that go in and come out, are float32;
+what bfloat16 calls keep of them for the products of outputs and gradients is bfloat16,
+as those products take it.  Keys should not be longer than one
+(``torch.nn.functional.normalize``): what a longer one writes can grow from token to
+token.
 """
 
 from __future__ import annotations
@@ -175,9 +177,10 @@ def delta_scan(
     (int32 on the GPU; None: all) are taken: what lies behind is not read, changes no
     state and gives zeros.
 
-    A gate of -inf forgets what came before, one of +inf keeps it whole.  From a k, v,
-    beta or gate that is not finite otherwise on, its head gives NaN.  Differentiable
-    in q, k, v, gate, beta and state."""
+    A gate of -inf forgets what came before, one of +inf keeps it whole; a beta of -inf
+    writes nothing, one of +inf with b = 1.  From a gate or beta that is NaN on, or a k or
+    v that is not finite, its head gives NaN.  Differentiable in q, k, v, gate, beta and
+    state."""
     # needs_input_grad does not know of no_grad, under which nothing is kept for a backward.
     backward = torch.is_grad_enabled() and any(
         t is not None and t.requires_grad for t in (q, k, v, gate, beta, state))
@@ -191,8 +194,10 @@ def delta_scan_step(
     """One token of each of ``batch`` streams: q and k [batch, key_heads, key_dim], v
     [batch, heads, dim], gate and beta [batch, heads], ``state`` float32 [batch, heads,
     key_dim, dim].  Returns ``(out, state)`` with the state after the token, written
-    to ``state_out`` where given (``state`` itself to step in place).  Not
-    differentiable; no host synchronisation, so a step can be captured in a graph."""
+    to ``state_out`` where given (``state`` itself to step in place).  Inputs that are
+    not finite go where the formula takes them: a v into its own column of the state,
+    for which :func:`delta_scan` gives up the head.  Not differentiable; no host
+    synchronisation, so a step can be captured in a graph."""
     if state is None:
         raise TypeError("delta_scan_step needs a state")
     problem = _problem(q, k, v, gate, beta, state, scale, 0)

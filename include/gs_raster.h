@@ -760,10 +760,11 @@ typedef struct gs_delta {
  * lengths[b] on (int32, device memory; NULL: all exist) change no state, are not read
  * as values and get zeros.  strides, host memory: batch, token and head stride in
  * elements of q, k, v, gate and beta (the backward: grad_out's after them); rows of q,
- * k, v and grad_out on 16-byte boundaries.  From a k, v, gate or beta that is not
- * finite on (gate may be infinite) outputs and states of its head are NaN; tokens
- * before it keep theirs.  States are float32 throughout.  The results do not depend on
- * the schedule.  With no token nothing is written. */
+ * k, v and grad_out on 16-byte boundaries.  From a k or v that is not finite on, or a
+ * gate or beta that is NaN (they may be infinite), outputs and states of its head are
+ * NaN; tokens before it keep theirs.  The recurrence, state and last are float32; kept
+ * holds what products of outputs and gradients take, in GS_BF16 in bfloat16.  The
+ * results do not depend on the schedule.  With no token nothing is written. */
 GS_API size_t gs_delta_scan_kept_bytes(const gs_delta* delta, int32_t backward);
 GS_API size_t gs_delta_scan_workspace_bytes(const gs_delta* delta);
 GS_API int gs_delta_scan_fwd(
@@ -788,7 +789,8 @@ GS_API int gs_delta_scan_bwd(
     void* workspace, size_t workspace_bytes, void* stream);
 
 /* One token of the rule (tokens is not read): all tensors contiguous, without the
- * token's dimension; state_out may be state. */
+ * token's dimension; state_out may be state.  What is not finite goes where the formula
+ * takes it. */
 GS_API int gs_delta_scan_step(
     const gs_delta* delta, const void* q, const void* k, const void* v,
     const void* gate, const void* beta, const float* state, void* out,
@@ -865,7 +867,8 @@ GS_API int gs_window_attention_step(
  * 127; 255: the block is NaN.  A block is encoded with the power floor(log2 max|x|)
  * - 2, not below -127, elements to the nearest code (ties to the even one, 6 beyond
  * 6); one with an infinity or a NaN becomes NaN.  The new token's key and value are
- * encoded, written and attended to as they are held. */
+ * encoded, written and attended to as they are held; out is rounded to its type once.
+ * GS_F16 holds every value of blocks that were made from it, not of all others. */
 GS_API size_t gs_window_attention_step_quant_workspace_bytes(const gs_attention* attention);
 GS_API int gs_window_attention_step_quant(
     const gs_attention* attention, const void* q, const void* k, const void* v,

@@ -540,3 +540,24 @@ def test_offsets_beyond_32_bits():
         results.append((out, last, *delta_scan_backward(*inputs, kept, do, None)))
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_step_not_finite(dtype):
+    """A step takes what is not finite where the formula does: a value into its column of
+    the state, a key, gate or beta into its head; all else keeps its bits."""
+    inputs = [t[:, 0].to(DEV) for t in _inputs(2, 1, 4, 2, 32, 40, dtype)]
+    state = normal((2, 4, 32, 40), torch.float32, 9).to(DEV)
+    want, new = delta_scan_step(*inputs, state)
+    for which, place in ((1, (0, 1, 3)), (2, (0, 2, 5)), (3, (0, 2)), (4, (0, 2))):
+        bad = [t.clone() for t in inputs]
+        bad[which][place] = float("nan")
+        out, end = delta_scan_step(*bad, state)
+        keep = torch.ones_like(want, dtype=torch.bool)
+        if which == 2:
+            keep[0, 2, 5] = False
+        else:
+            keep[0, 2:4 if which == 1 else 3] = False  # the key's two heads
+        assert out[~keep].isnan().all() and torch.equal(out[keep], want[keep])
+        there = keep[:, :, None].expand_as(end)
+        assert end[~there].isnan().all() and torch.equal(end[there], new[there])
